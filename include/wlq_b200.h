@@ -277,12 +277,81 @@ WLQ_API int wlq_gemv_last_warps(void);
 WLQ_API int wlq_gemv_set_overlap(int on);
 WLQ_API int wlq_gemv_get_overlap(void);
 
+/* ------------------------------------------------------- attention --- */
+/* What stands between the qkv and the o projection of a served decoder
+ * layer.  No counterpart in the reference, which leaves it to vLLM.
+ *
+ * Paged cache: k_cache and v_cache [num_pages, Hkv, page_size, D], page_size
+ * 16, 32, 64 or 128.  With k_exp = v_exp = NULL the values are in act_dtype;
+ * otherwise they are e4m3 codes and k_exp / v_exp ([num_pages, Hkv,
+ * page_size] bytes) hold e + 127 of each row's scale 2^e.  block_table int32
+ * [B, table_cols] names the pages of each sequence in order; entries past a
+ * sequence's length are never read, and a page outside the pool reads as
+ * zeros.  q, k, v and outputs are [T, heads, D] in act_dtype with D
+ * contiguous; their token and head strides (elements) are given, rows
+ * 16-byte aligned.  Query head h reads kv head h / (Hq / Hkv). */
+
+/* Rotary positions on q and k, and the cache write of k and v.  cos_sin
+ * [table_rows, rot] holds rot / 2 cosines then rot / 2 sines of every
+ * position, fp32 (frequencies and their scaling for long contexts are the
+ * table's matter); the first rot values of each head turn as pairs
+ * (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved.  rot and D multiples
+ * of 16, D <= 256.  slots[t] = page * page_size + offset; a slot outside the
+ * pool (negative: a padding token) is not written.  8-bit rows are quantised
+ * from the fp32 rotated values with e the smallest integer for which
+ * max|x| <= 448 * 2^e (in fp16 values beyond +-61440 are stored as that).
+ * q_out may be q; k_out (the rotated k, for wlq_prompt_attention) may be
+ * NULL.  A position outside the table sets WLQ_DEVERR_POSITION and leaves
+ * the token's outputs and slot as they were. */
+WLQ_API int wlq_rope_kv_write(const void* q, const void* k, const void* v, const int64_t* positions,
+             const float* cos_sin, const int64_t* slots, void* k_cache, void* v_cache, uint8_t* k_exp,
+             uint8_t* v_exp, void* q_out, void* k_out, int64_t q_tok, int64_t q_head, int64_t k_tok,
+             int64_t k_head, int64_t v_tok, int64_t v_head, int64_t qo_tok, int64_t qo_head, int64_t ko_tok,
+             int64_t ko_head, int64_t T, int64_t table_rows, int64_t num_pages, int Hq, int Hkv, int D, int rot,
+             int page_size, int interleaved, int act_dtype, wlq_stream_t stream);
+
+/* The cached k and v of whole sequences as packed act_dtype rows: k_out and
+ * v_out [T, Hkv, D] contiguous, sequence b in rows cu_lens[b] ..
+ * cu_lens[b + 1] (int32 [B + 1]), from its first token on. */
+WLQ_API int wlq_kv_read(const void* k_cache, const void* v_cache, const uint8_t* k_exp, const uint8_t* v_exp,
+             const int32_t* block_table, const int32_t* cu_lens, void* k_out, void* v_out, int64_t T, int B,
+             int64_t num_pages, int64_t table_cols, int Hkv, int D, int page_size, int act_dtype,
+             wlq_stream_t stream);
+
+/* softmax(scale q k^T) v of packed prompts: sequence b is rows cu_seqlens[b]
+ * .. cu_seqlens[b + 1] (int32 [B + 1], ascending, within T) of q, k, v and
+ * out; with causal a token sees the tokens up to itself, otherwise its whole
+ * sequence.  Statistics and sums in fp32, probabilities rounded to act_dtype
+ * for the tensor cores.  D 64 or 128.  Rows of no sequence are not written. */
+WLQ_API int wlq_prompt_attention(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, void* out,
+             int64_t q_tok, int64_t q_head, int64_t k_tok, int64_t k_head, int64_t v_tok, int64_t v_head,
+             int64_t o_tok, int64_t o_head, int64_t T, int B, int Hq, int Hkv, int D, float scale, int causal,
+             int act_dtype, wlq_stream_t stream);
+
+/* softmax(scale q k^T) v of each sequence's newest tokens over the paged
+ * cache, which holds them already: sequence b has kv_lens[b] cached tokens,
+ * of which the last n = cu_q[b + 1] - cu_q[b] are its rows of q; row i of
+ * them sees the tokens up to kv_lens[b] - n + i (a row that sees none is
+ * zeros).  cu_q NULL: one new token per sequence, T = B.  max_q is an upper
+ * bound of n.  `workspace` (wlq_paged_attention_workspace_bytes, 16-byte
+ * aligned, zero-filled before its first use, left zero where it has to be)
+ * joins the parts of sequences that several CTAs share; calls that share one
+ * must not overlap.  Results do not depend on timing. */
+WLQ_API size_t wlq_paged_attention_workspace_bytes(int64_t T, int B, int Hq, int Hkv, int D, int max_q);
+WLQ_API int wlq_paged_attention(const void* q, const void* k_cache, const void* v_cache, const uint8_t* k_exp,
+             const uint8_t* v_exp, const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_q, void* out,
+             int64_t q_tok, int64_t q_head, int64_t o_tok, int64_t o_head, int64_t T, int B, int Hq, int Hkv, int D,
+             int page_size, int64_t num_pages, int64_t table_cols, int max_q, float scale, int act_dtype,
+             void* workspace, size_t workspace_bytes, wlq_stream_t stream);
+
 /* Device error word of `device`: bit 0 (WLQ_DEVERR_WAIT_TIMEOUT) is set when
  * a pipeline wait inside a tensor-core GEMM kernel gave up (the kernel then
- * abandons its tile and its output is undefined).  Synchronous; clears the
+ * abandons its tile and its output is undefined), bit 1 (WLQ_DEVERR_POSITION)
+ * when wlq_rope_kv_write met a position outside its table.  Synchronous; clears the
  * word when `clear` is non-zero.  No reference counterpart: the reference
  * kernels have no bounded waits. */
 #define WLQ_DEVERR_WAIT_TIMEOUT 1u
+#define WLQ_DEVERR_POSITION 2u
 WLQ_API int wlq_device_error(int device, unsigned int* flags_out, int clear);
 
 /* ---------------------------------------------------------------- CPU --- */

@@ -45,6 +45,10 @@ int current_device(int* dev) {
     return WLQ_OK;
 }
 
+}  // namespace
+
+void clear_last_error() { g_last_error[0] = '\0'; }
+
 int require_sm100() {
     int dev = 0;
     int rc = current_device(&dev);
@@ -54,6 +58,8 @@ int require_sm100() {
                     g_cc_major[dev]);
     return WLQ_OK;
 }
+
+namespace {
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 

@@ -1,0 +1,913 @@
+// Attention of many query rows: 256 rows of one kv head against tiles of 128
+// keys on the tensor cores (tcgen05, scores and outputs in TMEM).
+//
+// With s_ij = q_i . k_j, o_i = sum_j 2^(c s_ij - M_i) v_j / sum_j 2^(c s_ij -
+// M_i), c = scale log2(e), the sums taken tile by tile with a running
+// reference M_i; both sums carry the same factor, so M_i only has to keep the
+// exponentials in range.  It is raised, and the output accumulator rescaled,
+// only when a row's maximum has grown by more than 2^8: the probabilities
+// then stay below 256, no precision is lost (they are floating-point numbers
+// and the sum is fp32), and after the first tiles the accumulator is hardly
+// ever touched.
+//
+// The rows of a CTA are the new tokens of one sequence times the G query
+// heads of one kv head, token-major, so that a short prompt or a chunk of few
+// tokens fills its tiles whatever G is, and every row of a tile needs about
+// the same keys.
+//
+// Roles (one CTA per SM):
+//   warps 0..3, 4..7  softmax of rows 0..127 and 128..255, a thread per row:
+//                     scores TMEM -> registers, maximum, exponentials, the
+//                     16-bit probabilities back into TMEM over the scores;
+//                     they load q at the start and write the output at the end
+//   warp 8            issues the MMAs: S = Q K^T (both from shared memory),
+//                     O += P V (P from TMEM).  The order P0 V, S0, P1 V, S1
+//                     lets the tensor cores work on one half's tiles while
+//                     the other half's softmax runs
+//   warp 9            TMA producer of the k and v tiles: packed rows, or one
+//                     copy per page
+//   warps 12..15      8-bit caches: the pages' codes land in a staging ring
+//                     and are written as the 16-bit tiles the MMAs read,
+//                     code * 2^e, which is exact
+//
+// Every mbarrier wait is bounded; a wait that runs out sets the device error
+// word and the CTA winds down, releasing its TMEM.
+#pragma once
+
+#include "wlq_attn.cuh"
+#include "wlq_internal.h"
+#include "wlq_sm100.cuh"
+
+namespace wlq {
+
+namespace {
+
+constexpr int kRowsT = 128;   // query rows of one tile (MMA M)
+constexpr int kRows = 256;    // query rows of one CTA
+constexpr int kKeys = 128;    // keys of one tile
+
+enum KvSource { kPacked = 0, kPaged = 1, kPaged8 = 2 };
+
+struct TileParams {
+    CUtensorMap tm_k, tm_v;
+    AttnParams a;
+    float* part;  // [split CTAs][kRows][D] unnormalised outputs of a part of the keys
+    float* stat;  // [split CTAs][kRows][2] their row maxima (times c) and sums
+    int sms;
+};
+
+template <int D, int SRC>
+struct TilePlan {
+    static constexpr int kHalves = D / 64;           // 128-byte-wide column blocks of a tile
+    static constexpr int kBlock = kKeys * 128;       // bytes of one block
+    static constexpr int kTileBytes = kBlock * kHalves;
+    static constexpr int kQBytes = 2 * kTileBytes;
+    static constexpr int kStageBytes = kKeys * D;    // 8-bit codes of one tile
+    static constexpr int kStages = SRC == kPaged8 ? 3 : 0;
+    static constexpr int kBudget = 227 * 1024 - 2048 - kQBytes - kStages * kStageBytes;
+    static constexpr int kFit = kBudget / kTileBytes;
+    static constexpr int kSlots = kFit > 8 ? 8 : kFit;
+    static constexpr int kKvOff = kQBytes;
+    static constexpr int kStageOff = kKvOff + kSlots * kTileBytes;
+    static constexpr int kBarOff = kStageOff + kStages * kStageBytes;
+    static constexpr int kAlloc = kBarOff + 512 + 1024;  // barriers, alignment slack
+    // registers a thread: the softmax groups hold a row's 128 scores; the
+    // groups' shares add up to what the block is launched with (168 x 3, 128 x 4)
+    static constexpr int kThreads = SRC == kPaged8 ? 512 : 384;
+    static constexpr int kRegsSoftmax = SRC == kPaged8 ? 184 : 208, kRegsOther = SRC == kPaged8 ? 72 : 88;
+    static_assert(2 * kRegsSoftmax + (kThreads / 128 - 2) * kRegsOther == 65536 / kThreads / 8 * 8 * (kThreads / 128),
+                  "register shares");
+    static_assert(kSlots >= 3, "k and v tiles in flight");
+};
+
+// What one CTA works on.
+struct Unit {
+    int b, hk;        // sequence, kv head
+    int row0, rows;   // its first row in the sequence, rows of the sequence
+    int first;        // first query token of the sequence in q
+    int past;         // keys a row of the first token does not count itself: row r sees keys <= past + r / G
+    int len;          // keys of the sequence
+    int tile0, tiles; // key tiles [tile0, tile0 + tiles)
+    int slot;         // partial result slot, or -1: the whole row is here
+};
+
+struct Seq {
+    int rows, tiles, rtiles, len, n, first;
+};
+
+template <bool PAGED>
+__device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
+    Seq s;
+    if (p.cu) {
+        s.first = p.cu[b];
+        s.n = p.cu[b + 1] - s.first;
+    } else {
+        s.first = b;
+        s.n = 1;
+    }
+    // rows outside q are nobody's
+    if (s.first < 0 || s.n < 0 || (int64_t)s.first + s.n > p.T) s.n = 0;
+    s.len = s.n;
+    if (PAGED) s.len = (int)max((int64_t)0, min((int64_t)p.kv_lens[b], p.table_cols << p.log2_page));
+    s.rows = s.n * p.G;
+    s.rtiles = (s.rows + kRows - 1) / kRows;
+    s.tiles = (s.len + kKeys - 1) / kKeys;
+    return s;
+}
+
+// Parts of a sequence's keys: as many CTAs as fill the device once, shared
+// out in proportion to the keys, none with less than 4 tiles.
+__device__ __forceinline__ int splits_of(const Seq& s, int64_t work, int sms) {
+    if (s.rtiles == 0) return 0;
+    const int most = (int)min((int64_t)s.tiles * sms / max(work, (int64_t)1), (int64_t)s.tiles / 4);
+    return max(1, most);
+}
+
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+// Key tiles times row tiles of all sequences (paged form), by one warp.
+__device__ __forceinline__ int64_t total_work(const AttnParams& p, int lane) {
+    int64_t w = 0;
+    for (int b = lane; b < p.B; b += 32) {
+        const Seq s = seq_of<true>(p, b);
+        w += (int64_t)s.rtiles * s.tiles;
+    }
+    return warp_sum(w) * p.Hkv;
+}
+
+// The work of CTA c, found by one warp: sequences in order, row tiles from
+// the last (the longest, where the mask is causal) to the first, then parts
+// of the keys, then heads.  False if there is none.
+template <bool PAGED>
+__device__ __forceinline__ bool find_unit(const AttnParams& p, int sms, int c, int lane, Unit& u) {
+    const int64_t work = PAGED ? total_work(p, lane) : 0;
+    int before = 0, slots = 0;  // CTAs of earlier sequences, those of them that hold parts
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+        const int b = b0 + lane;
+        Seq s{};
+        int sp = 0;
+        if (b < p.B) {
+            s = seq_of<PAGED>(p, b);
+            sp = PAGED ? splits_of(s, work, sms) : (s.rtiles ? 1 : 0);
+        }
+        const int mine = s.rtiles * sp * p.Hkv, part = sp > 1 ? mine : 0;
+        const int cum = warp_scan(mine, lane), pcum = warp_scan(part, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, c < before + cum);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            const int x = c - before - __shfl_sync(0xffffffffu, cum - mine, l);  // CTA within the sequence
+            const int slot0 = slots + __shfl_sync(0xffffffffu, pcum - part, l);
+            sp = __shfl_sync(0xffffffffu, sp, l);
+            s.rows = __shfl_sync(0xffffffffu, s.rows, l);
+            s.rtiles = __shfl_sync(0xffffffffu, s.rtiles, l);
+            s.tiles = __shfl_sync(0xffffffffu, s.tiles, l);
+            s.len = __shfl_sync(0xffffffffu, s.len, l);
+            s.n = __shfl_sync(0xffffffffu, s.n, l);
+            s.first = __shfl_sync(0xffffffffu, s.first, l);
+            u.b = b0 + l;
+            u.hk = x % p.Hkv;
+            const int y = x / p.Hkv;
+            const int part_no = y % sp;
+            u.row0 = (s.rtiles - 1 - y / sp) * kRows;
+            u.rows = s.rows;
+            u.first = s.first;
+            u.len = s.len;
+            u.past = s.len - s.n;
+            // keys the last row of the tile sees
+            const int last = (min(u.row0 + kRows, s.rows) - 1) / p.G;
+            const int seen = p.causal ? max(0, min(s.len, u.past + last + 1)) : s.len;
+            const int need = (seen + kKeys - 1) / kKeys;
+            const int per = (s.tiles + sp - 1) / sp;
+            u.tile0 = min(need, part_no * per);
+            u.tiles = min(need, u.tile0 + per) - u.tile0;
+            u.slot = sp > 1 ? slot0 + x : -1;
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, cum, 31);
+        slots += __shfl_sync(0xffffffffu, pcum, 31);
+    }
+    return false;
+}
+
+// mbar_wait by a whole warp, which goes on or gives up together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// ------------------------------------------------------------ tcgen05 extras
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// Descriptor of a tile stored as its transpose (the MMA's N contiguous): 128
+// key rows of 64 values in the 128-byte swizzle, 8-row atoms of 1024 bytes
+// along K, the next 64 columns of N one block further.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t block) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(block >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]: A is M x 16 16-bit values, two per column
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+          "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// Byte offset of 16-byte chunk c (of 8 values) of row r in a tile: blocks of
+// 64 columns, the chunk index XORed with row % 8 inside a 128-byte row (the
+// layout TMA writes and tcgen05 reads).
+__device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
+    return (uint32_t)((c >> 3) * (kKeys * 128) + r * 128 + (((c ^ r) & 7) << 4));
+}
+
+// Lane values of one cached or packed row in fp32 (E = D / 32 each).
+template <typename T, int D, int SRC>
+__device__ __forceinline__ void load_row(const AttnParams& p, const Unit& u, int j, bool v, int lane,
+                                         float (&f)[D / 32]) {
+    constexpr int E = D / 32;
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] = 0.f;
+    if constexpr (SRC == kPacked) {
+        const uint16_t* s = v ? p.v + (int64_t)(u.first + j) * p.v_tok + u.hk * p.v_head
+                              : p.k + (int64_t)(u.first + j) * p.k_tok + u.hk * p.k_head;
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = ActTraits<T>::bits_to_f32(s[lane * E + i]);
+    } else {
+        const int page = p.table[(int64_t)u.b * p.table_cols + (j >> p.log2_page)];
+        if (page < 0 || page >= p.num_pages) return;
+        const int64_t row = ((int64_t)page * p.Hkv + u.hk) * p.page_size + (j & (p.page_size - 1));
+        if constexpr (SRC == kPaged) {
+            const uint16_t* s = static_cast<const uint16_t*>(v ? p.v_cache : p.k_cache) + row * D;
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] = ActTraits<T>::bits_to_f32(s[lane * E + i]);
+        } else {
+            const uint8_t* s = static_cast<const uint8_t*>(v ? p.v_cache : p.k_cache) + row * D;
+            const float e = exp2_biased((v ? p.v_exp : p.k_exp)[row]);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                float g[4];
+                e4m3x4_to_f32(s[lane * E + i], g);
+                f[i] = g[0] * e;
+            }
+        }
+    }
+}
+
+// One row over its keys [j0, j1) without the tensor cores, by one warp.  A
+// tensor-core product multiplies the values of keys a row does not see by
+// zero; where those are infinite or NaN the product is NaN, and the row is
+// computed here instead.  m is in powers of two.
+template <typename T, int D, int SRC>
+__device__ __noinline__ void row_alone(const AttnParams& p, const Unit& u, int row, int j0, int j1, int lane,
+                                       float (&o)[D / 32], float& m, float& l) {
+    constexpr int E = D / 32;
+    const int h = u.hk * p.G + row % p.G;
+    const int64_t tok = u.first + row / p.G;
+    float q[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        q[i] = ActTraits<T>::bits_to_f32(p.q[tok * p.q_tok + h * p.q_head + lane * E + i]);
+        o[i] = 0.f;
+    }
+    m = -INFINITY;
+    l = 0.f;
+    for (int j = j0; j < j1; ++j) {
+        float k[E], v[E];
+        load_row<T, D, SRC>(p, u, j, false, lane, k);
+        load_row<T, D, SRC>(p, u, j, true, lane, v);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += q[i] * k[i];
+#pragma unroll
+        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        s *= p.scale_log2;
+        const float mn = fmaxf(m, s);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float c = exp2f(m - ref), e = exp2f(s - ref);
+        l = l * c + e;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = o[i] * c + e * v[i];
+        m = mn;
+    }
+}
+
+template <typename T, int D, int SRC>
+__global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kernel(const __grid_constant__ TileParams tp) {
+    using P = TilePlan<D, SRC>;
+    constexpr int NS = P::kSlots, NST = P::kStages;
+    constexpr bool kPagedSrc = SRC != kPacked;
+    const AttnParams& p = tp.a;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Unit su;
+    __shared__ int work_here;
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t sb = (raw + 1023u) & ~1023u;
+    uint8_t* sgen = smem_raw + (sb - raw);
+    const uint32_t bars = sb + P::kBarOff;
+    const uint32_t q_full = bars, v_fixed = bars + 8u;
+    auto s_full = [&](int t) { return bars + 8u * (2 + t); };    // scores of half t are in TMEM
+    auto p_full = [&](int t) { return bars + 8u * (4 + t); };    // its probabilities are
+    auto pv_done = [&](int t) { return bars + 8u * (6 + t); };   // its output has the tile's part
+    auto full = [&](int s) { return bars + 8u * (8 + s); };
+    auto empty = [&](int s) { return bars + 8u * (8 + NS + s); };
+    auto st_full = [&](int s) { return bars + 8u * (8 + 2 * NS + s); };
+    auto st_empty = [&](int s) { return bars + 8u * (8 + 2 * NS + NST + s); };
+    const uint32_t tmem_slot = bars + 8u * (8 + 2 * NS + 2 * NST);
+    auto slot = [&](int s) { return sb + P::kKvOff + s * P::kTileBytes; };
+    auto stage = [&](int s) { return sb + P::kStageOff + s * P::kStageBytes; };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0) {
+        Unit u;
+        const bool any = find_unit<kPagedSrc>(p, tp.sms, (int)blockIdx.x, lane, u);
+        if (lane == 0) {
+            su = u;
+            work_here = any;
+        }
+    }
+    if (threadIdx.x == 32) {
+        mbar_init(q_full, 8);
+        mbar_init(v_fixed, 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(s_full(t), 1);
+            mbar_init(p_full(t), 4);
+            mbar_init(pv_done(t), 1);
+        }
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(full(s), SRC == kPaged8 ? 4 : 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int s = 0; s < NST; ++s) {
+            mbar_init(st_full(s), 1);
+            mbar_init(st_empty(s), 4);
+        }
+        mbar_fence_init();
+        tma_prefetch_desc(&tp.tm_k);
+        tma_prefetch_desc(&tp.tm_v);
+    }
+    __syncthreads();
+    if (!work_here) return;
+    if (warp == 8) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sgen + P::kBarOff + (tmem_slot - bars));
+    const Unit u = su;
+    const int n = u.tiles;
+    const int halves = u.row0 + kRowsT < u.rows ? 2 : 1;
+    const int key0 = u.tile0 * kKeys;
+    // keys past the sequence's end in the last tile here
+    const int last_keys = min(kKeys, u.len - (key0 + (n - 1) * kKeys));
+
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::kRegsSoftmax));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::kRegsOther));
+
+    if (warp < 8) {
+        // ------------------------------------------------------- softmax
+        const int t = warp >> 2;
+        const int r = threadIdx.x;           // row of the CTA
+        const int row = u.row0 + r;          // row of the sequence
+        // q rows, 16 bytes a lane: a row's chunks are next to one another
+        {
+            constexpr int C = D / 8;
+            const int rt0 = t * kRowsT;
+            for (int i = threadIdx.x & 127; i < kRowsT * C; i += 128) {
+                const int rr = i / C, c = i % C;
+                const int rw = u.row0 + rt0 + rr;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (rw < u.rows) {
+                    const int tk = rw / p.G;
+                    const int h = u.hk * p.G + (rw - tk * p.G);
+                    v = ldg_stream_v4(p.q + (int64_t)(u.first + tk) * p.q_tok + h * p.q_head + c * 8);
+                }
+                sts128(sb + t * P::kTileBytes + tile_chunk(rr, c), v);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * D + lanes;
+        const float c = p.scale_log2;
+        // the row's last visible key, and the first one any row of the half cannot see
+        const int lim = p.causal ? min(u.len - 1, u.past + row / p.G) : u.len - 1;
+        const int lim0 = p.causal ? min(u.len - 1, u.past + (u.row0 + t * kRowsT) / p.G) : u.len - 1;
+        float m = -INFINITY;
+        uint64_t l2 = f2_pack(0.f, 0.f);
+        bool ok = true;
+        if (t < halves) {
+            for (int i = 0; i < n; ++i) {
+                if (!(ok = warp_wait(s_full(t), i & 1))) break;
+                tc_fence_after_sync();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(ts + 32 * k, s[k]);
+                tmem_ld_wait();
+                const int kb = key0 + i * kKeys;
+                if (kb + kKeys - 1 > lim0) {
+                    const int see = lim - kb;
+#pragma unroll
+                    for (int k = 0; k < 128; ++k)
+                        if (k > see) s[k >> 5][k & 31] = 0xff800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    mx[k] = __uint_as_float(s[k][0]);
+#pragma unroll
+                    for (int j = 1; j < 31; j += 2)
+                        mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(s[k][j]), __uint_as_float(s[k][j + 1])));
+                    mx[k] = fmaxf(mx[k], __uint_as_float(s[k][31]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
+                    const float mn = fmaxf(m, top);
+                    const float f = mn == m ? 1.f : ex2((m - mn) * c);
+                    m = mn;
+                    float la, lb;
+                    f2_unpack(l2, la, lb);
+                    l2 = f2_pack(la * f, lb * f);
+                    if (i > 0) {
+                        if (!(ok = warp_wait(pv_done(t), (i - 1) & 1))) break;
+                        tc_fence_after_sync();
+#pragma unroll 1
+                        for (int k = 0; k < D / 32; ++k) {
+                            uint32_t o[32];
+                            tmem_ld_32x32b_x32(to + 32 * k, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tmem_st_32x32b_x32(to + 32 * k, o);
+                        }
+                    }
+                }
+                const float neg = m == -INFINITY ? 0.f : -m * c;
+                const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(neg, neg);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const uint32_t* x = &s[2 * k + (j >> 4)][(2 * j) & 31];
+                        float a, b;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(x[0]), __uint_as_float(x[1])), c2, n2), a, b);
+                        a = ex2(a);
+                        b = ex2(b);
+                        l2 = f2_add(l2, f2_pack(a, b));
+                        w[j] = pack2<T>(a, b);
+                    }
+                    tmem_st_32x32b_x32(ts + 32 * k, w);
+                }
+                tmem_st_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(t));
+            }
+            // ------------------------------------------------------ output
+            float la, lb;
+            f2_unpack(l2, la, lb);
+            float l = la + lb;
+            if (n > 0 && ok) ok = warp_wait(pv_done(t), (n - 1) & 1);
+            tc_fence_after_sync();
+            const bool mine = row < u.rows;
+            const int tk = row / p.G, h = u.hk * p.G + (row - tk * p.G);
+            const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+            uint16_t* dst = p.out + (int64_t)(u.first + tk) * p.o_tok + h * p.o_head;
+            float* pdst = u.slot < 0 ? nullptr : tp.part + ((int64_t)u.slot * kRows + r) * D;
+            float bad = 0.f;
+#pragma unroll 1
+            for (int k = 0; k < D / 32; ++k) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld_32x32b_x32(to + 32 * k, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = 0u;
+                }
+                float f[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    f[j] = __uint_as_float(o[j]);
+                    bad = fmaf(f[j], 0.f, bad);  // NaN where a value is not finite
+                }
+                if (mine && pdst) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        *reinterpret_cast<float4*>(pdst + 32 * k + 4 * j) =
+                            make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                } else if (mine) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<uint4*>(dst + 32 * k + 8 * j) =
+                            make_uint4(pack2<T>(f[8 * j] * inv, f[8 * j + 1] * inv),
+                                       pack2<T>(f[8 * j + 2] * inv, f[8 * j + 3] * inv),
+                                       pack2<T>(f[8 * j + 4] * inv, f[8 * j + 5] * inv),
+                                       pack2<T>(f[8 * j + 6] * inv, f[8 * j + 7] * inv));
+                }
+                __syncwarp();
+            }
+            if (mine && pdst) {
+                float* st = tp.stat + ((int64_t)u.slot * kRows + r) * 2;
+                st[0] = m * c;
+                st[1] = l;
+            }
+            // rows that values behind the mask may have spoilt
+            const bool masked = key0 + n * kKeys - 1 > lim;
+            unsigned again = __ballot_sync(0xffffffffu, ok && mine && masked && bad != bad);
+            while (again) {
+                const int x = __ffs(again) - 1;
+                again &= again - 1;
+                const int rx = __shfl_sync(0xffffffffu, row, x);
+                const int j1 = __shfl_sync(0xffffffffu, lim, x) + 1;
+                float o[D / 32], mx, lx;
+                row_alone<T, D, SRC>(p, u, rx, key0, min(j1, key0 + n * kKeys), lane, o, mx, lx);
+                const int tx = rx / p.G, hx = u.hk * p.G + (rx - tx * p.G);
+                if (u.slot < 0) {
+                    const float ix = lx > 0.f ? 1.f / lx : (lx == lx ? 0.f : lx);
+                    uint16_t* d = p.out + (int64_t)(u.first + tx) * p.o_tok + hx * p.o_head + lane * (D / 32);
+#pragma unroll
+                    for (int j = 0; j < D / 32; j += 2)
+                        *reinterpret_cast<uint32_t*>(d + j) = pack2<T>(o[j] * ix, o[j + 1] * ix);
+                } else {
+                    const int64_t at = (int64_t)u.slot * kRows + (rx - u.row0);
+#pragma unroll
+                    for (int j = 0; j < D / 32; ++j) tp.part[at * D + lane * (D / 32) + j] = o[j];
+                    if (lane == 0) {
+                        tp.stat[at * 2] = mx;
+                        tp.stat[at * 2 + 1] = lx;
+                    }
+                }
+            }
+        }
+    } else if (warp == 8) {
+        // ------------------------------------------------------ MMA issue
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t fmt = ActTraits<T>::kIsF16 ? 0u : 1u;
+            constexpr uint32_t id_s = umma_idesc_f16(fmt, kRowsT, kKeys);
+            constexpr uint32_t id_o = umma_idesc_f16(fmt, kRowsT, D) | (1u << 16);  // V is stored with N contiguous
+            auto issue_s = [&](int t, int sl) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (uint32_t)((k >> 2) * P::kBlock + (k & 3) * 32);
+                    umma_f16(tmem + t * 128, umma_desc_sw128(sb + t * P::kTileBytes + off),
+                             umma_desc_sw128(slot(sl) + off), id_s, k > 0);
+                }
+            };
+            bool ok = mbar_wait(q_full, 0) && mbar_wait(full(0), 0);
+            tc_fence_after_sync();
+            if (ok) {
+                for (int t = 0; t < halves; ++t) {
+                    issue_s(t, 0);
+                    umma_commit(s_full(t));
+                }
+                umma_commit(empty(0));
+            }
+            // tiles arrive as K0 V0 K1 V1 ...
+            for (int i = 0; ok && i < n; ++i) {
+                const int gv = 2 * i + 1, sv = gv % NS, gk = gv + 1, sk = gk % NS;
+                if (!(ok = mbar_wait(full(sv), (gv / NS) & 1))) break;
+                if (SRC != kPaged8 && i == n - 1 && last_keys < kKeys && !(ok = mbar_wait(v_fixed, 0))) break;
+                for (int t = 0; ok && t < halves; ++t) {
+                    if (!(ok = mbar_wait(p_full(t), i & 1))) break;
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k,
+                                    umma_desc_mn_sw128(slot(sv) + k * 2048, P::kBlock), id_o, i > 0 || k > 0);
+                    umma_commit(pv_done(t));
+                    if (i + 1 < n) {
+                        if (t == 0 && !(ok = mbar_wait(full(sk), (gk / NS) & 1))) break;
+                        tc_fence_after_sync();
+                        issue_s(t, sk);
+                        umma_commit(s_full(t));
+                    }
+                }
+                if (ok) {
+                    umma_commit(empty(sv));
+                    if (i + 1 < n) umma_commit(empty(sk));
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // -------------------------------------------------- TMA producer
+        bool ok = true;
+        int g = 0;
+        constexpr int NR = SRC == kPaged8 ? NST : NS;
+        auto rfull = [&](int s) { return SRC == kPaged8 ? st_full(s) : full(s); };
+        auto rempty = [&](int s) { return SRC == kPaged8 ? st_empty(s) : empty(s); };
+        for (int i = 0; i < n && ok; ++i) {
+            const int kb = key0 + i * kKeys;
+            int z = 0, pages = 1;
+            if constexpr (kPagedSrc) {
+                // this lane's page of the tile; one outside the pool reads as zeros
+                const int ps = p.page_size;
+                pages = (min(kKeys, u.len - kb) + ps - 1) >> p.log2_page;
+                if (lane < pages) {
+                    const int id = p.table[(int64_t)u.b * p.table_cols + (kb >> p.log2_page) + lane];
+                    z = (id >= 0 && id < p.num_pages ? id : (int)p.num_pages) * p.Hkv + u.hk;
+                }
+            }
+            for (int kv = 0; kv < 2 && ok; ++kv, ++g) {
+                const int s = g % NR, use = g / NR;
+                if (use > 0 && !(ok = warp_wait(rempty(s), (use - 1) & 1))) break;
+                const CUtensorMap* map = kv ? &tp.tm_v : &tp.tm_k;
+                if constexpr (SRC == kPacked) {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(rfull(s), P::kTileBytes);
+#pragma unroll
+                        for (int h = 0; h < P::kHalves; ++h)
+                            tma_load_3d(slot(s) + h * P::kBlock, map, rfull(s), h * 64, u.hk, u.first + kb);
+                    }
+                } else {
+                    const int ps = p.page_size;
+                    if (lane == 0) mbar_arrive_expect_tx(rfull(s), pages * ps * (SRC == kPaged8 ? D : 2 * D));
+                    __syncwarp();
+                    if (lane < pages) {
+                        if constexpr (SRC == kPaged8) {
+                            tma_load_3d(stage(s) + lane * ps * D, map, rfull(s), 0, 0, z);
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < P::kHalves; ++h)
+                                tma_load_3d(slot(s) + h * P::kBlock + lane * ps * 128, map, rfull(s), h * 64, 0, z);
+                        }
+                    }
+                }
+            }
+        }
+        if (SRC != kPaged8 && ok && n > 0 && last_keys < kKeys) {
+            // v rows behind the sequence's end: zeros, as their probabilities are
+            const int gl = 2 * n - 1, s = gl % NS;
+            if ((ok = warp_wait(full(s), (gl / NS) & 1))) {
+                for (int x = last_keys * (D / 8) + lane; x < kKeys * (D / 8); x += 32)
+                    sts128(slot(s) + tile_chunk(x / (D / 8), x % (D / 8)), make_uint4(0u, 0u, 0u, 0u));
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_fixed);
+            }
+        }
+        // no copy may still be landing when the CTA exits
+        for (int j = g > NR ? g - NR : 0; j < g; ++j) mbar_wait(rfull(j % NR), (j / NR) & 1);
+    } else if constexpr (SRC == kPaged8) {
+        if (warp >= 12) {
+            // ------------------------------------------- codes -> 16-bit tiles
+            constexpr int C = D / 16;  // 16-code chunks of a row
+            const int tid = threadIdx.x - 384;
+            const int ch = tid % C, r0 = tid / C;
+            bool ok = true;
+            for (int i = 0; i < n && ok; ++i) {
+                const int kb = key0 + i * kKeys;
+                const int keys = min(kKeys, u.len - kb);
+                for (int kv = 0; kv < 2 && ok; ++kv) {
+                    const int g = 2 * i + kv, st = g % NST, s = g % NS;
+                    // the rows' scales, before the waits
+                    const uint8_t* exps = kv ? p.v_exp : p.k_exp;
+                    uint32_t e[C];
+#pragma unroll
+                    for (int x = 0; x < C; ++x) {
+                        const int r = r0 + x * (128 / C);
+                        e[x] = 0;
+                        if (r < keys) {
+                            const int id = p.table[(int64_t)u.b * p.table_cols + ((kb + r) >> p.log2_page)];
+                            if (id >= 0 && id < p.num_pages)
+                                e[x] = exps[((int64_t)id * p.Hkv + u.hk) * p.page_size + ((kb + r) & (p.page_size - 1))];
+                        }
+                    }
+                    if (!(ok = warp_wait(st_full(st), (g / NST) & 1))) break;
+                    if (g >= NS && !(ok = warp_wait(empty(s), (g / NS - 1) & 1))) break;
+#pragma unroll
+                    for (int x = 0; x < C; ++x) {
+                        const int r = r0 + x * (128 / C);
+                        uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+                        if (r < keys) {
+                            const uint4 q = lds128(stage(st) + r * D + ch * 16);
+                            const float sc = exp2_biased(e[x]);
+                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                            uint32_t o[8];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                float f[4];
+                                e4m3x4_to_f32(w[y], f);
+                                o[2 * y] = pack2<T>(f[0] * sc, f[1] * sc);
+                                o[2 * y + 1] = pack2<T>(f[2] * sc, f[3] * sc);
+                            }
+                            lo = make_uint4(o[0], o[1], o[2], o[3]);
+                            hi = make_uint4(o[4], o[5], o[6], o[7]);
+                        }
+                        sts128(slot(s) + tile_chunk(r, 2 * ch), lo);
+                        sts128(slot(s) + tile_chunk(r, 2 * ch + 1), hi);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(full(s));
+                        mbar_arrive(st_empty(st));
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the parts of the sequences whose keys several CTAs shared: block x
+// takes 256 / gridDim.y rows of the x-th such row tile, a warp per row.  The
+// parts are added in the order of the keys.
+constexpr int kJoinThreads = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) attn_tile_join_kernel(const __grid_constant__ TileParams tp) {
+    const AttnParams& p = tp.a;
+    __shared__ int sh[6];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0) {
+        const int64_t work = total_work(p, lane);
+        int before = 0, slots = 0, found = 0;
+        for (int b0 = 0; b0 < p.B && !found; b0 += 32) {
+            const int b = b0 + lane;
+            Seq s{};
+            int sp = 0;
+            if (b < p.B) {
+                s = seq_of<true>(p, b);
+                sp = splits_of(s, work, tp.sms);
+            }
+            const int mine = sp > 1 ? s.rtiles * p.Hkv : 0;
+            const int cum = warp_scan(mine, lane), scum = warp_scan(mine * sp, lane);
+            const unsigned hit = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + cum);
+            if (hit) {
+                found = 1;
+                if (lane == __ffs(hit) - 1) {
+                    const int x = (int)blockIdx.x - before - (cum - mine);
+                    const int hk = x % p.Hkv, rt = x / p.Hkv;
+                    sh[0] = slots + scum - mine * sp + rt * sp * p.Hkv + hk;  // slot of the first part
+                    sh[1] = sp;
+                    sh[2] = (s.rtiles - 1 - rt) * kRows;
+                    sh[3] = s.rows;
+                    sh[4] = s.first;
+                    sh[5] = hk;
+                }
+            }
+            before += __shfl_sync(0xffffffffu, cum, 31);
+            slots += __shfl_sync(0xffffffffu, scum, 31);
+        }
+        if (!found && lane == 0) sh[1] = 0;
+    }
+    __syncthreads();
+    const int sp = sh[1];
+    if (sp == 0) return;
+    const int slot = sh[0], row0 = sh[2], rows = sh[3], first = sh[4], hk = sh[5];
+    constexpr int E = D / 32;
+    for (int r = blockIdx.y * 8 + warp; r < min(kRows, rows - row0); r += gridDim.y * 8) {
+        float m = -INFINITY, l = 0.f, o[E];
+        for (int s = 0; s < sp; ++s) m = fmaxf(m, tp.stat[((int64_t)(slot + s * p.Hkv) * kRows + r) * 2]);
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] = 0.f;
+        for (int s = 0; s < sp; ++s) {
+            const int64_t at = (int64_t)(slot + s * p.Hkv) * kRows + r;
+            const float2 st = *reinterpret_cast<const float2*>(tp.stat + at * 2);
+            const float f = exp2f(st.x - ref);
+            l += st.y * f;
+            if (st.x == -INFINITY && st.y == 0.f) continue;  // a part the row saw nothing of
+#pragma unroll
+            for (int j = 0; j < E; ++j) o[j] += tp.part[at * D + lane * E + j] * f;
+        }
+        const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+        const int tk = (row0 + r) / p.G, h = hk * p.G + (row0 + r) % p.G;
+        uint16_t* d = p.out + (int64_t)(first + tk) * p.o_tok + h * p.o_head + lane * E;
+#pragma unroll
+        for (int j = 0; j < E; j += 2) *reinterpret_cast<uint32_t*>(d + j) = pack2<T>(o[j] * inv, o[j + 1] * inv);
+    }
+}
+
+template <typename T, int D, int SRC>
+int launch_tile(const AttnParams& a, cudaStream_t stream) {
+    using P = TilePlan<D, SRC>;
+    TileParams tp;
+    tp.a = a;
+    tp.sms = device_sm_count();
+    int rc;
+    constexpr bool f16 = ActTraits<T>::kIsF16;
+    const CUtensorMapDataType dt = SRC == kPaged8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : f16          ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if constexpr (SRC == kPacked) {
+        // a single kv head's stride is never used
+        const uint64_t kh = a.Hkv == 1 ? D * 2 : a.k_head * 2, vh = a.Hkv == 1 ? D * 2 : a.v_head * 2;
+        const uint64_t kt = a.T == 1 ? D * 2 : a.k_tok * 2, vt = a.T == 1 ? D * 2 : a.v_tok * 2;
+        if ((rc = encode_3d(&tp.tm_k, dt, a.k, D, a.Hkv, a.T, kh, kt, 64, 1, kKeys, CU_TENSOR_MAP_SWIZZLE_128B, "k")) ||
+            (rc = encode_3d(&tp.tm_v, dt, a.v, D, a.Hkv, a.T, vh, vt, 64, 1, kKeys, CU_TENSOR_MAP_SWIZZLE_128B, "v")))
+            return rc;
+    } else {
+        constexpr int es = SRC == kPaged8 ? 1 : 2;
+        const uint64_t pg = (uint64_t)a.num_pages * a.Hkv, ps = a.page_size;
+        const CUtensorMapSwizzle sw = SRC == kPaged8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+        const uint32_t box = SRC == kPaged8 ? D : 64;
+        if ((rc = encode_3d(&tp.tm_k, dt, a.k_cache, D, ps, pg, D * es, ps * D * es, box, ps, 1, sw, "k_cache")) ||
+            (rc = encode_3d(&tp.tm_v, dt, a.v_cache, D, ps, pg, D * es, ps * D * es, box, ps, 1, sw, "v_cache")))
+            return rc;
+    }
+    tp.part = static_cast<float*>(a.ws);
+    tp.stat = tp.part + (size_t)tp.sms * kRows * D;
+    const int64_t grid = (a.T * a.G / kRows + a.B) * a.Hkv + (SRC == kPacked ? 0 : tp.sms);
+    if (grid > 0x7fffffff) return fail(WLQ_ERR_UNSUPPORTED, "attention: %lld row tiles in one call", (long long)grid);
+    static const cudaError_t attr = cudaFuncSetAttribute(attn_tile_kernel<T, D, SRC>,
+                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, P::kAlloc);
+    if (attr != cudaSuccess) return check_cuda(attr, "attn_tile_kernel shared memory");
+    attn_tile_kernel<T, D, SRC><<<(unsigned)grid, P::kThreads, P::kAlloc, stream>>>(tp);
+    if ((rc = check_cuda(cudaGetLastError(), "attn_tile_kernel"))) return rc;
+    if constexpr (SRC != kPacked) {
+        attn_tile_join_kernel<T, D><<<dim3(tp.sms / 2, 8), kJoinThreads, 0, stream>>>(tp);
+        rc = check_cuda(cudaGetLastError(), "attn_tile_join_kernel");
+    }
+    return rc;
+}
+
+template <typename T>
+int launch_tile_any(const AttnParams& a, cudaStream_t stream) {
+    if (!a.k_cache) return a.D == 64 ? launch_tile<T, 64, kPacked>(a, stream) : launch_tile<T, 128, kPacked>(a, stream);
+    if (a.k_exp) return a.D == 64 ? launch_tile<T, 64, kPaged8>(a, stream) : launch_tile<T, 128, kPaged8>(a, stream);
+    return a.D == 64 ? launch_tile<T, 64, kPaged>(a, stream) : launch_tile<T, 128, kPaged>(a, stream);
+}
+
+}  // namespace
+
+}  // namespace wlq

@@ -944,12 +944,14 @@ int read_device_error(int device, unsigned int* flags, int clear) {
     cudaError_t e = cudaGetDevice(&prev);
     if (e != cudaSuccess) return check_cuda(e, "cudaGetDevice");
     if (device != prev && (e = cudaSetDevice(device)) != cudaSuccess) return check_cuda(e, "cudaSetDevice");
-    // only this translation unit's kernels wait on mbarriers
-    unsigned int v = 0;
-    const int rc = tu_device_error(&v, clear);
+    unsigned int v = 0, tile16 = 0, tilebf = 0, position = 0;
+    int rc = tu_device_error(&v, clear);
+    if (!rc) rc = attn_tile_error_f16(&tile16, clear);
+    if (!rc) rc = attn_tile_error_bf16(&tilebf, clear);
+    if (!rc) rc = rope_position_error(&position, clear);
     if (device != prev) cudaSetDevice(prev);
     if (rc) return rc;
-    *flags = v;
+    *flags = v | tile16 | tilebf | (position ? WLQ_DEVERR_POSITION : 0u);
     return WLQ_OK;
 }
 

@@ -14,6 +14,11 @@ int fail(int code, const char* fmt, ...);
 // Maps a CUDA error to WLQ_ERR_CUDA with its name, or returns WLQ_OK.
 int check_cuda(cudaError_t e, const char* what);
 
+// Empties this thread's last error (every entry point does so first).
+void clear_last_error();
+// WLQ_OK where the current device is one this build runs on (sm_100).
+int require_sm100();
+
 // Arguments of one quantized-linear call, already validated.
 struct LinearArgs {
     const uint32_t* q;       // [N * wpr]
@@ -89,6 +94,23 @@ int launch_dequant(const uint32_t* q, const uint16_t* lut, uint16_t* W, const in
                    int group_size, int group_offset, int ngroups, int chunk_m, int ncsr,
                    cudaStream_t stream);
 
+// The attention operators (wlq_attn.cuh has their arguments).
+struct RopeParams;
+struct KvReadParams;
+struct AttnParams;
+int launch_rope_kv_write(RopeParams& p, bool f16, bool quant, cudaStream_t stream);
+int launch_kv_read(KvReadParams& p, bool f16, bool quant, cudaStream_t stream);
+int launch_attention(const AttnParams& p, bool f16, cudaStream_t stream);
+size_t attention_workspace_bytes(int64_t T, int B, int Hq, int Hkv, int D, int max_q);
+int launch_attn_tile_f16(const AttnParams& p, cudaStream_t stream);
+int launch_attn_tile_bf16(const AttnParams& p, cudaStream_t stream);
+// The device error words of their translation units, on the current device.
+int attn_tile_error_f16(unsigned int* flags, int clear);
+int attn_tile_error_bf16(unsigned int* flags, int clear);
+// Reads (and optionally clears) the current device's flag of a rope_kv_write
+// position outside the cos/sin table.
+int rope_position_error(unsigned int* flag, int clear);
+
 // Reads (and optionally clears) the device error word of `device`.
 int read_device_error(int device, unsigned int* flags, int clear);
 
@@ -97,6 +119,11 @@ int read_device_error(int device, unsigned int* flags, int clear);
 // WLQ_ERR_CUDA.  Loads past the array's edges read zeros.
 int encode_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
               uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz, const char* what);
+
+// 3-D tensor map of 16-byte aligned rows of d0 elements (strides in bytes).
+int encode_3d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
+              uint64_t stride1, uint64_t stride2, uint32_t b0, uint32_t b1, uint32_t b2, CUtensorMapSwizzle swz,
+              const char* what);
 
 // Multiprocessor count of the current device (cached per device).
 int device_sm_count();

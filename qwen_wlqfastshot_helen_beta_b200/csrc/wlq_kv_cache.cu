@@ -1,0 +1,312 @@
+// The paged k/v cache of an attention layer: rotary positions with the
+// cache write (rope_kv_write_kernel) and the read-back (kv_read_kernel).
+//
+// Cache layout: [pages, kv_heads, page_size, D], one head's tokens of a page
+// contiguous, so that an attention kernel fetches a page of one head as one
+// 2-D tile.  16-bit caches hold the activation type.  8-bit caches hold e4m3
+// codes and one byte e + 127 per row of D codes, e the smallest integer with
+// max|x| <= 448 * 2^e.  The scale is a power of two on purpose: code * 2^e is
+// a bf16 number (and an fp16 one in fp16's range), so whoever reads the cache
+// dequantises into tensor-core operands without rounding a second time, and a
+// floating format loses nothing to the coarse scale (its relative step does
+// not depend on it).
+//
+// Both kernels are HBM-bound: every value is read once and written once.
+#include <cuda_fp8.h>
+
+#include "wlq_attn.cuh"
+#include "wlq_common.cuh"
+#include "wlq_internal.h"
+
+namespace wlq {
+
+namespace {
+
+constexpr int kRopeThreads = 128;
+constexpr int kReadThreads = 256;
+
+// Set when a token's position lies outside the cos/sin table; the token's
+// outputs are then left as they were.
+static __device__ unsigned int g_position_error = 0;
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4 w, float (&f)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = ActTraits<T>::bits_to_f32((uint16_t)u[i]);
+        f[2 * i + 1] = ActTraits<T>::bits_to_f32((uint16_t)(u[i] >> 16));
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+    return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
+
+// A warp takes one token (its cos/sin values stay in registers) and walks
+// part of the token's heads, 32 / G rows at a time: G lanes share a row, each
+// with two 8-value chunks that hold both members of its pairs.  Few tokens
+// spread their heads over several warps (`parts`), so that a decoding step is
+// one round of loads.
+template <typename T, bool QUANT>
+__global__ void __launch_bounds__(kRopeThreads) rope_kv_write_kernel(const RopeParams p) {
+    const int lane = threadIdx.x & 31;
+    const int64_t w = (int64_t)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
+    const int64_t tok = w / p.parts;
+    if (tok >= p.T) return;
+    const int64_t pos = p.positions[tok];
+    const int64_t slot = p.slots[tok];
+    if (pos < 0 || pos >= p.table_rows) {
+        if (lane == 0) atomicOr(&g_position_error, 1u);
+        return;
+    }
+    const bool store = slot >= 0 && slot < p.num_pages * p.page_size;  // a negative slot: a padding token
+    const int64_t page = store ? slot / p.page_size : 0;
+    const int off = store ? (int)(slot - page * p.page_size) : 0;
+
+    const int G = p.lanes_per_row, rows = 32 / G;
+    const int l = lane & (G - 1), sub = lane / G;
+    const bool live = 16 * l < p.D;  // D / 16 lanes work where G is rounded up
+    const int nrot = p.rot >> 3;     // chunks that are rotated
+    int ca, cb;                      // this lane's chunks
+    if (p.interleaved) {
+        ca = l;
+        cb = l + (p.D >> 4);
+    } else if (l < nrot / 2) {
+        ca = l;
+        cb = l + nrot / 2;
+    } else {
+        ca = nrot + 2 * (l - nrot / 2);
+        cb = ca + 1;
+    }
+    // interleaved: 4 pairs of each chunk; halves: 8 pairs across the chunks
+    float cs[8], sn[8];
+    const float* row = p.cos_sin + pos * p.rot;
+    const bool turn_a = live && ca < nrot, turn_b = live && cb < nrot;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
+    {
+        const int ia = p.interleaved ? 4 * ca : 8 * ca, ib = p.interleaved ? 4 * cb : 8 * ca + 4;
+        if (turn_a) {
+            const float4 c = *reinterpret_cast<const float4*>(row + ia);
+            const float4 s = *reinterpret_cast<const float4*>(row + p.rot / 2 + ia);
+            cs[0] = c.x, cs[1] = c.y, cs[2] = c.z, cs[3] = c.w;
+            sn[0] = s.x, sn[1] = s.y, sn[2] = s.z, sn[3] = s.w;
+        }
+        if (turn_b) {
+            const float4 c = *reinterpret_cast<const float4*>(row + ib);
+            const float4 s = *reinterpret_cast<const float4*>(row + p.rot / 2 + ib);
+            cs[4] = c.x, cs[5] = c.y, cs[6] = c.z, cs[7] = c.w;
+            sn[4] = s.x, sn[5] = s.y, sn[6] = s.z, sn[7] = s.w;
+        }
+    }
+
+    const int heads = p.Hq + 2 * p.Hkv;
+    const int part = (int)(w - tok * p.parts);
+    for (int h0 = part * rows; h0 < heads; h0 += p.parts * rows) {
+        const int h = h0 + sub;
+        const bool ok = live && h < heads;
+        const int kind = h < p.Hq ? 0 : (h < p.Hq + p.Hkv ? 1 : 2);  // q, k, v
+        const int hh = kind == 0 ? h : (kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv);
+        float a[8], b[8];
+        if (ok) {
+            const uint16_t* src = kind == 0   ? p.q + tok * p.q_tok + hh * p.q_head
+                                  : kind == 1 ? p.k + tok * p.k_tok + hh * p.k_head
+                                              : p.v + tok * p.v_tok + hh * p.v_head;
+            unpack8<T>(ldg_stream_v4(src + 8 * ca), a);
+            unpack8<T>(ldg_stream_v4(src + 8 * cb), b);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+        }
+        if (kind != 2) {
+            if (p.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], t = b[2 * i + 1];
+                    if (turn_a) {
+                        a[2 * i] = x * cs[i] - y * sn[i];
+                        a[2 * i + 1] = y * cs[i] + x * sn[i];
+                    }
+                    if (turn_b) {
+                        b[2 * i] = z * cs[4 + i] - t * sn[4 + i];
+                        b[2 * i + 1] = t * cs[4 + i] + z * sn[4 + i];
+                    }
+                }
+            } else if (turn_a) {  // both chunks are rotated, or neither
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = a[i], y = b[i];
+                    a[i] = x * cs[i] - y * sn[i];
+                    b[i] = y * cs[i] + x * sn[i];
+                }
+            }
+        }
+        if (kind == 0) {
+            if (ok) {
+                uint16_t* d = p.q_out + tok * p.qo_tok + hh * p.qo_head;
+                *reinterpret_cast<uint4*>(d + 8 * ca) = pack8<T>(a);
+                *reinterpret_cast<uint4*>(d + 8 * cb) = pack8<T>(b);
+            }
+        } else if (kind == 1 && p.k_out && ok) {
+            uint16_t* d = p.k_out + tok * p.ko_tok + hh * p.ko_head;
+            *reinterpret_cast<uint4*>(d + 8 * ca) = pack8<T>(a);
+            *reinterpret_cast<uint4*>(d + 8 * cb) = pack8<T>(b);
+        }
+        if (!store) continue;  // uniform over the warp
+        const int64_t crow = (page * p.Hkv + hh) * p.page_size + off;
+        if constexpr (QUANT) {
+            if (ActTraits<T>::kIsF16) {
+                // the largest e4m3 grid value below 65504, so that what is read back stays finite in fp16
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    a[i] = fminf(fmaxf(a[i], -61440.f), 61440.f);
+                    b[i] = fminf(fmaxf(b[i], -61440.f), 61440.f);
+                }
+            }
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(a[i]), fabsf(b[i])));
+            for (int d = 1; d < G; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            // top = m 2^x with m in [1, 2) and 448 = 1.75 * 2^8
+            const uint32_t bits = __float_as_uint(top);
+            const int e = max(1, (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));  // + 127
+            const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+            if (ok && kind != 0) {
+                uint8_t* d = reinterpret_cast<uint8_t*>(kind == 1 ? p.k_cache : p.v_cache) + crow * p.D;
+                *reinterpret_cast<uint2*>(d + 8 * ca) =
+                    make_uint2(e4m3x4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv),
+                               e4m3x4(a[4] * inv, a[5] * inv, a[6] * inv, a[7] * inv));
+                *reinterpret_cast<uint2*>(d + 8 * cb) =
+                    make_uint2(e4m3x4(b[0] * inv, b[1] * inv, b[2] * inv, b[3] * inv),
+                               e4m3x4(b[4] * inv, b[5] * inv, b[6] * inv, b[7] * inv));
+                if (l == 0) (kind == 1 ? p.k_exp : p.v_exp)[crow] = (uint8_t)e;
+            }
+        } else if (ok && kind != 0) {
+            uint16_t* d = reinterpret_cast<uint16_t*>(kind == 1 ? p.k_cache : p.v_cache) + crow * p.D;
+            *reinterpret_cast<uint4*>(d + 8 * ca) = pack8<T>(a);
+            *reinterpret_cast<uint4*>(d + 8 * cb) = pack8<T>(b);
+        }
+    }
+}
+
+// A CTA reads back `tokens` consecutive rows of the packed output, all heads
+// of k then of v: the first threads look the rows' cache slots up, then every
+// thread moves one 8-value chunk per step (8 codes in, 16 bytes out; a warp's
+// stores are 512 contiguous bytes).  Rows outside the table or the pool are
+// zeros.
+template <typename T, bool QUANT>
+__global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const KvReadParams p) {
+    __shared__ int64_t base[kReadTokens];  // cache row of head 0, or -1
+    const int64_t t0 = (int64_t)blockIdx.x * p.tokens;
+    const int nt = (int)min((int64_t)p.tokens, p.T - t0);
+    if ((int)threadIdx.x < nt) {
+        const int64_t t = t0 + threadIdx.x;
+        int lo = 0, hi = p.B;  // last sequence with cu[lo] <= t
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.cu[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        const int64_t pos = t - p.cu[lo];
+        const int64_t pg = pos / p.page_size;
+        int64_t r = -1;
+        if (pos >= 0 && t < p.cu[lo + 1] && pg < p.table_cols) {
+            const int id = p.table[(int64_t)lo * p.table_cols + pg];
+            if (id >= 0 && id < p.num_pages) r = (int64_t)id * p.Hkv * p.page_size + (pos - pg * p.page_size);
+        }
+        base[threadIdx.x] = r;
+    }
+    __syncthreads();
+    const int per = p.Hkv * (p.D >> 3);  // chunks of one token
+    const int n = nt * per;
+    for (int which = 0; which < 2; ++which) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(which ? p.v_cache : p.k_cache);
+        const uint8_t* exps = which ? p.v_exp : p.k_exp;
+        uint16_t* dst = (which ? p.v_out : p.k_out) + t0 * per * 8;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += kReadThreads) {
+            const int tk = __umulhi((uint32_t)i, p.per_magic);
+            const int e = i - tk * per;
+            const int h = __umulhi((uint32_t)e, p.chunk_magic);
+            const int c = e - h * (p.D >> 3);
+            const int64_t r = base[tk];
+            uint4 o = make_uint4(0u, 0u, 0u, 0u);
+            if (r >= 0) {
+                const int64_t row = r + (int64_t)h * p.page_size;
+                if constexpr (QUANT) {
+                    const uint2 q = ldg_stream_v2(src + row * p.D + 8 * c);
+                    const float s = exp2_biased(exps[row]);
+                    float f[8];
+                    e4m3x4_to_f32(q.x, f);
+                    e4m3x4_to_f32(q.y, f + 4);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] *= s;
+                    o = pack8<T>(f);
+                } else {
+                    o = ldg_stream_v4(src + (row * p.D + 8 * c) * 2);
+                }
+            }
+            *reinterpret_cast<uint4*>(dst + (int64_t)i * 8) = o;
+        }
+    }
+}
+
+// q = i / d for i < n as a multiply-high, exact while n * d < 2^32
+uint32_t magic_u32(uint32_t d) { return d == 1 ? 0u : (uint32_t)((0x100000000ull + d - 1) / d); }
+
+}  // namespace
+
+int launch_rope_kv_write(RopeParams& p, bool f16, bool quant, cudaStream_t stream) {
+    p.lanes_per_row = 1;
+    while (p.lanes_per_row * 16 < p.D) p.lanes_per_row <<= 1;
+    const int steps = (p.Hq + 2 * p.Hkv + 32 / p.lanes_per_row - 1) / (32 / p.lanes_per_row);
+    // enough warps for 16 per SM before a warp walks several steps
+    const int64_t want = (int64_t)device_sm_count() * 16;
+    p.parts = (int)std::min<int64_t>(steps, std::max<int64_t>(1, (want + p.T - 1) / p.T));
+    const int64_t warps = p.T * p.parts;
+    const unsigned grid = (unsigned)((warps + kRopeThreads / 32 - 1) / (kRopeThreads / 32));
+    if (f16)
+        quant ? rope_kv_write_kernel<__half, true><<<grid, kRopeThreads, 0, stream>>>(p)
+              : rope_kv_write_kernel<__half, false><<<grid, kRopeThreads, 0, stream>>>(p);
+    else
+        quant ? rope_kv_write_kernel<__nv_bfloat16, true><<<grid, kRopeThreads, 0, stream>>>(p)
+              : rope_kv_write_kernel<__nv_bfloat16, false><<<grid, kRopeThreads, 0, stream>>>(p);
+    return check_cuda(cudaGetLastError(), "rope_kv_write_kernel");
+}
+
+int launch_kv_read(KvReadParams& p, bool f16, bool quant, cudaStream_t stream) {
+    // a few tokens per CTA until every SM has some
+    p.tokens = p.T >= (int64_t)device_sm_count() * 2 * kReadTokens ? kReadTokens : 8;
+    p.per_magic = magic_u32((uint32_t)(p.Hkv * (p.D >> 3)));
+    p.chunk_magic = magic_u32((uint32_t)(p.D >> 3));
+    const unsigned grid = (unsigned)((p.T + p.tokens - 1) / p.tokens);
+    if (f16)
+        quant ? kv_read_kernel<__half, true><<<grid, kReadThreads, 0, stream>>>(p)
+              : kv_read_kernel<__half, false><<<grid, kReadThreads, 0, stream>>>(p);
+    else
+        quant ? kv_read_kernel<__nv_bfloat16, true><<<grid, kReadThreads, 0, stream>>>(p)
+              : kv_read_kernel<__nv_bfloat16, false><<<grid, kReadThreads, 0, stream>>>(p);
+    return check_cuda(cudaGetLastError(), "kv_read_kernel");
+}
+
+// Reads (and with `clear` zeroes) the position error of the current device.
+int rope_position_error(unsigned int* flag, int clear) {
+    unsigned int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_position_error, sizeof(v));
+    if (e == cudaSuccess && clear && v) {
+        const unsigned int z = 0;
+        e = cudaMemcpyToSymbol(g_position_error, &z, sizeof(z));
+    }
+    if (e != cudaSuccess) return check_cuda(e, "position error word");
+    *flag = v;
+    return WLQ_OK;
+}
+
+}  // namespace wlq

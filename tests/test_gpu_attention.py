@@ -1,0 +1,486 @@
+"""The attention operators on the GPU against plain 64-bit forms, at the sizes
+and masks where they can go wrong."""
+import os
+import sys
+import zlib
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import _attention as R  # noqa: E402
+from _gpu import C  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+BOTH = [torch.float16, torch.bfloat16]
+
+
+def gen_of(*key):
+    return torch.Generator(device="cuda").manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def randn(gen, *shape):
+    return torch.randn(shape, generator=gen, device="cuda")
+
+
+def table_of(rows, rot):
+    from qwen_wlqfastshot_helen_beta_b200.attention import rope_table
+    return rope_table(rows, rot, device="cuda")
+
+
+# ------------------------------------------------------------ rope + cache ---
+
+ROPE = [  # T, Hq, Hkv, D, rot, interleaved, page, strided
+    (1, 28, 4, 128, 128, False, 16, False),
+    (33, 28, 4, 128, 128, False, 16, True),
+    (300, 14, 2, 64, 64, True, 32, True),
+    (7, 5, 5, 64, 32, False, 64, False),
+    (19, 6, 3, 96, 48, True, 128, True),
+    (5, 3, 1, 80, 32, False, 16, False),
+    (4, 2, 1, 256, 64, True, 16, False),
+    (3, 2, 2, 16, 16, False, 16, False),
+    (6, 4, 2, 48, 0, False, 16, True),
+    (5000, 8, 1, 128, 64, False, 16, True),
+]
+
+
+def rope_inputs(case, dtype, bits):
+    T, Hq, Hkv, D, rot, inter, page, strided = case
+    g = gen_of("rope", T, Hq, D, rot, bits)
+    if strided:
+        qkv = (randn(g, T, (Hq + 2 * Hkv) * D + 16) * R.log2_spread(g, (T, 1))).to(dtype)
+        q, k, v, _ = (x for x in qkv.split([Hq * D, Hkv * D, Hkv * D, 16], 1))
+        q, k, v = (x.view(T, -1, D) for x in (q, k, v))
+    else:
+        q, k, v = ((randn(g, T, h, D) * R.log2_spread(g, (T, 1, 1))).to(dtype) for h in (Hq, Hkv, Hkv))
+    rows = 2 * T + 5
+    pos = torch.randint(0, rows, (T,), generator=g, device="cuda")
+    pages = -(-T // page) + 2
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:T]
+    return g, q, k, v, pos, slots, rows, pages
+
+
+@pytest.mark.parametrize("case", ROPE, ids=str)
+@pytest.mark.parametrize("dtype", BOTH, ids=str)
+@pytest.mark.parametrize("bits", [16, 8])
+def test_rope_kv_write(case, dtype, bits):
+    T, Hq, Hkv, D, rot, inter, page, strided = case
+    g, q, k, v, pos, slots, rows, pages = rope_inputs(case, dtype, bits)
+    cs = table_of(rows, max(rot, 16))[:, :rot].contiguous()
+    if T > 3:
+        slots[2], slots[3] = -1, pages * page + 3  # a padding token, a slot past the pool
+        k[1] = 0  # a row of zeros
+    stored = dtype if bits == 16 else torch.float8_e4m3fn
+    kc, vc = (torch.full((pages, Hkv, page, D), 3.0, device="cuda").to(stored) for _ in range(2))
+    ke = ve = None
+    if bits == 8:
+        ke, ve = (torch.full((pages, Hkv, page), 77, dtype=torch.uint8, device="cuda") for _ in range(2))
+    q_out = torch.full_like(q, float("nan")).contiguous()
+    k_out = torch.full_like(k, float("nan")).contiguous()
+    C().rope_kv_write(q, k, v, pos, cs, slots, kc, vc, q_out, k_out, ke, ve, inter)
+    turn = cs[pos]
+    # a product and a sum in fp32 (2^-23 of either term's size), then one rounding
+    size = lambda x: x.double().abs().amax(-1, keepdim=True) * 2  # noqa: E731
+    qr, kr = R.rotate(q.double(), turn, inter), R.rotate(k.double(), turn, inter)
+    for got, ref, src in ((q_out, qr, q), (k_out, kr, k)):
+        tol = R.UNIT[dtype] * ref.abs() + 2.0 ** -22 * size(src) + 2.0 ** -25
+        assert ((got.double() - ref).abs() <= tol).all()
+    kept = (slots >= 0) & (slots < pages * page)
+    at = slots[kept]
+    for cache, exp, ref, src, exact in ((kc, ke, kr, k, rot == 0), (vc, ve, v.double(), v, True)):
+        rows_ = cache.transpose(1, 2).reshape(-1, Hkv, D)
+        untouched = torch.ones(pages * page, dtype=torch.bool, device="cuda")
+        untouched[at] = False
+        assert (rows_[untouched].float() == 3.0).all(), "a slot that was not given changed"
+        got, ref, slack = rows_[at].double(), ref[kept], 2.0 ** -22 * size(src[kept])
+        if bits == 16:
+            if exact:
+                assert (got == src[kept].double()).all()
+            tol = R.UNIT[dtype] * ref.abs() + slack + 2.0 ** -25
+            assert ((got - ref).abs() <= tol).all()
+            continue
+        e = exp.transpose(1, 2).reshape(-1, Hkv)[at].long() - 127
+        assert (exp.transpose(1, 2).reshape(-1, Hkv)[untouched] == 77).all()
+        # the scale is the smallest that holds the row, with fp32's slack on its largest value
+        low, high = R.exponents(ref.abs().sub(slack).clamp(min=0)), R.exponents(ref.abs() + slack * (not exact))
+        assert ((e >= (high if exact else low)) & (e <= high)).all()
+        scale = torch.exp2(e.double())[..., None]
+        want, margin = R.nearest(ref / scale, R.e4m3_grid("cuda"))
+        sure = margin * 2.0 ** -9 > slack / scale if not exact else margin > 0
+        assert (got[sure] == want[sure]).all()
+        # half a step (a sixteenth of the value, or 2^-10 of the scale) and the slack
+        assert ((got * scale - ref).abs() <= ref.abs() / 16 + 2.0 ** -10 * scale + slack).all()
+
+
+def test_rope_in_place_and_position_error():
+    g = gen_of("inplace")
+    T, Hq, Hkv, D = 9, 4, 2, 128
+    q, k, v = (randn(g, T, h, D).bfloat16() for h in (Hq, Hkv, Hkv))
+    cs = table_of(64, D)
+    pos, slots = torch.arange(T, device="cuda"), torch.arange(T, device="cuda")
+    kc, vc = (torch.zeros(2, Hkv, 16, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    want = torch.empty_like(q)
+    C().rope_kv_write(q, k, v, pos, cs, slots, kc, vc, want)
+    again = q.clone()
+    C().rope_kv_write(again, k, v, pos, cs, slots, kc, vc, again)
+    assert torch.equal(again, want) and C().device_error() == 0
+    pos[4] = 64
+    out = torch.full_like(q, 5.0)
+    kc.zero_()
+    C().rope_kv_write(q, k, v, pos, cs, slots, kc, vc, out)
+    assert (out[4] == 5.0).all() and (kc.transpose(1, 2).reshape(-1, Hkv, D)[4] == 0).all()
+    keep = [i for i in range(T) if i != 4]
+    assert torch.equal(out[keep], want[keep])
+    assert C().device_error() == 2 and C().device_error() == 0
+
+
+def test_rope_fp16_largest_values_stay_finite():
+    k = torch.full((1, 1, 64), 65504.0, device="cuda", dtype=torch.float16)
+    kc, vc = (torch.zeros(1, 1, 16, 64, device="cuda").to(torch.float8_e4m3fn) for _ in range(2))
+    ke, ve = (torch.zeros(1, 1, 16, dtype=torch.uint8, device="cuda") for _ in range(2))
+    pos = torch.zeros(1, dtype=torch.int64, device="cuda")
+    C().rope_kv_write(k, k, -k, pos, table_of(4, 64), pos, kc, vc, torch.empty_like(k), None, ke, ve)
+    ko, vo = (torch.empty(1, 1, 64, device="cuda", dtype=torch.float16) for _ in range(2))
+    tab, cu = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    C().kv_read(kc, vc, tab, cu, ko, vo, ke, ve)
+    assert (ko == 61440).all() and (vo == -61440).all()
+
+
+# -------------------------------------------------------------------- read ---
+
+def make_cache(g, pages, Hkv, page, D, dtype, bits, spread=True):
+    """A cache of random values; 8-bit: random codes with exponents around -6."""
+    if bits == 16:
+        c = [randn(g, pages, Hkv, page, D).to(dtype) for _ in range(2)]
+        return c + [None, None]
+    c = [(randn(g, pages, Hkv, page, D) * 100).clamp(-448, 448).to(torch.float8_e4m3fn) for _ in range(2)]
+    e = [torch.randint(127 - 9 if spread else 127 - 7, 127 - 4 if spread else 127 - 6, (pages, Hkv, page), generator=g,
+                       device="cuda").to(torch.uint8) for _ in range(2)]
+    return c + e
+
+
+@pytest.mark.parametrize("lens", [[1], [16, 17], [0, 5, 0, 130], [997], [64] * 5, [40000, 3]], ids=str)
+@pytest.mark.parametrize("bits,page,Hkv,D", [(8, 16, 4, 128), (16, 32, 2, 64), (8, 128, 1, 80), (8, 64, 3, 256),
+                                             (16, 16, 7, 16)])
+@pytest.mark.parametrize("dtype", BOTH, ids=str)
+def test_kv_read(lens, bits, page, Hkv, D, dtype):
+    g = gen_of("read", bits, page, D, *lens)
+    table, pages = R.pages_of(lens, page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, dtype, bits)
+    T = sum(lens)
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0).to(torch.int32)
+    ko, vo = (torch.full((T, Hkv, D), float("nan"), device="cuda", dtype=dtype) for _ in range(2))
+    C().kv_read(kc, vc, table, cu, ko, vo, ke, ve)
+    for got, cache, exp in ((ko, kc, ke), (vo, vc, ve)):
+        want = torch.cat([R.gather(cache, exp, table, i, n) for i, n in enumerate(lens)])
+        assert torch.equal(got.double(), want)  # code * 2^e needs no rounding
+
+
+def test_kv_read_missing_pages_are_zeros():
+    g = gen_of("missing")
+    kc, vc, _, _ = make_cache(g, 3, 2, 16, 64, torch.bfloat16, 16)
+    table = torch.tensor([[1, -1], [5, 2]], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 40, 72], dtype=torch.int32, device="cuda")  # 40 rows of a table that holds 32
+    ko, vo = (torch.full((72, 2, 64), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    C().kv_read(kc, vc, table, cu, ko, vo)
+    assert torch.equal(ko[:16], kc[1].transpose(0, 1)) and torch.equal(vo[56:], vc[2].transpose(0, 1))
+    assert (ko[16:56] == 0).all() and (vo[16:56] == 0).all()
+
+
+# ------------------------------------------------------------------ prompt ---
+
+PROMPT = [  # lens, Hq, Hkv, D
+    ([1], 4, 2, 128), ([2, 1, 3], 28, 4, 128), ([0, 5, 0, 0, 33, 0], 14, 2, 64), ([127, 128, 129], 2, 1, 128),
+    ([256, 255, 257], 1, 1, 64), ([37, 130, 1, 64], 14, 2, 64), ([300], 28, 4, 128), ([513, 90], 3, 3, 128),
+    ([700], 16, 1, 64), ([19] * 40, 6, 2, 128),
+]
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv,D", PROMPT, ids=str)
+@pytest.mark.parametrize("dtype", BOTH, ids=str)
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_attention(lens, Hq, Hkv, D, dtype, causal):
+    g = gen_of("prompt", D, Hq, *lens)
+    T = sum(lens)
+    qkv = randn(g, T + 3, (Hq + 2 * Hkv) * D).to(dtype)
+    qkv[T:] = float("nan")  # rows of no sequence
+    q, k, v = (x.view(T + 3, -1, D) for x in qkv.split([Hq * D, Hkv * D, Hkv * D], 1))
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0).to(torch.int32)
+    out = torch.full((T + 3, Hq, D), 9.0, device="cuda", dtype=dtype)
+    C().prompt_attention(q, k, v, cu, out, causal=causal)
+    assert C().device_error() == 0
+    assert (out[T:] == 9.0).all(), "rows of no sequence were written"
+    at = 0
+    for n in lens:
+        r = slice(at, at + n)
+        R.check(out[r], *R.attention(q[r].double(), k[r].double(), v[r].double(), 1 if causal else None, R.scale_of(D)))
+        at += n
+    again = torch.empty_like(out)
+    C().prompt_attention(q, k, v, cu, again, causal=causal)
+    assert torch.equal(again[:T], out[:T])
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=str)
+def test_prompt_attention_other_sequences_do_not_leak(dtype):
+    """Infinities and NaN of one sequence stay in it."""
+    g = gen_of("leak")
+    lens, Hq, Hkv, D = [70, 50, 200], 4, 2, 128
+    q, k, v = (randn(g, sum(lens), h, D).to(dtype) for h in (Hq, Hkv, Hkv))
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0).to(torch.int32)
+    clean = torch.empty_like(q)
+    C().prompt_attention(q, k, v, cu, clean)
+    k[70:120], v[70:100], v[100:120] = float("inf"), float("nan"), float("-inf")
+    out = torch.empty_like(q)
+    C().prompt_attention(q, k, v, cu, out)
+    assert torch.equal(out[:70], clean[:70]) and torch.equal(out[120:], clean[120:])
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")], ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_attention_later_tokens_do_not_leak(D, bad):
+    """A row does not see the k and v of tokens after it, whatever they are."""
+    g = gen_of("later", D)
+    n, Hq, Hkv = 200, 6, 2
+    q, k, v = (randn(g, n, h, D).bfloat16() for h in (Hq, Hkv, Hkv))
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    k[150:], v[150:] = bad, bad
+    C().prompt_attention(q, k, v, cu, out)
+    R.check(out[:150], *R.attention(q[:150].double(), k[:150].double(), v[:150].double(), 1, R.scale_of(D)))
+    assert not torch.isfinite(out[150:]).any()
+
+
+def test_prompt_attention_large_scores():
+    """Scores of +-thousands: the running maximum keeps the exponentials in range."""
+    g = gen_of("large")
+    n, H, D = 300, 2, 64
+    q, k, v = (randn(g, n, H, D).bfloat16() for _ in range(3))
+    q = (q.float() * 40 * torch.linspace(-1, 1, n, device="cuda")[:, None, None]).bfloat16()
+    k = (k.float() * torch.linspace(0.1, 40, n, device="cuda")[:, None, None]).bfloat16()
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    C().prompt_attention(q, k, v, cu, out)
+    R.check(out, *R.attention(q.double(), k.double(), v.double(), 1, R.scale_of(D)))
+
+
+def test_prompt_attention_strides_and_streams():
+    """Heads first in memory, an out with gaps, another stream."""
+    g = gen_of("strides")
+    n, Hq, Hkv, D = 140, 4, 2, 64
+    q, k, v = (randn(g, h, n + 8, D).half()[:, 4:n + 4].transpose(0, 1) for h in (Hq, Hkv, Hkv))
+    cu = torch.tensor([0, 60, n], dtype=torch.int32, device="cuda")
+    buf = torch.full((n, Hq, 2 * D), 7.0, device="cuda", dtype=torch.float16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        C().prompt_attention(q, k, v, cu, buf[..., :D], 0.3)
+    torch.cuda.current_stream().wait_stream(side)
+    assert (buf[..., D:] == 7.0).all()
+    for a, b in ((0, 60), (60, n)):
+        R.check(buf[a:b, :, :D], *R.attention(q[a:b].double(), k[a:b].double(), v[a:b].double(), 1, 0.3))
+
+
+# ------------------------------------------------------------------- paged ---
+
+PAGED = [  # kv_lens, new tokens, Hq, Hkv, D, page
+    ([1], [1], 28, 4, 128, 16), ([5, 1, 17], [1, 1, 1], 8, 1, 128, 16), ([63, 64, 65, 200], [1] * 4, 14, 2, 64, 32),
+    ([1501], [1], 28, 4, 128, 16), ([3000, 1, 129], [1, 1, 1], 4, 4, 64, 128), ([5000], [1], 16, 1, 128, 64),
+    ([70] * 30, [1] * 30, 32, 8, 128, 16), ([40, 300], [2, 2], 6, 1, 128, 16), ([130, 50], [3, 1], 4, 1, 64, 64),
+    ([20, 700, 129], [20, 5, 100], 14, 2, 64, 16), ([300, 33, 257], [40, 33, 1], 28, 4, 128, 16),
+    ([260], [129], 2, 1, 128, 32), ([1000], [37], 7, 1, 64, 128), ([128, 256], [128, 2], 1, 1, 128, 16),
+    ([2600, 20], [9, 20], 8, 2, 128, 16), ([400], [300], 3, 3, 64, 32), ([6000], [17], 2, 1, 128, 128),
+]
+
+
+@pytest.mark.parametrize("lens,new,Hq,Hkv,D,page", PAGED, ids=str)
+@pytest.mark.parametrize("dtype", BOTH, ids=str)
+@pytest.mark.parametrize("bits", [16, 8])
+def test_paged_attention(lens, new, Hq, Hkv, D, page, dtype, bits):
+    g = gen_of("paged", D, Hq, bits, *lens)
+    table, pages = R.pages_of(lens, page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, dtype, bits)
+    # what lies behind a sequence's last token in its page is not looked at
+    nan = torch.tensor(0x7f, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) if bits == 8 else float("nan")
+    for i, n in enumerate(lens):
+        if n % page:
+            for c in (kc, vc):
+                tail = c[table[i, n // page].long(), :, n % page:]
+                (tail.view(torch.uint8).fill_(0x7f) if bits == 8 else tail.fill_(nan))
+            if bits == 8:
+                for e in (ke, ve):
+                    e[table[i, n // page].long(), :, n % page:] = 255
+    T = sum(new)
+    q = randn(g, T, Hq, D).to(dtype)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0] + new, device="cuda").cumsum(0).to(torch.int32)
+    single = max(new) == 1
+    out = torch.full_like(q, float("nan"))
+    for _ in range(2):  # the workspace serves a second call
+        out.fill_(float("nan"))
+        C().paged_attention(q, kc, vc, table, kv_lens, out, None if single else cu, max(new), ke, ve)
+    assert C().device_error() == 0
+    at = 0
+    for i, (m, n) in enumerate(zip(lens, new)):
+        k, v = R.gather(kc, ke, table, i, m), R.gather(vc, ve, table, i, m)
+        R.check(out[at:at + n], *R.attention(q[at:at + n].double(), k, v, m - n + 1, R.scale_of(D)))
+        at += n
+    again = torch.empty_like(out)
+    C().paged_attention(q, kc, vc, table, kv_lens, again, None if single else cu, max(new), ke, ve)
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("max_q", [4, 60])
+def test_paged_attention_rows_that_see_nothing(max_q):
+    """Empty caches, more new tokens than cached ones, sequences without new tokens."""
+    g = gen_of("nothing")
+    Hq, Hkv, D, page = 4, 2, 64, 16
+    lens, new = [0, 2, 50, 0], [3, 4, 0, 1]
+    if max_q == 60:
+        lens, new = [0, 2, 50, 10], [3, 60, 0, 12]
+    table, pages = R.pages_of([max(n, 1) for n in lens], page, g)
+    kc, vc, _, _ = make_cache(g, pages, Hkv, page, D, torch.float16, 16)
+    q = randn(g, sum(new), Hq, D).half()
+    cu = torch.tensor([0] + new, device="cuda").cumsum(0).to(torch.int32)
+    out = torch.full_like(q, float("nan"))
+    C().paged_attention(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), out, cu, max_q)
+    at = 0
+    for i, (m, n) in enumerate(zip(lens, new)):
+        k, v = R.gather(kc, None, table, i, m), R.gather(vc, None, table, i, m)
+        R.check(out[at:at + n], *R.attention(q[at:at + n].double(), k, v, m - n + 1, R.scale_of(D)))
+        assert (out[at:at + max(0, n - m)] == 0).all()
+        at += n
+    # one token each, some sequences empty
+    one = torch.full((4, Hq, D), float("nan"), device="cuda", dtype=torch.float16)
+    C().paged_attention(q[:4], kc, vc, table, torch.tensor([0, 1, 0, 2], dtype=torch.int32, device="cuda"), one)
+    assert (one[0] == 0).all() and (one[2] == 0).all() and torch.isfinite(one).all()
+    assert (one[1] == R.gather(vc, None, table, 1, 1)[0].half().repeat_interleave(2, 0)).all()
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_paged_attention_scales_far_apart(new):
+    """8-bit rows whose scales differ by 2^40, rows of zeros, scores that grow along the sequence."""
+    g = gen_of("far", new)
+    Hq, Hkv, D, page, n = 7, 1, 128, 16, 700
+    table, pages = R.pages_of([n], page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, torch.bfloat16, 8)
+    ve.copy_(torch.randint(87, 128, ve.shape, generator=g, device="cuda").to(torch.uint8))
+    vc.view(torch.uint8)[table[0, 3].long()] = 0
+    ve[table[0, 3].long()] = 1
+    ke.copy_(torch.where(torch.arange(page, device="cuda") % 5 == 0, 123, 119).to(torch.uint8))
+    q = randn(g, new, Hq, D).bfloat16()
+    cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    C().paged_attention(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda"), out, cu, new, ke, ve)
+    k, v = R.gather(kc, ke, table, 0, n), R.gather(vc, ve, table, 0, n)
+    R.check(out, *R.attention(q.double(), k, v, n - new + 1, R.scale_of(D)))
+
+
+def test_paged_attention_large_q_values():
+    """bf16 queries beyond fp16's range over an 8-bit cache."""
+    g = gen_of("largeq")
+    Hq, D, page, n = 4, 128, 16, 100
+    table, pages = R.pages_of([n], page, g)
+    kc, vc, ke, ve = make_cache(g, pages, 1, page, D, torch.bfloat16, 8)
+    ke -= 60
+    q = (randn(g, 1, Hq, D) * 2.0 ** 60).bfloat16()
+    q[0, 1] = 0
+    out = torch.full_like(q, float("nan"))
+    C().paged_attention(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda"), out, None, 1, ke, ve)
+    k, v = R.gather(kc, ke, table, 0, n), R.gather(vc, ve, table, 0, n)
+    R.check(out, *R.attention(q.double(), k, v, n, R.scale_of(D)))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_paged_attention_missing_pages(new):
+    """A page outside the pool reads as zeros, entries past the table end the sequence."""
+    g = gen_of("pool", new)
+    Hq, D, page = 4, 128, 16
+    kc, vc, _, _ = make_cache(g, 6, 1, page, D, torch.bfloat16, 16)
+    table = torch.tensor([[1, 6, -3, 2]], dtype=torch.int32, device="cuda")
+    q = randn(g, new, Hq, D).bfloat16()
+    cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    C().paged_attention(q, kc, vc, table, torch.tensor([100], dtype=torch.int32, device="cuda"), out, cu, new)
+    z = torch.zeros(32, 1, D, device="cuda", dtype=torch.float64)
+    k, v = (torch.cat((c[1].transpose(0, 1).double(), z, c[2].transpose(0, 1).double())) for c in (kc, vc))
+    R.check(out, *R.attention(q.double(), k, v, 64 - new + 1, R.scale_of(D)))
+
+
+@pytest.mark.parametrize("new", [2, 50])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_paged_attention_later_tokens_do_not_leak(new, bits):
+    g = gen_of("plater", new, bits)
+    Hq, Hkv, D, page, n = 6, 2, 128, 16, 170
+    table, pages = R.pages_of([n], page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, torch.bfloat16, bits)
+    q = randn(g, new, Hq, D).bfloat16()
+    cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    C().paged_attention(q, kc, vc, table, lens, clean, cu, new, ke, ve)
+    late = table[0, (n - 1) // page].long()
+    for c in (kc, vc):  # the last token
+        row = c[late, :, (n - 1) % page]
+        row.view(torch.uint8).fill_(0x7f) if bits == 8 else row.fill_(float("nan"))
+    C().paged_attention(q, kc, vc, table, lens, out, cu, new, ke, ve)
+    R.check(out[:-1], *R.attention(q[:-1].double(), R.gather(kc, ke, table, 0, n - 1),
+                                   R.gather(vc, ve, table, 0, n - 1), n - new + 1, R.scale_of(D)))
+    assert torch.isnan(out[-1].float()).all()
+
+
+def test_paged_attention_past_32_bits():
+    """A pool whose values pass 2^32: the last pages are read where they are."""
+    g = gen_of("wide")
+    Hkv, D, page, n = 1, 128, 128, 500
+    pages = (1 << 32) // (Hkv * page * D) + 8
+    kc, vc = (torch.zeros(pages, Hkv, page, D, device="cuda", dtype=torch.float16) for _ in range(2))
+    for c in (kc, vc):
+        c[-4:] = randn(g, 4, Hkv, page, D).half()
+    table = torch.tensor([[pages - 2, pages - 4, pages - 1, pages - 3]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    k, v = R.gather(kc, None, table, 0, n), R.gather(vc, None, table, 0, n)
+    for new in (1, 20):
+        q = randn(g, new, 4, D).half()
+        cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+        out = torch.full_like(q, float("nan"))
+        C().paged_attention(q, kc, vc, table, lens, out, cu, new)
+        R.check(out, *R.attention(q.double(), k, v, n - new + 1, R.scale_of(D)))
+    ko, vo = (torch.empty(n, Hkv, D, device="cuda", dtype=torch.float16) for _ in range(2))
+    C().kv_read(kc, vc, table, torch.tensor([0, n], dtype=torch.int32, device="cuda"), ko, vo)
+    assert torch.equal(ko.double(), k) and torch.equal(vo.double(), v)
+
+
+def test_paged_attention_streams_and_graph():
+    """Calls on two streams at once and a replayed graph agree with a plain call."""
+    g = gen_of("graph")
+    Hq, Hkv, D, page, lens = 28, 4, 128, 16, [3000, 800, 2]
+    table, pages = R.pages_of(lens, page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, torch.bfloat16, 8)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = randn(g, 3, Hq, D).bfloat16()
+    want = torch.empty_like(q)
+    C().paged_attention(q, kc, vc, table, kv_lens, want, None, 1, ke, ve)
+    torch.cuda.synchronize()
+    outs = [torch.empty_like(q) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for o, s in zip(outs, streams):
+            with torch.cuda.stream(s):
+                C().paged_attention(q, kc, vc, table, kv_lens, o, None, 1, ke, ve)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(q)
+    with torch.cuda.graph(graph):
+        C().paged_attention(q, kc, vc, table, kv_lens, out, None, 1, ke, ve)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        C().paged_attention(q, kc, vc, table, kv_lens, outs[0], None, 1, ke, ve)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(outs[0], want)
+    kv_lens.copy_(torch.tensor([5, 700, 1], dtype=torch.int32))  # the graph follows the lengths
+    graph.replay()
+    torch.cuda.synchronize()
+    for i, n in enumerate([5, 700, 1]):
+        k, v = R.gather(kc, ke, table, i, n), R.gather(vc, ve, table, i, n)
+        R.check(out[i:i + 1], *R.attention(q[i:i + 1].double(), k, v, n, R.scale_of(D)))
