@@ -333,11 +333,14 @@ WLQ_API int wlq_prompt_attention(const void* q, const void* k, const void* v, co
  * of which the last n = cu_q[b + 1] - cu_q[b] are its rows of q; row i of
  * them sees the tokens up to kv_lens[b] - n + i (a row that sees none is
  * zeros).  cu_q NULL: one new token per sequence, T = B.  max_q is an upper
- * bound of n.  `workspace` (wlq_paged_attention_workspace_bytes, 16-byte
- * aligned, zero-filled before its first use, left zero where it has to be)
- * joins the parts of sequences that several CTAs share; calls that share one
- * must not overlap.  Results do not depend on timing. */
-WLQ_API size_t wlq_paged_attention_workspace_bytes(int64_t T, int B, int Hq, int Hkv, int D, int max_q);
+ * bound of n.  `workspace` (device memory of
+ * wlq_paged_attention_workspace_bytes on the current device, 16-byte aligned,
+ * its first WLQ_ATTENTION_ZERO_BYTES zero before the first use and left zero
+ * by every call) joins the parts of sequences that several CTAs share; calls
+ * that share one must not overlap.  B * Hkv is at most
+ * WLQ_ATTENTION_ZERO_BYTES / 4.  Results do not depend on timing. */
+#define WLQ_ATTENTION_ZERO_BYTES (256u * 1024u)
+WLQ_API size_t wlq_paged_attention_workspace_bytes(int Hq, int Hkv, int D, int max_q);
 WLQ_API int wlq_paged_attention(const void* q, const void* k_cache, const void* v_cache, const uint8_t* k_exp,
              const uint8_t* v_exp, const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_q, void* out,
              int64_t q_tok, int64_t q_head, int64_t o_tok, int64_t o_head, int64_t T, int B, int Hq, int Hkv, int D,

@@ -496,20 +496,20 @@ def prompt_attention(q, k, v, cu_seqlens, out, scale=None, causal=True):
 # Workspaces of paged_attention, one per device and stream (calls on several
 # streams may overlap), grown when a call needs more and kept for the process.
 _ATTN_WS = {}
+_ATTN_ZERO_BYTES = 256 * 1024  # WLQ_ATTENTION_ZERO_BYTES
 
 
 def attention_workspace(dev, stream, nbytes):
     """This stream's workspace.  While a CUDA graph is captured the graph gets
     one of its own, from its memory pool: a replay may overlap later calls on
     the stream that captured it."""
-    if nbytes == 0:
-        return None
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-    ws = _ATTN_WS.get((dev.index, stream))
+    capturing = torch.cuda.is_current_stream_capturing()
+    ws = None if capturing else _ATTN_WS.get((dev.index, stream))
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-        _ATTN_WS[(dev.index, stream)] = ws
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws[:_ATTN_ZERO_BYTES].zero_()
+        if not capturing:
+            _ATTN_WS[(dev.index, stream)] = ws
     return ws
 
 
@@ -538,12 +538,12 @@ def paged_attention(q, k_cache, v_cache, block_table, kv_lens, out, cu_q=None, m
     max_q = int(max_q)
     with _DeviceGuard(dev):
         stream = _raw_stream(dev)
-        ws = attention_workspace(dev, stream, lib.wlq_paged_attention_workspace_bytes(T, B, Hq, Hkv, D, max_q))
+        ws = attention_workspace(dev, stream, lib.wlq_paged_attention_workspace_bytes(Hq, Hkv, D, max_q))
         rc = lib.wlq_paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _addr(k_exp), _addr(v_exp),
                                      block_table.data_ptr(), kv_lens.data_ptr(), _addr(cu_q), out.data_ptr(), *sq,
                                      *so, T, B, Hq, Hkv, D, ps, pages, block_table.shape[1], max_q,
-                                     D ** -0.5 if scale is None else float(scale), dt, _addr(ws),
-                                     0 if ws is None else ws.numel(), stream)
+                                     D ** -0.5 if scale is None else float(scale), dt, ws.data_ptr(), ws.numel(),
+                                     stream)
     check(rc, "wlq_paged_attention")
 
 

@@ -61,7 +61,7 @@ SIGNATURES = {
     "wlq_rope_kv_write": (_i32, [_p] * 12 + [_i64] * 13 + [_i32] * 7 + [_p]),
     "wlq_kv_read": (_i32, [_p] * 8 + [_i64, _i32, _i64, _i64, _i32, _i32, _i32, _i32, _p]),
     "wlq_prompt_attention": (_i32, [_p] * 5 + [_i64] * 9 + [_i32, _i32, _i32, _i32, _f32, _i32, _i32, _p]),
-    "wlq_paged_attention_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "wlq_paged_attention_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32]),
     "wlq_paged_attention": (_i32, [_p] * 9 + [_i64] * 5 + [_i32] * 5 + [_i64, _i64, _i32, _f32, _i32, _p,
                                                                        ctypes.c_size_t, _p]),
     "wlq_words_per_row": (_i64, [_i64, _i32]),

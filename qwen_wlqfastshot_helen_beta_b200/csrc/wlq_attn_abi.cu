@@ -159,9 +159,9 @@ int wlq_prompt_attention(const void* q, const void* k, const void* v, const int3
     return launch_attention(p, act_dtype == WLQ_DTYPE_F16, static_cast<cudaStream_t>(stream));
 }
 
-size_t wlq_paged_attention_workspace_bytes(int64_t T, int B, int Hq, int Hkv, int D, int max_q) {
-    if (T < 1 || B < 1 || Hq < 1 || Hkv < 1 || D < 1 || max_q < 1) return 0;
-    return attention_workspace_bytes(T, B, Hq, Hkv, D, max_q);
+size_t wlq_paged_attention_workspace_bytes(int Hq, int Hkv, int D, int max_q) {
+    if (Hq < 1 || Hkv < 1 || D < 1 || max_q < 1) return 0;
+    return attention_workspace_bytes(Hq, Hkv, D, max_q);
 }
 
 int wlq_paged_attention(const void* q, const void* k_cache, const void* v_cache, const uint8_t* k_exp,
@@ -185,8 +185,13 @@ int wlq_paged_attention(const void* q, const void* k_cache, const void* v_cache,
     if ((rc = bad_rows(fn, "q", q, q_tok, q_head)) || (rc = bad_rows(fn, "out", out, o_tok, o_head))) return rc;
     if (T * (Hq / Hkv) > 0x7fffffff || table_cols * page_size > 0x7fffffff)
         return fail(WLQ_ERR_UNSUPPORTED, "%s: too many tokens for one call", fn);
+    if ((int64_t)B * Hkv > (int64_t)WLQ_ATTENTION_ZERO_BYTES / 4)
+        return fail(WLQ_ERR_UNSUPPORTED, "%s: %d sequences of %d kv heads (at most %u pairs)", fn, B, Hkv,
+                    WLQ_ATTENTION_ZERO_BYTES / 4);
+    if (k_exp && (!aligned16(k_exp) || !aligned16(v_exp)))
+        return fail(WLQ_ERR_ALIGNMENT, "%s: k_exp and v_exp must be 16-byte aligned", fn);
     if ((rc = require_sm100())) return rc;
-    const size_t need = wlq_paged_attention_workspace_bytes(T, B, Hq, Hkv, D, max_q);
+    const size_t need = wlq_paged_attention_workspace_bytes(Hq, Hkv, D, max_q);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(WLQ_ERR_CAPACITY, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need,
                     workspace ? workspace_bytes : (size_t)0);

@@ -1,0 +1,129 @@
+// Pieces that both attention kernels use: waits, copies, exponentials, and a
+// row computed by one warp alone.
+#pragma once
+
+#include "wlq_attn.cuh"
+#include "wlq_sm100.cuh"
+
+namespace wlq {
+
+namespace {
+
+// Where k and v lie: packed rows, a 16-bit paged cache, an 8-bit one.
+enum KvSource { kPacked = 0, kPaged = 1, kPaged8 = 2 };
+
+// mbar_wait by a whole warp, which goes on or gives up together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+// The sequence and kv head a row belongs to, the sequence's first row in q.
+struct RowOf {
+    int b, hk, first;
+};
+
+// Lane values of one cached or packed row in fp32 (E = D / 32 each).
+template <typename T, int D, int SRC>
+__device__ __forceinline__ void load_row(const AttnParams& p, const RowOf& u, int j, bool v, int lane,
+                                         float (&f)[D / 32]) {
+    constexpr int E = D / 32;
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] = 0.f;
+    if constexpr (SRC == kPacked) {
+        const uint16_t* s = v ? p.v + (int64_t)(u.first + j) * p.v_tok + u.hk * p.v_head
+                              : p.k + (int64_t)(u.first + j) * p.k_tok + u.hk * p.k_head;
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = ActTraits<T>::bits_to_f32(s[lane * E + i]);
+    } else {
+        const int page = p.table[(int64_t)u.b * p.table_cols + (j >> p.log2_page)];
+        if (page < 0 || page >= p.num_pages) return;
+        const int64_t row = ((int64_t)page * p.Hkv + u.hk) * p.page_size + (j & (p.page_size - 1));
+        if constexpr (SRC == kPaged) {
+            const uint16_t* s = static_cast<const uint16_t*>(v ? p.v_cache : p.k_cache) + row * D;
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] = ActTraits<T>::bits_to_f32(s[lane * E + i]);
+        } else {
+            const uint8_t* s = static_cast<const uint8_t*>(v ? p.v_cache : p.k_cache) + row * D;
+            const float e = exp2_biased((v ? p.v_exp : p.k_exp)[row]);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                float g[4];
+                e4m3x4_to_f32(s[lane * E + i], g);
+                f[i] = g[0] * e;
+            }
+        }
+    }
+}
+
+// One row over its keys [j0, j1) without the tensor cores, by one warp.  A
+// tensor-core product multiplies the values of keys a row does not see by
+// zero; where those are infinite or NaN the product is NaN, and the row is
+// computed here instead.  m is in powers of two.
+template <typename T, int D, int SRC>
+__device__ __noinline__ void row_alone(const AttnParams& p, const RowOf& u, int row, int j0, int j1, int lane,
+                                       float (&o)[D / 32], float& m, float& l) {
+    constexpr int E = D / 32;
+    const int h = u.hk * p.G + row % p.G;
+    const int64_t tok = u.first + row / p.G;
+    float q[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        q[i] = ActTraits<T>::bits_to_f32(p.q[tok * p.q_tok + h * p.q_head + lane * E + i]);
+        o[i] = 0.f;
+    }
+    m = -INFINITY;
+    l = 0.f;
+    for (int j = j0; j < j1; ++j) {
+        float k[E], v[E];
+        load_row<T, D, SRC>(p, u, j, false, lane, k);
+        load_row<T, D, SRC>(p, u, j, true, lane, v);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += q[i] * k[i];
+#pragma unroll
+        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        s *= p.scale_log2;
+        const float mn = fmaxf(m, s);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float c = exp2f(m - ref), e = exp2f(s - ref);
+        l = l * c + e;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = o[i] * c + e * v[i];
+        m = mn;
+    }
+}
+
+}  // namespace
+
+}  // namespace wlq

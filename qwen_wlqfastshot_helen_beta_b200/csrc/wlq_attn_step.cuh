@@ -1,0 +1,749 @@
+// Attention of few query rows (a decoding step: the new tokens of a sequence
+// times the query heads of a kv head are at most 16) over the paged cache.
+//
+// HBM-bound: the cache is read once.  The key tiles of all sequences and kv
+// heads, 64 keys each, form one list that is shared out evenly over the CTAs
+// whatever the sequences' lengths are; a CTA walks its share, one segment per
+// (sequence, kv head) it touches.  Where a segment is only a part, its
+// unnormalised output and statistics go to the workspace, and the CTA that
+// delivers a (sequence, kv head)'s last part adds the parts up in the order
+// of the keys: one launch, and results that do not depend on timing.
+//
+// A CTA is one TMA producer warp, which keeps the ring of tiles full across
+// segments, and four consumer warps with 16 keys of each tile.  Scores are
+// computed transposed, S^T = K Q^T: the 16 keys are the MMA's rows and the
+// query rows its 8 columns, so 7 query heads of a group waste one column of
+// eight instead of nine rows of sixteen.  The probabilities change layout in
+// registers (movmatrix) and O^T += V^T P^T follows.
+//
+// 8-bit caches: the tensor cores take the e4m3 codes as fp16 (exact), the
+// scales are applied to the scores and folded into the probabilities.  The
+// queries become fp16 with a power of two per row (exact but for values
+// 2^-29 of the row's largest).  A probability p times its value's scale 2^e
+// is kept relative to the largest such product of the row (m1), the sum of
+// the p relative to the largest score (m0), so neither the scales' spread
+// nor rows of zeros cost any precision.
+#pragma once
+
+#include "wlq_attn_row.cuh"
+#include "wlq_internal.h"
+
+namespace wlq {
+
+namespace {
+
+constexpr int kStepKeys = 64;      // keys of a tile, 16 per consumer warp
+constexpr int kStepThreads = 160;  // 4 consumer warps, 1 producer warp
+
+struct StepParams {
+    CUtensorMap tm_k, tm_v;
+    AttnParams a;
+    float* part;        // [2 * CTAs][8 NT][D] parts' outputs, two slots per CTA
+    float* stat;        // [2 * CTAs][8 NT][4] their m1, m0, sum
+    uint32_t* arrived;  // [B * Hkv] parts delivered; zero between calls
+};
+
+template <int D, bool Q8, int NT>
+struct StepPlan {
+    static constexpr int kRowsMax = 8 * NT;
+    static constexpr int kSide = kStepKeys * D * (Q8 ? 1 : 2);  // k or v of a tile
+    static constexpr int kStage = 2 * kSide + (Q8 ? 1024 : 0);  // 8-bit: the rows' scales behind them
+    static constexpr int kMerge = 2 * kRowsMax * D * 4;         // two warps' outputs
+    static constexpr int kStat = 4 * kRowsMax * 4 * 4;
+    static constexpr int kFit = (112 * 1024 - 1024 - 256 - kMerge - kStat) / kStage;  // two CTAs per SM
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kMergeOff = kStages * kStage;
+    static constexpr int kStatOff = kMergeOff + kMerge;
+    static constexpr int kBarOff = kStatOff + kStat;
+    static constexpr int kAlloc = kBarOff + 256 + 1024;
+    static_assert(kStages >= 2, "tiles in flight");
+};
+
+struct StepSeq {
+    int rows, tiles, len, n, first;
+};
+
+__device__ __forceinline__ StepSeq step_seq(const AttnParams& p, int b, int rows_max) {
+    StepSeq s;
+    s.first = b;
+    s.n = 1;
+    if (p.cu) {
+        s.first = p.cu[b];
+        s.n = p.cu[b + 1] - s.first;
+    }
+    if (s.first < 0 || s.n < 0 || (int64_t)s.first + s.n > p.T) s.n = 0;  // rows outside q are nobody's
+    s.len = (int)max((int64_t)0, min((int64_t)p.kv_lens[b], p.table_cols << p.log2_page));
+    s.rows = min(s.n * p.G, rows_max);
+    // an empty sequence's rows (zeros) still have to be written: one tile without keys
+    s.tiles = s.n ? max(1, (s.len + kStepKeys - 1) / kStepKeys) : 0;
+    return s;
+}
+
+// The tiles of one CTA, segment by segment.
+struct StepWalk {
+    int it, it1;      // this CTA's tiles of the list
+    int b, cum;       // current sequence, tiles of the list before it
+    StepSeq s;
+    // the segment: kv head, tiles [t0, t1) of the sequence, list index of tile 0
+    int hk, t0, t1, base;
+
+    __device__ __forceinline__ bool next(const AttnParams& p, int rows_max) {
+        if (it >= it1) return false;
+        while (it >= cum + s.tiles * p.Hkv) {
+            cum += s.tiles * p.Hkv;
+            s = step_seq(p, ++b, rows_max);
+        }
+        hk = (it - cum) / s.tiles;
+        base = cum + hk * s.tiles;
+        t0 = it - base;
+        t1 = min(s.tiles, t0 + (it1 - it));
+        it += t1 - t0;
+        return true;
+    }
+};
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&a)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&a)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64u(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_sync_step() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ float4 ldcg4(const float* a) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(a)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ldcg2(const float* a) {
+    float2 v;
+    asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(a) : "memory");
+    return v;
+}
+// Barrier of the four consumer warps; whether `v` holds for all of them.
+__device__ __forceinline__ bool bar_and_step(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
+}
+// 2^(a - b) where b may be -inf (nothing seen yet)
+__device__ __forceinline__ float rescale(float a, float b) { return a == b ? 1.f : ex2(a - (b == -INFINITY ? 0.f : b)); }
+
+// One finished row: x = (m1, m0, sum, -), a this lane's E values relative to 2^m1.
+template <typename T, int E>
+__device__ __forceinline__ void store_row(const AttnParams& p, int hk, int first, int r, int lane, const float (&a)[E],
+                                          const float4 x) {
+    const float f = x.z > 0.f ? rescale(x.x, x.y) / x.z : (x.z == x.z ? 0.f : x.z);
+    const int tk = r / p.G;
+    uint16_t* d = p.out + (int64_t)(first + tk) * p.o_tok + (hk * p.G + r - tk * p.G) * p.o_head + lane * E;
+#pragma unroll
+    for (int j = 0; j < E; j += 2) *reinterpret_cast<uint32_t*>(d + j) = pack2<T>(a[j] * f, a[j + 1] * f);
+}
+
+template <typename T, int D, bool Q8, int NT>
+__global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid_constant__ StepParams sp) {
+    using P = StepPlan<D, Q8, NT>;
+    using MT = typename std::conditional<Q8, __half, T>::type;  // the MMAs' operand type
+    constexpr int NS = P::kStages, KK = D / 16, RM = P::kRowsMax;
+    const AttnParams& p = sp.a;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int plan[3];  // tiles of the list, first sequence, tiles before it
+    __shared__ uint32_t last_part;
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t sb = (raw + 1023u) & ~1023u;
+    uint8_t* sgen = smem_raw + (sb - raw);
+    const uint32_t bars = sb + P::kBarOff;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (NS + s); };
+    float* merge = reinterpret_cast<float*>(sgen + P::kMergeOff);
+    float* wstat = reinterpret_cast<float*>(sgen + P::kStatOff);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 128) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 4);
+        }
+        mbar_fence_init();
+        tma_prefetch_desc(&sp.tm_k);
+        tma_prefetch_desc(&sp.tm_v);
+    }
+    int G = (int)gridDim.x;  // CTAs with work
+    if (warp == 0) {
+        int total = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 32)
+            total += b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
+        total = (int)warp_sum(total) * p.Hkv;
+        G = min(G, total);
+        int first = 0, cum0 = 0;
+        if ((int)blockIdx.x < G) {
+            const int it = (int)((int64_t)blockIdx.x * total / G);
+            int before = 0;
+            for (int b0 = 0; b0 < p.B; b0 += 32) {
+                const int mine = b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles * p.Hkv : 0;
+                const int cum = warp_scan(mine, lane);
+                const unsigned hit = __ballot_sync(0xffffffffu, it < before + cum);
+                if (hit) {
+                    const int l = __ffs(hit) - 1;
+                    first = b0 + l;
+                    cum0 = before + __shfl_sync(0xffffffffu, cum - mine, l);
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, cum, 31);
+            }
+        }
+        if (lane == 0) {
+            plan[0] = total;
+            plan[1] = first;
+            plan[2] = cum0;
+        }
+    }
+    __syncthreads();
+    const int total = plan[0];
+    G = min((int)gridDim.x, total);
+    if ((int)blockIdx.x >= G) return;
+    StepWalk w;
+    w.it = (int)((int64_t)blockIdx.x * total / G);
+    w.it1 = (int)((int64_t)(blockIdx.x + 1) * total / G);
+    w.b = plan[1];
+    w.cum = plan[2];
+    w.s = step_seq(p, w.b, RM);
+    const int first_it = w.it;
+
+    if (warp == 4) {
+        // ------------------------------------------------------ producer
+        const int box = min(p.page_size, kStepKeys);  // keys of one copy
+        int g = 0;
+        bool ok = true;
+        while (ok && w.next(p, RM)) {
+            for (int t = w.t0; t < w.t1; ++t, ++g) {
+                const int kb = t * kStepKeys;
+                const int pieces = (max(0, min(kStepKeys, w.s.len - kb)) + box - 1) / box;
+                // this lane's page; one outside the pool reads as zeros
+                int z = 0, y = 0;
+                int64_t row = 0;
+                if (lane < pieces) {
+                    const int key = kb + lane * box;
+                    const int id = p.table[(int64_t)w.b * p.table_cols + (key >> p.log2_page)];
+                    const bool in = id >= 0 && id < p.num_pages;
+                    y = key & (p.page_size - 1);
+                    z = (in ? id : (int)p.num_pages) * p.Hkv + w.hk;
+                    row = ((int64_t)(in ? id : 0) * p.Hkv + w.hk) * p.page_size + y;
+                }
+                const int s = g % NS, use = g / NS;
+                if (use > 0 && !(ok = warp_wait(empty(s), (use - 1) & 1))) break;
+                if (lane == 0) mbar_arrive_expect_tx(full(s), pieces * box * (2 * D * (Q8 ? 1 : 2) + (Q8 ? 2 : 0)));
+                __syncwarp();
+                const uint32_t dst = sb + s * P::kStage;
+                if (lane < pieces) {
+                    if constexpr (Q8) {
+                        tma_load_3d(dst + lane * box * D, &sp.tm_k, full(s), 0, y, z);
+                        tma_load_3d(dst + P::kSide + lane * box * D, &sp.tm_v, full(s), 0, y, z);
+                        bulk_load(dst + 2 * P::kSide + lane * box, p.k_exp + row, box, full(s));
+                        bulk_load(dst + 2 * P::kSide + kStepKeys + lane * box, p.v_exp + row, box, full(s));
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h) {
+                            const uint32_t d = dst + h * kStepKeys * 128 + lane * box * 128;
+                            tma_load_3d(d, &sp.tm_k, full(s), h * 64, y, z);
+                            tma_load_3d(d + P::kSide, &sp.tm_v, full(s), h * 64, y, z);
+                        }
+                    }
+                }
+            }
+        }
+        // no copy may still be landing when the CTA exits
+        for (int j = g > NS ? g - NS : 0; j < g; ++j) mbar_wait(full(j % NS), (j / NS) & 1);
+        return;
+    }
+
+    // --------------------------------------------------------- consumers
+    const int gq = lane >> 2, tq = lane & 3;
+    int g = 0;
+    bool ok = true;
+    while (ok && w.next(p, RM)) {
+        const StepSeq s = w.s;
+        const int past = s.len - s.n;
+        // q as the MMAs' B operand: row 8 nt + gq, the head values this lane's k indexes stand for
+        uint32_t qf[NT][KK][2];
+        float fac[NT][2];  // scale of the scores of rows 8 nt + 2 tq, + 1
+        int lim[NT][2];    // their last visible key
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = 8 * nt + gq;
+            const bool in = r < s.rows;
+            const int tk = in ? r / p.G : 0;
+            const uint16_t* src = p.q + (int64_t)(s.first + tk) * p.q_tok + (w.hk * p.G + (in ? r - tk * p.G : 0)) * p.q_head;
+            if constexpr (Q8) {
+                constexpr int C = D / 32;  // 8-value chunks of this lane: its 16-code chunks of a key
+                uint4 v[C];
+                float f[C][8], top = 0.f;
+#pragma unroll
+                for (int x = 0; x < C; ++x) v[x] = in ? ldg_stream_v4(src + tq * (D / 4) + 8 * x) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int x = 0; x < C; ++x) {
+                    const uint32_t u[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        f[x][i] = ActTraits<T>::bits_to_f32((uint16_t)(u[i >> 1] >> (16 * (i & 1))));
+                        top = fmaxf(top, fabsf(f[x][i]));
+                    }
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // 2^14 <= largest * 2^-e < 2^15 (a row of zeros, or of subnormals, as it is)
+                const int eb = min(254, max(15, (int)(__float_as_uint(top) >> 23)));  // e = eb - 127 - 14
+                const float down = __uint_as_float((uint32_t)(127 + 141 - eb) << 23);
+                const float up = __uint_as_float((uint32_t)(eb - 14) << 23) * p.scale_log2;
+                fac[nt][0] = __shfl_sync(0xffffffffu, up, 8 * tq);
+                fac[nt][1] = __shfl_sync(0xffffffffu, up, 8 * tq + 4);
+#pragma unroll
+                for (int x = 0; x < C; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const __half2 h = __floats2half2_rn(f[x][2 * i] * down, f[x][2 * i + 1] * down);
+                        qf[nt][2 * x + (i >> 1)][i & 1] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < KK; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        qf[nt][k][i] = in ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * tq + 8 * i) : 0u;
+                fac[nt][0] = fac[nt][1] = p.scale_log2;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) lim[nt][i] = min(s.len - 1, past + (8 * nt + 2 * tq + i) / p.G);
+        }
+        float o[KK][NT][4];
+        float m1[NT][2], m0[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) m1[nt][i] = m0[nt][i] = -INFINITY, l[nt][i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KK; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[k][nt][i] = 0.f;
+        }
+
+        for (int t = w.t0; t < w.t1; ++t, ++g) {
+            const int st = g % NS;
+            if (!(ok = warp_wait(full(st), (g / NS) & 1))) break;
+            const int kb = t * kStepKeys + warp * 16;
+            if (kb < s.len) {
+                const uint32_t ks = sb + st * P::kStage, vs = ks + P::kSide;
+                const int k0 = warp * 16;
+                float c[2][NT][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) c[h][nt][i] = 0.f;
+                if constexpr (Q8) {
+                    uint4 a[D / 64], b[D / 64];
+#pragma unroll
+                    for (int x = 0; x < D / 64; ++x) {
+                        const int r0 = k0 + gq, r1 = r0 + 8, ch = (D / 64) * tq + x;
+                        if constexpr (D == 128) {
+                            a[x] = lds128(ks + r0 * 128 + (((ch ^ r0) & 7) << 4));
+                            b[x] = lds128(ks + r1 * 128 + (((ch ^ r1) & 7) << 4));
+                        } else {
+                            a[x] = lds128(ks + r0 * 64 + (((ch ^ (r0 >> 1)) & 3) << 4));
+                            b[x] = lds128(ks + r1 * 64 + (((ch ^ (r1 >> 1)) & 3) << 4));
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < D / 64; ++x) {
+                        const uint32_t wa[4] = {a[x].x, a[x].y, a[x].z, a[x].w}, wb[4] = {b[x].x, b[x].y, b[x].z, b[x].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t f[4] = {e4m3x2_to_f16x2(wa[i]), e4m3x2_to_f16x2(wb[i]),
+                                                   e4m3x2_to_f16x2(wa[i] >> 16), e4m3x2_to_f16x2(wb[i] >> 16)};
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                Mma16816<MT>::run(c[i & 1][nt], f, qf[nt][4 * x + i][0], qf[nt][4 * x + i][1]);
+                        }
+                    }
+                } else {
+                    const int r = k0 + (lane & 15);
+#pragma unroll
+                    for (int k = 0; k < KK; ++k) {
+                        uint32_t f[4];
+                        const int ch = 2 * (k & 3) + (lane >> 4);
+                        ldmatrix_x4(ks + (k >> 2) * kStepKeys * 128 + r * 128 + (((ch ^ r) & 7) << 4), f);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) Mma16816<MT>::run(c[k & 1][nt], f, qf[nt][k][0], qf[nt][k][1]);
+                    }
+                }
+                // scores in powers of two; x0 of a key's value scale 2^ve
+                float ke[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f};
+                if constexpr (Q8) {
+                    const uint32_t es = ks + 2 * P::kSide + k0 + gq;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        ke[h] = exp2_biased(lds8(es + 8 * h));
+                        ve[h] = (float)((int)lds8(es + kStepKeys + 8 * h) - 127);
+                    }
+                }
+                float sc[NT][4];
+                bool grow = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = kb + gq + 8 * (i >> 1);
+                        float x = (c[0][nt][i] + c[1][nt][i]) * fac[nt][i & 1];
+                        if constexpr (Q8) x *= ke[i >> 1];
+                        x = key <= lim[nt][i & 1] ? x : -INFINITY;
+                        sc[nt][i] = x;
+                        grow |= x - m0[nt][i & 1] > 8.f;
+                        if constexpr (Q8) grow |= x + ve[i >> 1] - m1[nt][i & 1] > 8.f;
+                    }
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float f1[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float a = fmaxf(m0[nt][i], fmaxf(sc[nt][i], sc[nt][i + 2]));
+                            float b = fmaxf(m1[nt][i], fmaxf(sc[nt][i] + ve[0], sc[nt][i + 2] + ve[1]));
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) {
+                                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+                                if constexpr (Q8) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, d));
+                            }
+                            if constexpr (!Q8) b = a;
+                            l[nt][i] *= rescale(m0[nt][i], a);
+                            f1[i] = rescale(m1[nt][i], b);
+                            m0[nt][i] = a;
+                            m1[nt][i] = b;
+                        }
+#pragma unroll
+                        for (int k = 0; k < KK; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[k][nt][i] *= f1[i & 1];
+                    }
+                }
+                // probabilities: this lane's keys gq, gq + 8 -> B fragments with keys 2 tq ..
+                uint32_t pf[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float x[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float r0 = m0[nt][i] == -INFINITY ? 0.f : m0[nt][i];
+                            const float e = ex2(sc[nt][2 * h + i] - r0);
+                            l[nt][i] += e;
+                            x[i] = e;
+                            if constexpr (Q8) {
+                                const float r1 = m1[nt][i] == -INFINITY ? 0.f : m1[nt][i];
+                                x[i] = ex2(sc[nt][2 * h + i] + ve[h] - r1);
+                            }
+                        }
+                        pf[nt][h] = movmatrix_trans(pack2<MT>(x[0], x[1]));
+                    }
+                const int behind = s.len - kb;  // keys of the 16 that exist
+                if constexpr (Q8) {
+                    constexpr int W = D / 32;  // words of 4 codes of a lane: its chunk of each of 4 keys
+                    uint32_t v[4][W];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int kx = 2 * tq + (x & 1) + 8 * (x >> 1), r = k0 + kx;
+                        if constexpr (D == 128) {
+                            const uint4 q = lds128(vs + r * 128 + (((gq ^ r) & 7) << 4));
+                            v[x][0] = q.x, v[x][1] = q.y, v[x][2] = q.z, v[x][3] = q.w;
+                        } else {
+                            const uint2 q = lds64u(vs + r * 64 + ((((gq >> 1) ^ (r >> 1)) & 3) << 4) + (gq & 1) * 8);
+                            v[x][0] = q.x, v[x][1] = q.y;
+                        }
+                        if (behind < 16 && kx >= behind) {
+#pragma unroll
+                            for (int y = 0; y < W; ++y) v[x][y] = 0u;
+                        }
+                    }
+#pragma unroll
+                    for (int y = 0; y < W; ++y)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t sel = j ? 0x7362u : 0x5140u;
+                            const uint32_t a = prmt(v[0][y], v[1][y], sel), b = prmt(v[2][y], v[3][y], sel);
+                            const uint32_t f[4] = {e4m3x2_to_f16x2(a), e4m3x2_to_f16x2(a >> 16), e4m3x2_to_f16x2(b),
+                                                   e4m3x2_to_f16x2(b >> 16)};
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) Mma16816<MT>::run(o[2 * y + j][nt], f, pf[nt][0], pf[nt][1]);
+                        }
+                } else {
+                    const int r = k0 + (lane & 7) + 8 * (lane >> 4);
+                    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+                    if (behind < 16) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int kx = 2 * tq + 8 * h;
+                            keep[h] = (kx < behind ? 0xffffu : 0u) | (kx + 1 < behind ? 0xffff0000u : 0u);
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < KK; ++k) {
+                        uint32_t f[4];
+                        const int ch = 2 * (k & 3) + ((lane >> 3) & 1);
+                        ldmatrix_x4_trans(vs + (k >> 2) * kStepKeys * 128 + r * 128 + (((ch ^ r) & 7) << 4), f);
+                        if (behind < 16) {
+                            f[0] &= keep[0], f[1] &= keep[0];
+                            f[2] &= keep[1], f[3] &= keep[1];
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) Mma16816<MT>::run(o[k][nt], f, pf[nt][0], pf[nt][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(st));
+        }
+        // ------------------------------- the segment's result, in warp 0
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], d);
+                if (gq == 0)
+                    *reinterpret_cast<float4*>(wstat + (warp * RM + 8 * nt + 2 * tq + i) * 4) =
+                        make_float4(m1[nt][i], m0[nt][i], l[nt][i], 0.f);
+            }
+        if (!(ok = bar_and_step(ok))) break;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float f[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float4 x[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    x[y] = *reinterpret_cast<const float4*>(wstat + (y * RM + 8 * nt + 2 * tq + i) * 4);
+                const float a = fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x));
+                const float b = fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y));
+                f[i] = rescale(m1[nt][i], a);
+                float sum = 0.f;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sum += x[y].z * rescale(x[y].y, b);
+                m1[nt][i] = a;
+                m0[nt][i] = b;
+                l[nt][i] = sum;
+            }
+#pragma unroll
+            for (int k = 0; k < KK; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[k][nt][i] *= f[i & 1];
+        }
+        auto out_to = [&](int y) {
+#pragma unroll
+            for (int k = 0; k < KK; ++k)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    *reinterpret_cast<float4*>(merge + (((y * KK + k) * NT + nt) * 32 + lane) * 4) =
+                        make_float4(o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]);
+        };
+        auto add_from = [&](int y) {
+#pragma unroll
+            for (int k = 0; k < KK; ++k)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float4 x = *reinterpret_cast<const float4*>(merge + (((y * KK + k) * NT + nt) * 32 + lane) * 4);
+                    o[k][nt][0] += x.x, o[k][nt][1] += x.y, o[k][nt][2] += x.z, o[k][nt][3] += x.w;
+                }
+        };
+        if (warp >= 2) out_to(warp - 2);
+        bar_sync_step();
+        if (warp < 2) add_from(warp);
+        if (warp == 1) out_to(1);
+        bar_sync_step();
+        const bool whole = w.t0 == 0 && w.t1 == s.tiles;
+        constexpr int E = D / 32;
+        const int c_first = (int)(((int64_t)(w.base + 1) * G - 1) / total);
+        const int c_last = (int)(((int64_t)(w.base + s.tiles) * G - 1) / total);
+        // the part a CTA has of this (sequence, kv head): its first segment, or (only where the
+        // sequence begins within its share) its last
+        auto slot_of = [&](int c) { return 2 * c + (c == c_first && (int)((int64_t)c * total / G) < w.base ? 1 : 0); };
+        if (warp == 0) {
+            add_from(1);
+            unsigned bad = 0;  // rows with a value that is not finite
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 8 * nt + 2 * tq + i;
+                    float x = 0.f;
+#pragma unroll
+                    for (int k = 0; k < KK; ++k)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float v = o[k][nt][2 * h + i];
+                            const int d = Q8 ? gq * (D / 8) + 2 * k + h : 16 * k + gq + 8 * h;
+                            merge[r * D + d] = v;
+                            x = fmaf(v, 0.f, x);
+                        }
+                    if (x != x) bad |= 1u << r;
+                    if (gq == 0)
+                        *reinterpret_cast<float4*>(wstat + r * 4) = make_float4(m1[nt][i], m0[nt][i], l[nt][i], 0.f);
+                }
+            bad = __reduce_or_sync(0xffffffffu, bad);
+            __syncwarp();
+            // with several new tokens, keys a row does not see may have spoilt it
+            if (s.n > 1 && bad) {
+                for (int r = 0; r < s.rows; ++r) {
+                    const int seen = min(s.len, past + r / p.G + 1);
+                    if (!((bad >> r) & 1) || seen >= w.t1 * kStepKeys) continue;
+                    float a[E], m, sum;
+                    row_alone<T, D, Q8 ? kPaged8 : kPaged>(p, RowOf{w.b, w.hk, s.first}, r, w.t0 * kStepKeys, seen, lane, a,
+                                                           m, sum);
+#pragma unroll
+                    for (int j = 0; j < E; ++j) merge[r * D + lane * E + j] = a[j];
+                    if (lane == 0) *reinterpret_cast<float4*>(wstat + r * 4) = make_float4(m, m, sum, 0.f);
+                }
+                __syncwarp();
+            }
+            const int slot = slot_of((int)blockIdx.x);
+            for (int r = 0; r < s.rows; ++r) {
+                const float4 x = *reinterpret_cast<const float4*>(wstat + r * 4);
+                float a[E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) a[j] = merge[r * D + lane * E + j];
+                if (whole) {
+                    store_row<T, E>(p, w.hk, s.first, r, lane, a, x);
+                } else {
+                    float* d = sp.part + ((int64_t)slot * RM + r) * D + lane * E;
+#pragma unroll
+                    for (int j = 0; j < E; j += 2) *reinterpret_cast<float2*>(d + j) = make_float2(a[j], a[j + 1]);
+                    if (lane == 0) *reinterpret_cast<float4*>(sp.stat + ((int64_t)slot * RM + r) * 4) = x;
+                }
+            }
+            if (!whole) {
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) {
+                    uint32_t* n = sp.arrived + w.b * p.Hkv + w.hk;
+                    const bool last = atomicAdd(n, 1u) == (uint32_t)(c_last - c_first);
+                    if (last) *n = 0u;  // every part is here: nobody else looks at it in this call
+                    __threadfence();
+                    last_part = last;
+                }
+            }
+        }
+        if (!whole) {
+            bar_sync_step();
+            if (last_part) {
+                for (int r = warp; r < s.rows; r += 4) {
+                    float a1 = -INFINITY, a0 = -INFINITY;
+                    for (int c = c_first + lane; c <= c_last; c += 32) {
+                        const float4 x = ldcg4(sp.stat + ((int64_t)slot_of(c) * RM + r) * 4);
+                        a1 = fmaxf(a1, x.x);
+                        a0 = fmaxf(a0, x.y);
+                    }
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) {
+                        a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, d));
+                        a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, d));
+                    }
+                    float a[E], sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < E; ++j) a[j] = 0.f;
+#pragma unroll 4
+                    for (int c = c_first; c <= c_last; ++c) {
+                        const int64_t at = (int64_t)slot_of(c) * RM + r;
+                        const float4 x = ldcg4(sp.stat + at * 4);
+                        const float f = rescale(x.x, a1);
+                        sum += x.z * rescale(x.y, a0);
+#pragma unroll
+                        for (int j = 0; j < E; j += 2) {
+                            const float2 v = ldcg2(sp.part + at * D + lane * E + j);
+                            a[j] += v.x * f;
+                            a[j + 1] += v.y * f;
+                        }
+                    }
+                    store_row<T, E>(p, w.hk, s.first, r, lane, a, make_float4(a1, a0, sum, 0.f));
+                }
+            }
+        }
+    }
+}
+
+// Counters of the (sequence, kv head) pairs ahead of the parts; their place
+// does not depend on the call, so that what one call leaves zero the next
+// one finds zero.
+constexpr size_t kStepCounters = WLQ_ATTENTION_ZERO_BYTES / 4;
+
+inline int step_ctas() { return 2 * device_sm_count(); }
+
+template <typename T, int D, bool Q8, int NT>
+int launch_step(const AttnParams& a, cudaStream_t stream) {
+    using P = StepPlan<D, Q8, NT>;
+    StepParams sp;
+    sp.a = a;
+    int rc;
+    const CUtensorMapDataType dt = Q8                            ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : (ActTraits<T>::kIsF16) ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    constexpr int es = Q8 ? 1 : 2;
+    const uint64_t pg = (uint64_t)a.num_pages * a.Hkv, ps = a.page_size;
+    const CUtensorMapSwizzle sw = Q8 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    const uint32_t box = Q8 ? D : 64, keys = a.page_size < kStepKeys ? a.page_size : kStepKeys;
+    if ((rc = encode_3d(&sp.tm_k, dt, a.k_cache, D, ps, pg, D * es, ps * D * es, box, keys, 1, sw, "k_cache")) ||
+        (rc = encode_3d(&sp.tm_v, dt, a.v_cache, D, ps, pg, D * es, ps * D * es, box, keys, 1, sw, "v_cache")))
+        return rc;
+    const int grid = step_ctas();
+    sp.arrived = static_cast<uint32_t*>(a.ws);
+    sp.stat = reinterpret_cast<float*>(sp.arrived + kStepCounters);
+    sp.part = sp.stat + (size_t)2 * grid * P::kRowsMax * 4;
+    static const cudaError_t attr = cudaFuncSetAttribute(attn_step_kernel<T, D, Q8, NT>,
+                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, P::kAlloc);
+    if (attr != cudaSuccess) return check_cuda(attr, "attn_step_kernel shared memory");
+    attn_step_kernel<T, D, Q8, NT><<<grid, kStepThreads, P::kAlloc, stream>>>(sp);
+    return check_cuda(cudaGetLastError(), "attn_step_kernel");
+}
+
+template <typename T>
+int launch_step_any(const AttnParams& a, cudaStream_t stream) {
+    const bool one = a.max_q * a.G <= 8;
+    if (a.k_exp) {
+        if (a.D == 64) return one ? launch_step<T, 64, true, 1>(a, stream) : launch_step<T, 64, true, 2>(a, stream);
+        return one ? launch_step<T, 128, true, 1>(a, stream) : launch_step<T, 128, true, 2>(a, stream);
+    }
+    if (a.D == 64) return one ? launch_step<T, 64, false, 1>(a, stream) : launch_step<T, 64, false, 2>(a, stream);
+    return one ? launch_step<T, 128, false, 1>(a, stream) : launch_step<T, 128, false, 2>(a, stream);
+}
+
+}  // namespace
+
+}  // namespace wlq

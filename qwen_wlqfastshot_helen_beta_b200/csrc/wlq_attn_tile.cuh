@@ -34,9 +34,8 @@
 // word and the CTA winds down, releasing its TMEM.
 #pragma once
 
-#include "wlq_attn.cuh"
+#include "wlq_attn_row.cuh"
 #include "wlq_internal.h"
-#include "wlq_sm100.cuh"
 
 namespace wlq {
 
@@ -45,8 +44,6 @@ namespace {
 constexpr int kRowsT = 128;   // query rows of one tile (MMA M)
 constexpr int kRows = 256;    // query rows of one CTA
 constexpr int kKeys = 128;    // keys of one tile
-
-enum KvSource { kPacked = 0, kPaged = 1, kPaged8 = 2 };
 
 struct TileParams {
     CUtensorMap tm_k, tm_v;
@@ -123,20 +120,6 @@ __device__ __forceinline__ int splits_of(const Seq& s, int64_t work, int sms) {
     return max(1, most);
 }
 
-__device__ __forceinline__ int64_t warp_sum(int64_t v) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
-}
-__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-
 // Key tiles times row tiles of all sequences (paged form), by one warp.
 __device__ __forceinline__ int64_t total_work(const AttnParams& p, int lane) {
     int64_t w = 0;
@@ -201,19 +184,7 @@ __device__ __forceinline__ bool find_unit(const AttnParams& p, int sms, int c, i
     return false;
 }
 
-// mbar_wait by a whole warp, which goes on or gives up together.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
-}
-
 // ------------------------------------------------------------ tcgen05 extras
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
-        : "memory");
-}
 
 // Descriptor of a tile stored as its transpose (the MMA's N contiguous): 128
 // key rows of 64 values in the 128-byte swizzle, 8-row atoms of 1024 bytes
@@ -272,92 +243,11 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
-    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-
 // Byte offset of 16-byte chunk c (of 8 values) of row r in a tile: blocks of
 // 64 columns, the chunk index XORed with row % 8 inside a 128-byte row (the
 // layout TMA writes and tcgen05 reads).
 __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
     return (uint32_t)((c >> 3) * (kKeys * 128) + r * 128 + (((c ^ r) & 7) << 4));
-}
-
-// Lane values of one cached or packed row in fp32 (E = D / 32 each).
-template <typename T, int D, int SRC>
-__device__ __forceinline__ void load_row(const AttnParams& p, const Unit& u, int j, bool v, int lane,
-                                         float (&f)[D / 32]) {
-    constexpr int E = D / 32;
-#pragma unroll
-    for (int i = 0; i < E; ++i) f[i] = 0.f;
-    if constexpr (SRC == kPacked) {
-        const uint16_t* s = v ? p.v + (int64_t)(u.first + j) * p.v_tok + u.hk * p.v_head
-                              : p.k + (int64_t)(u.first + j) * p.k_tok + u.hk * p.k_head;
-#pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = ActTraits<T>::bits_to_f32(s[lane * E + i]);
-    } else {
-        const int page = p.table[(int64_t)u.b * p.table_cols + (j >> p.log2_page)];
-        if (page < 0 || page >= p.num_pages) return;
-        const int64_t row = ((int64_t)page * p.Hkv + u.hk) * p.page_size + (j & (p.page_size - 1));
-        if constexpr (SRC == kPaged) {
-            const uint16_t* s = static_cast<const uint16_t*>(v ? p.v_cache : p.k_cache) + row * D;
-#pragma unroll
-            for (int i = 0; i < E; ++i) f[i] = ActTraits<T>::bits_to_f32(s[lane * E + i]);
-        } else {
-            const uint8_t* s = static_cast<const uint8_t*>(v ? p.v_cache : p.k_cache) + row * D;
-            const float e = exp2_biased((v ? p.v_exp : p.k_exp)[row]);
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                float g[4];
-                e4m3x4_to_f32(s[lane * E + i], g);
-                f[i] = g[0] * e;
-            }
-        }
-    }
-}
-
-// One row over its keys [j0, j1) without the tensor cores, by one warp.  A
-// tensor-core product multiplies the values of keys a row does not see by
-// zero; where those are infinite or NaN the product is NaN, and the row is
-// computed here instead.  m is in powers of two.
-template <typename T, int D, int SRC>
-__device__ __noinline__ void row_alone(const AttnParams& p, const Unit& u, int row, int j0, int j1, int lane,
-                                       float (&o)[D / 32], float& m, float& l) {
-    constexpr int E = D / 32;
-    const int h = u.hk * p.G + row % p.G;
-    const int64_t tok = u.first + row / p.G;
-    float q[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        q[i] = ActTraits<T>::bits_to_f32(p.q[tok * p.q_tok + h * p.q_head + lane * E + i]);
-        o[i] = 0.f;
-    }
-    m = -INFINITY;
-    l = 0.f;
-    for (int j = j0; j < j1; ++j) {
-        float k[E], v[E];
-        load_row<T, D, SRC>(p, u, j, false, lane, k);
-        load_row<T, D, SRC>(p, u, j, true, lane, v);
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) s += q[i] * k[i];
-#pragma unroll
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        s *= p.scale_log2;
-        const float mn = fmaxf(m, s);
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        const float c = exp2f(m - ref), e = exp2f(s - ref);
-        l = l * c + e;
-#pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = o[i] * c + e * v[i];
-        m = mn;
-    }
 }
 
 template <typename T, int D, int SRC>
@@ -593,7 +483,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                 const int rx = __shfl_sync(0xffffffffu, row, x);
                 const int j1 = __shfl_sync(0xffffffffu, lim, x) + 1;
                 float o[D / 32], mx, lx;
-                row_alone<T, D, SRC>(p, u, rx, key0, min(j1, key0 + n * kKeys), lane, o, mx, lx);
+                row_alone<T, D, SRC>(p, RowOf{u.b, u.hk, u.first}, rx, key0, min(j1, key0 + n * kKeys), lane, o, mx, lx);
                 const int tx = rx / p.G, hx = u.hk * p.G + (rx - tx * p.G);
                 if (u.slot < 0) {
                     const float ix = lx > 0.f ? 1.f / lx : (lx == lx ? 0.f : lx);
@@ -885,7 +775,7 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
             (rc = encode_3d(&tp.tm_v, dt, a.v_cache, D, ps, pg, D * es, ps * D * es, box, ps, 1, sw, "v_cache")))
             return rc;
     }
-    tp.part = static_cast<float*>(a.ws);
+    tp.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + WLQ_ATTENTION_ZERO_BYTES);
     tp.stat = tp.part + (size_t)tp.sms * kRows * D;
     const int64_t grid = (a.T * a.G / kRows + a.B) * a.Hkv + (SRC == kPacked ? 0 : tp.sms);
     if (grid > 0x7fffffff) return fail(WLQ_ERR_UNSUPPORTED, "attention: %lld row tiles in one call", (long long)grid);

@@ -944,14 +944,13 @@ int read_device_error(int device, unsigned int* flags, int clear) {
     cudaError_t e = cudaGetDevice(&prev);
     if (e != cudaSuccess) return check_cuda(e, "cudaGetDevice");
     if (device != prev && (e = cudaSetDevice(device)) != cudaSuccess) return check_cuda(e, "cudaSetDevice");
-    unsigned int v = 0, tile16 = 0, tilebf = 0, position = 0;
+    unsigned int v = 0, attention = 0, position = 0;
     int rc = tu_device_error(&v, clear);
-    if (!rc) rc = attn_tile_error_f16(&tile16, clear);
-    if (!rc) rc = attn_tile_error_bf16(&tilebf, clear);
+    if (!rc) rc = attention_error(&attention, clear);
     if (!rc) rc = rope_position_error(&position, clear);
     if (device != prev) cudaSetDevice(prev);
     if (rc) return rc;
-    *flags = v | tile16 | tilebf | (position ? WLQ_DEVERR_POSITION : 0u);
+    *flags = v | attention | (position ? WLQ_DEVERR_POSITION : 0u);
     return WLQ_OK;
 }
 

@@ -101,12 +101,18 @@ struct AttnParams;
 int launch_rope_kv_write(RopeParams& p, bool f16, bool quant, cudaStream_t stream);
 int launch_kv_read(KvReadParams& p, bool f16, bool quant, cudaStream_t stream);
 int launch_attention(const AttnParams& p, bool f16, cudaStream_t stream);
-size_t attention_workspace_bytes(int64_t T, int B, int Hq, int Hkv, int D, int max_q);
+size_t attention_workspace_bytes(int Hq, int Hkv, int D, int max_q);
 int launch_attn_tile_f16(const AttnParams& p, cudaStream_t stream);
 int launch_attn_tile_bf16(const AttnParams& p, cudaStream_t stream);
-// The device error words of their translation units, on the current device.
+int launch_attn_step_f16(const AttnParams& p, cudaStream_t stream);
+int launch_attn_step_bf16(const AttnParams& p, cudaStream_t stream);
+// The device error words of their translation units, and all of them in one,
+// on the current device.
 int attn_tile_error_f16(unsigned int* flags, int clear);
 int attn_tile_error_bf16(unsigned int* flags, int clear);
+int attn_step_error_f16(unsigned int* flags, int clear);
+int attn_step_error_bf16(unsigned int* flags, int clear);
+int attention_error(unsigned int* flags, int clear);
 // Reads (and optionally clears) the current device's flag of a rope_kv_write
 // position outside the cos/sin table.
 int rope_position_error(unsigned int* flag, int clear);
