@@ -125,9 +125,9 @@ __device__ __forceinline__ uint2 lds64u(uint32_t a) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+// Arrives on bar when this thread's cp.async copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void bar_sync_step() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ float4 ldcg4(const float* a) {
@@ -168,6 +168,87 @@ __device__ __forceinline__ void store_row(const AttnParams& p, int hk, int first
     for (int j = 0; j < E; j += 2) *reinterpret_cast<uint32_t*>(d + j) = pack2<T>(a[j] * f, a[j + 1] * f);
 }
 
+// Adds up the parts of one (sequence, kv head), by the four consumer warps:
+// the statistics first (a row per warp, a part per lane), then the outputs (a
+// quarter of the parts per warp, all rows), all loads of a part in flight
+// together.  Every sum has a fixed order.
+template <typename T, int D, int NT, typename Slot>
+__device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int hk, int first, int c_first, int c_last,
+                                           Slot slot_of, float* merge, float* wstat, int warp, int lane) {
+    constexpr int RM = 8 * NT, E = D / 32;
+    for (int r = warp; r < rows; r += 4) {
+        float a1 = -INFINITY, a0 = -INFINITY, sum = 0.f;
+        for (int c = c_first + lane; c <= c_last; c += 32) {
+            const float4 x = ldcg4(sp.stat + ((int64_t)slot_of(c) * RM + r) * 4);
+            const float m = fmaxf(a0, x.y);
+            sum = sum * rescale(a0, m) + x.z * rescale(x.y, m);
+            a0 = m;
+            a1 = fmaxf(a1, x.x);
+        }
+        const float mine = a0;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, d));
+            a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, d));
+        }
+        sum *= rescale(mine, a0);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) *reinterpret_cast<float4*>(wstat + (RM + r) * 4) = make_float4(a1, a0, sum, 0.f);
+    }
+    bar_sync_step();
+    const float top = lane < rows ? wstat[(RM + lane) * 4] : 0.f;
+    float a[RM][E];
+#pragma unroll
+    for (int r = 0; r < RM; ++r)
+#pragma unroll
+        for (int j = 0; j < E; ++j) a[r][j] = 0.f;
+#pragma unroll(NT == 1 ? 3 : 1)
+    for (int c = c_first + warp; c <= c_last; c += 4) {
+        const int64_t at = (int64_t)slot_of(c) * RM;
+        const float fl = lane < rows ? rescale(ldcg4(sp.stat + (at + lane) * 4).x, top) : 0.f;
+#pragma unroll
+        for (int r = 0; r < RM; ++r) {
+            if (r >= rows) break;
+            const float f = __shfl_sync(0xffffffffu, fl, r);
+#pragma unroll
+            for (int j = 0; j < E; j += 2) {
+                const float2 v = ldcg2(sp.part + (at + r) * D + lane * E + j);
+                a[r][j] += v.x * f;
+                a[r][j + 1] += v.y * f;
+            }
+        }
+    }
+    auto put = [&](int y) {
+#pragma unroll
+        for (int r = 0; r < RM; ++r)
+#pragma unroll
+            for (int j = 0; j < E; j += 2)
+                *reinterpret_cast<float2*>(merge + (y * RM + r) * D + lane * E + j) = make_float2(a[r][j], a[r][j + 1]);
+    };
+    auto add = [&](int y) {
+#pragma unroll
+        for (int r = 0; r < RM; ++r)
+#pragma unroll
+            for (int j = 0; j < E; j += 2) {
+                const float2 v = *reinterpret_cast<const float2*>(merge + (y * RM + r) * D + lane * E + j);
+                a[r][j] += v.x;
+                a[r][j + 1] += v.y;
+            }
+    };
+    if (warp >= 2) put(warp - 2);
+    bar_sync_step();
+    if (warp < 2) add(warp);
+    if (warp == 1) put(1);
+    bar_sync_step();
+    if (warp == 0) {
+        add(1);
+#pragma unroll
+        for (int r = 0; r < RM; ++r)
+            if (r < rows) store_row<T, E>(sp.a, hk, first, r, lane, a[r], *reinterpret_cast<const float4*>(wstat + (RM + r) * 4));
+    }
+}
+
 template <typename T, int D, bool Q8, int NT>
 __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid_constant__ StepParams sp) {
     using P = StepPlan<D, Q8, NT>;
@@ -175,7 +256,7 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
     constexpr int NS = P::kStages, KK = D / 16, RM = P::kRowsMax;
     const AttnParams& p = sp.a;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int plan[3];  // tiles of the list, first sequence, tiles before it
+    __shared__ int plan[4];  // tiles of the list, first sequence, tiles before it, CTAs with work
     __shared__ uint32_t last_part;
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sb = (raw + 1023u) & ~1023u;
@@ -189,20 +270,25 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
 
     if (threadIdx.x == 128) {
         for (int s = 0; s < NS; ++s) {
-            mbar_init(full(s), 1);
+            mbar_init(full(s), Q8 ? 33 : 1);  // the producer's bytes; its lanes' copies of the scales
             mbar_init(empty(s), 4);
         }
         mbar_fence_init();
         tma_prefetch_desc(&sp.tm_k);
         tma_prefetch_desc(&sp.tm_v);
     }
-    int G = (int)gridDim.x;  // CTAs with work
     if (warp == 0) {
-        int total = 0;
-        for (int b0 = 0; b0 < p.B; b0 += 32)
-            total += b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
+        int total = 0, units = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 32) {
+            const int tiles = b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
+            total += tiles;
+            units += tiles > 0;
+        }
         total = (int)warp_sum(total) * p.Hkv;
-        G = min(G, total);
+        units = (int)warp_sum(units) * p.Hkv;
+        // CTAs with work: with n tiles per (sequence, kv head) in P parts, a part's tiles take n / P * 0.4 us and
+        // joining P * 0.05 us, least at P = sqrt(8 n)
+        const int G = min(min((int)gridDim.x, total), (int)sqrtf(8.f * units * total) + 1);
         int first = 0, cum0 = 0;
         if ((int)blockIdx.x < G) {
             const int it = (int)((int64_t)blockIdx.x * total / G);
@@ -224,11 +310,11 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
             plan[0] = total;
             plan[1] = first;
             plan[2] = cum0;
+            plan[3] = G;
         }
     }
     __syncthreads();
-    const int total = plan[0];
-    G = min((int)gridDim.x, total);
+    const int total = plan[0], G = plan[3];
     if ((int)blockIdx.x >= G) return;
     StepWalk w;
     w.it = (int)((int64_t)blockIdx.x * total / G);
@@ -244,35 +330,43 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
         int g = 0;
         bool ok = true;
         while (ok && w.next(p, RM)) {
+            int ids = 0;  // page of this lane's 16 keys of a window of 8 tiles; one outside the pool reads as zeros
             for (int t = w.t0; t < w.t1; ++t, ++g) {
+                const int x = (t - w.t0) & 7;
+                if (x == 0) {
+                    const int key = t * kStepKeys + lane * 16;
+                    ids = key < w.s.len ? p.table[(int64_t)w.b * p.table_cols + (key >> p.log2_page)] : -1;
+                    if (ids < 0 || ids >= p.num_pages) ids = (int)p.num_pages;
+                }
                 const int kb = t * kStepKeys;
                 const int pieces = (max(0, min(kStepKeys, w.s.len - kb)) + box - 1) / box;
-                // this lane's page; one outside the pool reads as zeros
-                int z = 0, y = 0;
-                int64_t row = 0;
-                if (lane < pieces) {
-                    const int key = kb + lane * box;
-                    const int id = p.table[(int64_t)w.b * p.table_cols + (key >> p.log2_page)];
-                    const bool in = id >= 0 && id < p.num_pages;
-                    y = key & (p.page_size - 1);
-                    z = (in ? id : (int)p.num_pages) * p.Hkv + w.hk;
-                    row = ((int64_t)(in ? id : 0) * p.Hkv + w.hk) * p.page_size + y;
-                }
                 const int s = g % NS, use = g / NS;
+                const int key = kb + (lane & 3) * 16;  // 16 keys per lane, twice
+                const int id = __shfl_sync(0xffffffffu, ids, 4 * x + (lane & 3));
+                const int y = key & (p.page_size - 1);
                 if (use > 0 && !(ok = warp_wait(empty(s), (use - 1) & 1))) break;
-                if (lane == 0) mbar_arrive_expect_tx(full(s), pieces * box * (2 * D * (Q8 ? 1 : 2) + (Q8 ? 2 : 0)));
+                if (lane == 0) mbar_arrive_expect_tx(full(s), pieces * box * 2 * D * (Q8 ? 1 : 2));
                 __syncwarp();
                 const uint32_t dst = sb + s * P::kStage;
-                if (lane < pieces) {
+                if constexpr (Q8) {
+                    // the rows' scales, 16 bytes a lane: a copy of its own for them would cost the TMA unit as much as
+                    // the codes' (3.7 TB/s of cache with it, 16 sequences of 16384 tokens)
+                    if (lane < 8) {
+                        const int64_t row = ((int64_t)id * p.Hkv + w.hk) * p.page_size + y;
+                        cp_async16(dst + 2 * P::kSide + lane * 16, (lane < 4 ? p.k_exp : p.v_exp) + (id < p.num_pages ? row : 0),
+                                   id < p.num_pages);
+                    }
+                    cp_async_arrive(full(s));
+                }
+                if (lane < 4 && (lane * 16) % box == 0 && lane * 16 < pieces * box) {
+                    const int z = id * p.Hkv + w.hk;
                     if constexpr (Q8) {
-                        tma_load_3d(dst + lane * box * D, &sp.tm_k, full(s), 0, y, z);
-                        tma_load_3d(dst + P::kSide + lane * box * D, &sp.tm_v, full(s), 0, y, z);
-                        bulk_load(dst + 2 * P::kSide + lane * box, p.k_exp + row, box, full(s));
-                        bulk_load(dst + 2 * P::kSide + kStepKeys + lane * box, p.v_exp + row, box, full(s));
+                        tma_load_3d(dst + lane * 16 * D, &sp.tm_k, full(s), 0, y, z);
+                        tma_load_3d(dst + P::kSide + lane * 16 * D, &sp.tm_v, full(s), 0, y, z);
                     } else {
 #pragma unroll
                         for (int h = 0; h < D / 64; ++h) {
-                            const uint32_t d = dst + h * kStepKeys * 128 + lane * box * 128;
+                            const uint32_t d = dst + h * kStepKeys * 128 + lane * 16 * 128;
                             tma_load_3d(d, &sp.tm_k, full(s), h * 64, y, z);
                             tma_load_3d(d + P::kSide, &sp.tm_v, full(s), h * 64, y, z);
                         }
@@ -664,36 +758,7 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
         if (!whole) {
             bar_sync_step();
             if (last_part) {
-                for (int r = warp; r < s.rows; r += 4) {
-                    float a1 = -INFINITY, a0 = -INFINITY;
-                    for (int c = c_first + lane; c <= c_last; c += 32) {
-                        const float4 x = ldcg4(sp.stat + ((int64_t)slot_of(c) * RM + r) * 4);
-                        a1 = fmaxf(a1, x.x);
-                        a0 = fmaxf(a0, x.y);
-                    }
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) {
-                        a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, d));
-                        a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, d));
-                    }
-                    float a[E], sum = 0.f;
-#pragma unroll
-                    for (int j = 0; j < E; ++j) a[j] = 0.f;
-#pragma unroll 4
-                    for (int c = c_first; c <= c_last; ++c) {
-                        const int64_t at = (int64_t)slot_of(c) * RM + r;
-                        const float4 x = ldcg4(sp.stat + at * 4);
-                        const float f = rescale(x.x, a1);
-                        sum += x.z * rescale(x.y, a0);
-#pragma unroll
-                        for (int j = 0; j < E; j += 2) {
-                            const float2 v = ldcg2(sp.part + at * D + lane * E + j);
-                            a[j] += v.x * f;
-                            a[j + 1] += v.y * f;
-                        }
-                    }
-                    store_row<T, E>(p, w.hk, s.first, r, lane, a, make_float4(a1, a0, sum, 0.f));
-                }
+                join_parts<T, D, NT>(sp, s.rows, w.hk, s.first, c_first, c_last, slot_of, merge, wstat, warp, lane);
             }
         }
     }
