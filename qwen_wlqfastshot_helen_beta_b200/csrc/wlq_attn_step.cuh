@@ -50,7 +50,8 @@ struct StepPlan {
     static constexpr int kStage = 2 * kSide + (Q8 ? 1024 : 0);  // 8-bit: the rows' scales behind them
     static constexpr int kMerge = 2 * kRowsMax * D * 4;         // two warps' outputs
     static constexpr int kStat = 4 * kRowsMax * 4 * 4;
-    static constexpr int kFit = (112 * 1024 - 1024 - 256 - kMerge - kStat) / kStage;  // two CTAs per SM
+    static constexpr int kCtas = NT == 1 ? 3 : 2;               // per SM
+    static constexpr int kFit = ((kCtas == 3 ? 74 : 112) * 1024 - 1024 - 256 - kMerge - kStat) / kStage;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kMergeOff = kStages * kStage;
     static constexpr int kStatOff = kMergeOff + kMerge;
@@ -78,6 +79,22 @@ __device__ __forceinline__ StepSeq step_seq(const AttnParams& p, int b, int rows
     s.tiles = s.n ? max(1, (s.len + kStepKeys - 1) / kStepKeys) : 0;
     return s;
 }
+
+// The list's G - 1 cuts, at even distances; a cut within `slack` tiles of a
+// sequence's (and kv head's) end moves there, so that a part is worth the
+// joining it costs.
+struct StepCuts {
+    int total, G, slack;
+    __device__ __forceinline__ int raw(int c) const { return (int)((int64_t)c * total / G); }
+    // the cuts inside tiles [base, base + n): c in [lo, hi]
+    __device__ __forceinline__ void inside(int base, int n, int& lo, int& hi) const {
+        lo = (int)(((int64_t)(base + slack + 1) * G + total - 1) / total);
+        hi = (int)(((int64_t)(base + n - slack) * G + total - 1) / total) - 1;
+    }
+    __device__ __forceinline__ int moved(int at, int base, int n) const {
+        return at - base <= slack ? base : (base + n - at <= slack ? base + n : at);
+    }
+};
 
 // The tiles of one CTA, segment by segment.
 struct StepWalk {
@@ -141,6 +158,12 @@ __device__ __forceinline__ float2 ldcg2(const float* a) {
     asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(a) : "memory");
     return v;
 }
+// n += v; what this warp wrote before is visible to whoever adds after it, and the other way round.
+__device__ __forceinline__ uint32_t add_acq_rel(uint32_t* n, uint32_t v) {
+    uint32_t old;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], %2;" : "=r"(old) : "l"(n), "r"(v) : "memory");
+    return old;
+}
 // Barrier of the four consumer warps; whether `v` holds for all of them.
 __device__ __forceinline__ bool bar_and_step(bool v) {
     uint32_t r;
@@ -168,56 +191,78 @@ __device__ __forceinline__ void store_row(const AttnParams& p, int hk, int first
     for (int j = 0; j < E; j += 2) *reinterpret_cast<uint32_t*>(d + j) = pack2<T>(a[j] * f, a[j + 1] * f);
 }
 
-// Adds up the parts of one (sequence, kv head), by the four consumer warps:
-// the statistics first (a row per warp, a part per lane), then the outputs (a
-// quarter of the parts per warp, all rows), all loads of a part in flight
-// together.  Every sum has a fixed order.
-template <typename T, int D, int NT, typename Slot>
-__device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int hk, int first, int c_first, int c_last,
-                                           Slot slot_of, float* merge, float* wstat, int warp, int lane) {
-    constexpr int RM = 8 * NT, E = D / 32;
-    for (int r = warp; r < rows; r += 4) {
-        float a1 = -INFINITY, a0 = -INFINITY, sum = 0.f;
-        for (int c = c_first + lane; c <= c_last; c += 32) {
-            const float4 x = ldcg4(sp.stat + ((int64_t)slot_of(c) * RM + r) * 4);
-            const float m = fmaxf(a0, x.y);
-            sum = sum * rescale(a0, m) + x.z * rescale(x.y, m);
-            a0 = m;
-            a1 = fmaxf(a1, x.x);
-        }
-        const float mine = a0;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, d));
-            a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, d));
-        }
-        sum *= rescale(mine, a0);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) *reinterpret_cast<float4*>(wstat + (RM + r) * 4) = make_float4(a1, a0, sum, 0.f);
-    }
-    bar_sync_step();
-    const float top = lane < rows ? wstat[(RM + lane) * 4] : 0.f;
-    float a[RM][E];
+// Adds up the parts of one (sequence, kv head), by the four consumer warps: a
+// quarter of the parts per warp, all loads of a few parts in flight together,
+// the statistics of row r in lane r.  Every sum has a fixed order.  Part 0 is
+// CTA c0's last, part i > 0 the first of CTA c0 + i.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int hk, int first, int c0, int parts,
+                                           float* merge, float* wstat, int warp, int lane) {
+    constexpr int RM = 8 * NT, E = D / 32, U = 2 / NT;
+    float a[RM][E], a1 = -INFINITY, a0 = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int r = 0; r < RM; ++r)
 #pragma unroll
         for (int j = 0; j < E; ++j) a[r][j] = 0.f;
-#pragma unroll(NT == 1 ? 3 : 1)
-    for (int c = c_first + warp; c <= c_last; c += 4) {
-        const int64_t at = (int64_t)slot_of(c) * RM;
-        const float fl = lane < rows ? rescale(ldcg4(sp.stat + (at + lane) * 4).x, top) : 0.f;
+    for (int i0 = warp; i0 < parts; i0 += 4 * U) {
+        float4 x[U];
+        float v[U][RM][E];
+#pragma unroll
+        for (int y = 0; y < U; ++y) {
+            const int i = i0 + 4 * y;
+            const int64_t at = (int64_t)(2 * (c0 + i) + (i == 0)) * RM;
+            const bool in = i < parts;
+            x[y] = in && lane < rows ? ldcg4(sp.stat + (at + lane) * 4) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+#pragma unroll
+            for (int r = 0; r < RM; ++r)
+#pragma unroll
+                for (int j = 0; j < E; j += 2) {
+                    float2 t = make_float2(0.f, 0.f);
+                    if (in && r < rows) t = ldcg2(sp.part + (at + r) * D + lane * E + j);
+                    v[y][r][j] = t.x, v[y][r][j + 1] = t.y;
+                }
+        }
+        float b1 = a1, b0 = a0;
+#pragma unroll
+        for (int y = 0; y < U; ++y) b1 = fmaxf(b1, x[y].x), b0 = fmaxf(b0, x[y].y);
+        const float keep = rescale(a1, b1);
+        sum *= rescale(a0, b0);
+        a1 = b1, a0 = b0;
+        float f[U];
+#pragma unroll
+        for (int y = 0; y < U; ++y) {
+            f[y] = rescale(x[y].x, a1);
+            sum += x[y].z * rescale(x[y].y, a0);
+        }
 #pragma unroll
         for (int r = 0; r < RM; ++r) {
-            if (r >= rows) break;
-            const float f = __shfl_sync(0xffffffffu, fl, r);
+            const float k = __shfl_sync(0xffffffffu, keep, r);
 #pragma unroll
-            for (int j = 0; j < E; j += 2) {
-                const float2 v = ldcg2(sp.part + (at + r) * D + lane * E + j);
-                a[r][j] += v.x * f;
-                a[r][j + 1] += v.y * f;
+            for (int j = 0; j < E; ++j) a[r][j] *= k;
+#pragma unroll
+            for (int y = 0; y < U; ++y) {
+                const float g = __shfl_sync(0xffffffffu, f[y], r);
+#pragma unroll
+                for (int j = 0; j < E; ++j) a[r][j] += v[y][r][j] * g;
             }
         }
+    }
+    if (lane < RM) *reinterpret_cast<float4*>(wstat + (warp * RM + lane) * 4) = make_float4(a1, a0, sum, 0.f);
+    bar_sync_step();
+    float4 st[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) st[y] = *reinterpret_cast<const float4*>(wstat + (y * RM + (lane & (RM - 1))) * 4);
+    const float t1 = fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x));
+    const float t0 = fmaxf(fmaxf(st[0].y, st[1].y), fmaxf(st[2].y, st[3].y));
+    float all = 0.f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) all += st[y].z * rescale(st[y].y, t0);
+    const float fw = rescale(st[warp].x, t1);
+#pragma unroll
+    for (int r = 0; r < RM; ++r) {
+        const float k = __shfl_sync(0xffffffffu, fw, r);
+#pragma unroll
+        for (int j = 0; j < E; ++j) a[r][j] *= k;
     }
     auto put = [&](int y) {
 #pragma unroll
@@ -231,9 +276,9 @@ __device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int h
         for (int r = 0; r < RM; ++r)
 #pragma unroll
             for (int j = 0; j < E; j += 2) {
-                const float2 v = *reinterpret_cast<const float2*>(merge + (y * RM + r) * D + lane * E + j);
-                a[r][j] += v.x;
-                a[r][j + 1] += v.y;
+                const float2 t = *reinterpret_cast<const float2*>(merge + (y * RM + r) * D + lane * E + j);
+                a[r][j] += t.x;
+                a[r][j + 1] += t.y;
             }
     };
     if (warp >= 2) put(warp - 2);
@@ -244,19 +289,22 @@ __device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int h
     if (warp == 0) {
         add(1);
 #pragma unroll
-        for (int r = 0; r < RM; ++r)
-            if (r < rows) store_row<T, E>(sp.a, hk, first, r, lane, a[r], *reinterpret_cast<const float4*>(wstat + (RM + r) * 4));
+        for (int r = 0; r < RM; ++r) {
+            const float4 x = make_float4(__shfl_sync(0xffffffffu, t1, r), __shfl_sync(0xffffffffu, t0, r),
+                                         __shfl_sync(0xffffffffu, all, r), 0.f);
+            if (r < rows) store_row<T, E>(sp.a, hk, first, r, lane, a[r], x);
+        }
     }
 }
 
 template <typename T, int D, bool Q8, int NT>
-__global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid_constant__ StepParams sp) {
+__global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn_step_kernel(const __grid_constant__ StepParams sp) {
     using P = StepPlan<D, Q8, NT>;
     using MT = typename std::conditional<Q8, __half, T>::type;  // the MMAs' operand type
     constexpr int NS = P::kStages, KK = D / 16, RM = P::kRowsMax;
     const AttnParams& p = sp.a;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int plan[4];  // tiles of the list, first sequence, tiles before it, CTAs with work
+    __shared__ int plan[7];
     __shared__ uint32_t last_part;
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sb = (raw + 1023u) & ~1023u;
@@ -286,43 +334,69 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
         }
         total = (int)warp_sum(total) * p.Hkv;
         units = (int)warp_sum(units) * p.Hkv;
-        // CTAs with work: with n tiles per (sequence, kv head) in P parts, a part's tiles take n / P * 0.4 us and
-        // joining P * 0.05 us, least at P = sqrt(8 n)
-        const int G = min(min((int)gridDim.x, total), (int)sqrtf(8.f * units * total) + 1);
-        int first = 0, cum0 = 0;
-        if ((int)blockIdx.x < G) {
-            const int it = (int)((int64_t)blockIdx.x * total / G);
+        // CTAs with work.  n tiles of a (sequence, kv head) in P parts take n / P * 0.75 us and, for P > 1, 3 us + P *
+        // 0.05 us to be joined: least at P = sqrt(15 n), and worth it from 6 tiles on.  P is a whole number, so that
+        // sequences of one length are cut alike, unless every CTA has 16 tiles or more.
+        const int grid = (int)gridDim.x;
+        const float n = (float)total / (float)max(units, 1);
+        int P = n < 6.f ? 1 : (int)fminf(n, sqrtf(15.f * n));
+        if (units * P > grid) P = max(1, grid / max(units, 1));
+        StepCuts cuts;
+        cuts.total = total;
+        cuts.G = max(1, min(total, total / grid >= 16 ? grid : min(grid, units * P)));
+        cuts.slack = P == 1 ? 4 : min(total / cuts.G / 2, 8);
+        // this CTA's first tile and the next one's, each with the sequence it lies in
+        int first = 0, cum0 = 0, at = total, end = total;
+        if ((int)blockIdx.x < cuts.G) {
+            const int r0 = cuts.raw(blockIdx.x), r1 = cuts.raw(blockIdx.x + 1);
             int before = 0;
-            for (int b0 = 0; b0 < p.B; b0 += 32) {
-                const int mine = b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles * p.Hkv : 0;
-                const int cum = warp_scan(mine, lane);
-                const unsigned hit = __ballot_sync(0xffffffffu, it < before + cum);
-                if (hit) {
-                    const int l = __ffs(hit) - 1;
-                    first = b0 + l;
-                    cum0 = before + __shfl_sync(0xffffffffu, cum - mine, l);
-                    break;
+            for (int b0 = 0; b0 < p.B && before <= r1; b0 += 32) {
+                const int tiles = b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
+                const int mine = tiles * p.Hkv, cum = before + warp_scan(mine, lane) - mine;
+                // (sequences' tiles are disjoint: one lane of one round at most has either)
+                const bool h0 = r0 >= cum && r0 < cum + mine, h1 = r1 >= cum && r1 < cum + mine;
+                int m0 = 0, m1 = 0;
+                if (h0) {
+                    const int base = cum + (r0 - cum) / tiles * tiles;
+                    m0 = cuts.moved(r0, base, tiles);
                 }
-                before += __shfl_sync(0xffffffffu, cum, 31);
+                if (h1) {
+                    const int base = cum + (r1 - cum) / tiles * tiles;
+                    m1 = cuts.moved(r1, base, tiles);
+                }
+                const unsigned a0 = __ballot_sync(0xffffffffu, h0), a1 = __ballot_sync(0xffffffffu, h1);
+                if (a0) {
+                    const int l = __ffs(a0) - 1;
+                    first = b0 + l;
+                    cum0 = __shfl_sync(0xffffffffu, cum, l);
+                    at = __shfl_sync(0xffffffffu, m0, l);
+                }
+                if (a1) end = __shfl_sync(0xffffffffu, m1, __ffs(a1) - 1);
+                before = __shfl_sync(0xffffffffu, cum + mine, 31);
             }
         }
         if (lane == 0) {
             plan[0] = total;
             plan[1] = first;
             plan[2] = cum0;
-            plan[3] = G;
+            plan[3] = cuts.G;
+            plan[4] = cuts.slack;
+            plan[5] = at;
+            plan[6] = end;
         }
     }
     __syncthreads();
-    const int total = plan[0], G = plan[3];
-    if ((int)blockIdx.x >= G) return;
     StepWalk w;
-    w.it = (int)((int64_t)blockIdx.x * total / G);
-    w.it1 = (int)((int64_t)(blockIdx.x + 1) * total / G);
+    w.it = plan[5];
+    w.it1 = plan[6];
+    if (w.it >= w.it1) return;
+    StepCuts cuts;
+    cuts.total = plan[0];
+    cuts.G = plan[3];
+    cuts.slack = plan[4];
     w.b = plan[1];
     w.cum = plan[2];
     w.s = step_seq(p, w.b, RM);
-    const int first_it = w.it;
 
     if (warp == 4) {
         // ------------------------------------------------------ producer
@@ -685,11 +759,9 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
         bar_sync_step();
         const bool whole = w.t0 == 0 && w.t1 == s.tiles;
         constexpr int E = D / 32;
-        const int c_first = (int)(((int64_t)(w.base + 1) * G - 1) / total);
-        const int c_last = (int)(((int64_t)(w.base + s.tiles) * G - 1) / total);
-        // the part a CTA has of this (sequence, kv head): its first segment, or (only where the
-        // sequence begins within its share) its last
-        auto slot_of = [&](int c) { return 2 * c + (c == c_first && (int)((int64_t)c * total / G) < w.base ? 1 : 0); };
+        // its parts: the one a CTA ends its share with (slot 1), then those that begin with a cut (slot 0)
+        int c_lo, c_hi;
+        cuts.inside(w.base, s.tiles, c_lo, c_hi);
         if (warp == 0) {
             add_from(1);
             unsigned bad = 0;  // rows with a value that is not finite
@@ -728,7 +800,7 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
                 }
                 __syncwarp();
             }
-            const int slot = slot_of((int)blockIdx.x);
+            const int slot = 2 * (int)blockIdx.x + (w.t0 == 0);
             for (int r = 0; r < s.rows; ++r) {
                 const float4 x = *reinterpret_cast<const float4*>(wstat + r * 4);
                 float a[E];
@@ -744,13 +816,11 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
                 }
             }
             if (!whole) {
-                __threadfence();
                 __syncwarp();
                 if (lane == 0) {
                     uint32_t* n = sp.arrived + w.b * p.Hkv + w.hk;
-                    const bool last = atomicAdd(n, 1u) == (uint32_t)(c_last - c_first);
+                    const bool last = add_acq_rel(n, 1u) == (uint32_t)(c_hi - c_lo + 1);
                     if (last) *n = 0u;  // every part is here: nobody else looks at it in this call
-                    __threadfence();
                     last_part = last;
                 }
             }
@@ -758,7 +828,7 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
         if (!whole) {
             bar_sync_step();
             if (last_part) {
-                join_parts<T, D, NT>(sp, s.rows, w.hk, s.first, c_first, c_last, slot_of, merge, wstat, warp, lane);
+                join_parts<T, D, NT>(sp, s.rows, w.hk, s.first, c_lo - 1, c_hi - c_lo + 2, merge, wstat, warp, lane);
             }
         }
     }
@@ -769,7 +839,6 @@ __global__ void __launch_bounds__(kStepThreads, 2) attn_step_kernel(const __grid
 // one finds zero.
 constexpr size_t kStepCounters = WLQ_ATTENTION_ZERO_BYTES / 4;
 
-inline int step_ctas() { return 2 * device_sm_count(); }
 
 template <typename T, int D, bool Q8, int NT>
 int launch_step(const AttnParams& a, cudaStream_t stream) {
@@ -787,7 +856,7 @@ int launch_step(const AttnParams& a, cudaStream_t stream) {
     if ((rc = encode_3d(&sp.tm_k, dt, a.k_cache, D, ps, pg, D * es, ps * D * es, box, keys, 1, sw, "k_cache")) ||
         (rc = encode_3d(&sp.tm_v, dt, a.v_cache, D, ps, pg, D * es, ps * D * es, box, keys, 1, sw, "v_cache")))
         return rc;
-    const int grid = step_ctas();
+    const int grid = P::kCtas * device_sm_count();
     sp.arrived = static_cast<uint32_t*>(a.ws);
     sp.stat = reinterpret_cast<float*>(sp.arrived + kStepCounters);
     sp.part = sp.stat + (size_t)2 * grid * P::kRowsMax * 4;
