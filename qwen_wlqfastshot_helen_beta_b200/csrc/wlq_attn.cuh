@@ -69,10 +69,22 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-__device__ __forceinline__ uint2 ldg_stream_v2(const void* p) {
-    uint2 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+// Read-only loads that are used once.  Not volatile, and called without a
+// condition (at a valid address, the value dropped where it is not wanted): a
+// load inside a branch is waited for where the branch ends, and sixteen of
+// them take sixteen round trips.
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+    uint4 r;
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+    uint2 r;
+    asm("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint4 keep_if(bool c, uint4 v) {
+    return make_uint4(c ? v.x : 0u, c ? v.y : 0u, c ? v.z : 0u, c ? v.w : 0u);
 }
 
 // 2^(e - 127), e in 1..254

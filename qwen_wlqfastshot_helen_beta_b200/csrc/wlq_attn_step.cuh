@@ -209,19 +209,21 @@ __device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int h
         float v[U][RM][E];
 #pragma unroll
         for (int y = 0; y < U; ++y) {
-            const int i = i0 + 4 * y;
+            // past the last part: the last one, without weight; past the last row: whatever the slot holds, not used
+            const int i = min(i0 + 4 * y, parts - 1);
             const int64_t at = (int64_t)(2 * (c0 + i) + (i == 0)) * RM;
-            const bool in = i < parts;
-            x[y] = in && lane < rows ? ldcg4(sp.stat + (at + lane) * 4) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+            x[y] = ldcg4(sp.stat + (at + (lane & (RM - 1))) * 4);
 #pragma unroll
             for (int r = 0; r < RM; ++r)
 #pragma unroll
                 for (int j = 0; j < E; j += 2) {
-                    float2 t = make_float2(0.f, 0.f);
-                    if (in && r < rows) t = ldcg2(sp.part + (at + r) * D + lane * E + j);
+                    const float2 t = ldcg2(sp.part + (at + r) * D + lane * E + j);
                     v[y][r][j] = t.x, v[y][r][j + 1] = t.y;
                 }
         }
+#pragma unroll
+        for (int y = 0; y < U; ++y)
+            if (i0 + 4 * y >= parts || lane >= rows) x[y] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
         float b1 = a1, b0 = a0;
 #pragma unroll
         for (int y = 0; y < U; ++y) b1 = fmaxf(b1, x[y].x), b0 = fmaxf(b0, x[y].y);
@@ -243,7 +245,7 @@ __device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int h
             for (int y = 0; y < U; ++y) {
                 const float g = __shfl_sync(0xffffffffu, f[y], r);
 #pragma unroll
-                for (int j = 0; j < E; ++j) a[r][j] += v[y][r][j] * g;
+                for (int j = 0; j < E; ++j) a[r][j] += g == 0.f ? 0.f : v[y][r][j] * g;
             }
         }
     }
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
                 uint4 v[C];
                 float f[C][8], top = 0.f;
 #pragma unroll
-                for (int x = 0; x < C; ++x) v[x] = in ? ldg_stream_v4(src + tq * (D / 4) + 8 * x) : make_uint4(0u, 0u, 0u, 0u);
+                for (int x = 0; x < C; ++x) v[x] = keep_if(in, ldg16(src + tq * (D / 4) + 8 * x));
 #pragma unroll
                 for (int x = 0; x < C; ++x) {
                     const uint32_t u[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
@@ -504,8 +506,10 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
 #pragma unroll
                 for (int k = 0; k < KK; ++k)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        qf[nt][k][i] = in ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * tq + 8 * i) : 0u;
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t v = *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * tq + 8 * i);
+                        qf[nt][k][i] = in ? v : 0u;
+                    }
                 fac[nt][0] = fac[nt][1] = p.scale_log2;
             }
 #pragma unroll

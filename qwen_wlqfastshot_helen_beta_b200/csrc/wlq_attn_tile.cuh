@@ -265,13 +265,13 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
     const uint32_t bars = sb + P::kBarOff;
     const uint32_t q_full = bars, v_fixed = bars + 8u;
     auto s_full = [&](int t) { return bars + 8u * (2 + t); };    // scores of half t are in TMEM
-    auto p_full = [&](int t) { return bars + 8u * (4 + t); };    // its probabilities are
-    auto pv_done = [&](int t) { return bars + 8u * (6 + t); };   // its output has the tile's part
-    auto full = [&](int s) { return bars + 8u * (8 + s); };
-    auto empty = [&](int s) { return bars + 8u * (8 + NS + s); };
-    auto st_full = [&](int s) { return bars + 8u * (8 + 2 * NS + s); };
-    auto st_empty = [&](int s) { return bars + 8u * (8 + 2 * NS + NST + s); };
-    const uint32_t tmem_slot = bars + 8u * (8 + 2 * NS + 2 * NST);
+    auto p_full = [&](int t, int h) { return bars + 8u * (4 + 2 * t + h); };  // probabilities of its keys 64 h .. are
+    auto pv_done = [&](int t) { return bars + 8u * (8 + t); };   // its output has the tile's part
+    auto full = [&](int s) { return bars + 8u * (10 + s); };
+    auto empty = [&](int s) { return bars + 8u * (10 + NS + s); };
+    auto st_full = [&](int s) { return bars + 8u * (10 + 2 * NS + s); };
+    auto st_empty = [&](int s) { return bars + 8u * (10 + 2 * NS + NST + s); };
+    const uint32_t tmem_slot = bars + 8u * (10 + 2 * NS + 2 * NST);
     auto slot = [&](int s) { return sb + P::kKvOff + s * P::kTileBytes; };
     auto stage = [&](int s) { return sb + P::kStageOff + s * P::kStageBytes; };
 
@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
         mbar_init(v_fixed, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(s_full(t), 1);
-            mbar_init(p_full(t), 4);
+            mbar_init(p_full(t, 0), 4);
+            mbar_init(p_full(t, 1), 4);
             mbar_init(pv_done(t), 1);
         }
         for (int s = 0; s < NS; ++s) {
@@ -329,21 +330,27 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
         const int t = warp >> 2;
         const int r = threadIdx.x;           // row of the CTA
         const int row = u.row0 + r;          // row of the sequence
-        // q rows, 16 bytes a lane: a row's chunks are next to one another
+        // q rows, 16 bytes a lane, a row's chunks next to one another; all of a thread's loads in flight together
         {
-            constexpr int C = D / 8;
-            const int rt0 = t * kRowsT;
-            for (int i = threadIdx.x & 127; i < kRowsT * C; i += 128) {
-                const int rr = i / C, c = i % C;
-                const int rw = u.row0 + rt0 + rr;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (rw < u.rows) {
-                    const int tk = rw / p.G;
-                    const int h = u.hk * p.G + (rw - tk * p.G);
-                    v = ldg_stream_v4(p.q + (int64_t)(u.first + tk) * p.q_tok + h * p.q_head + c * 8);
+            constexpr int C = D / 8, S = 128 / C;  // chunks of a row; rows of one round
+            const int ch = (int)(threadIdx.x & 127) % C, r0 = (int)(threadIdx.x & 127) / C;
+            int tk = (u.row0 + t * kRowsT + r0) / p.G, hh = u.row0 + t * kRowsT + r0 - tk * p.G;
+            const int qs = S / p.G, rs = S - qs * p.G;
+            uint4 v[C];
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const bool in = u.row0 + t * kRowsT + r0 + i * S < u.rows;
+                v[i] = keep_if(in, ldg16(p.q + (int64_t)(u.first + (in ? tk : 0)) * p.q_tok +
+                                         (u.hk * p.G + hh) * p.q_head + ch * 8));
+                tk += qs;
+                hh += rs;
+                if (hh >= p.G) {
+                    hh -= p.G;
+                    ++tk;
                 }
-                sts128(sb + t * P::kTileBytes + tile_chunk(rr, c), v);
             }
+#pragma unroll
+            for (int i = 0; i < C; ++i) sts128(sb + t * P::kTileBytes + tile_chunk(r0 + i * S, ch), v[i]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
@@ -419,11 +426,11 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                         w[j] = pack2<T>(a, b);
                     }
                     tmem_st_32x32b_x32(ts + 32 * k, w);
+                    tmem_st_wait();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full(t, k));
                 }
-                tmem_st_wait();
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(t));
             }
             // ------------------------------------------------------ output
             float la, lb;
@@ -432,9 +439,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
             if (n > 0 && ok) ok = warp_wait(pv_done(t), (n - 1) & 1);
             tc_fence_after_sync();
             const bool mine = row < u.rows;
-            const int tk = row / p.G, h = u.hk * p.G + (row - tk * p.G);
             const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-            uint16_t* dst = p.out + (int64_t)(u.first + tk) * p.o_tok + h * p.o_head;
             float* pdst = u.slot < 0 ? nullptr : tp.part + ((int64_t)u.slot * kRows + r) * D;
             float bad = 0.f;
 #pragma unroll 1
@@ -458,14 +463,36 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     for (int j = 0; j < 8; ++j)
                         *reinterpret_cast<float4*>(pdst + 32 * k + 4 * j) =
                             make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-                } else if (mine) {
+                } else {
+                    // through this half's q tile, which no MMA reads any more
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        *reinterpret_cast<uint4*>(dst + 32 * k + 8 * j) =
-                            make_uint4(pack2<T>(f[8 * j] * inv, f[8 * j + 1] * inv),
-                                       pack2<T>(f[8 * j + 2] * inv, f[8 * j + 3] * inv),
-                                       pack2<T>(f[8 * j + 4] * inv, f[8 * j + 5] * inv),
-                                       pack2<T>(f[8 * j + 6] * inv, f[8 * j + 7] * inv));
+                        sts128(sb + t * P::kTileBytes + tile_chunk(r & 127, 4 * k + j),
+                               make_uint4(pack2<T>(f[8 * j] * inv, f[8 * j + 1] * inv),
+                                          pack2<T>(f[8 * j + 2] * inv, f[8 * j + 3] * inv),
+                                          pack2<T>(f[8 * j + 4] * inv, f[8 * j + 5] * inv),
+                                          pack2<T>(f[8 * j + 6] * inv, f[8 * j + 7] * inv)));
+                }
+                __syncwarp();
+            }
+            if (!pdst) {
+                // a warp's 32 rows, their 16-byte chunks next to one another
+                constexpr int C = D / 8, S = 32 / C;
+                const int ch = lane % C, rw = (r & ~31) + lane / C;
+                int tw = (u.row0 + rw) / p.G, hw = u.row0 + rw - tw * p.G;
+                const int qs = S / p.G, rs = S - qs * p.G;
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    const uint4 x = lds128(sb + t * P::kTileBytes + tile_chunk((rw + i * S) & 127, ch));
+                    if (u.row0 + rw + i * S < u.rows)
+                        *reinterpret_cast<uint4*>(p.out + (int64_t)(u.first + tw) * p.o_tok +
+                                                  (u.hk * p.G + hw) * p.o_head + ch * 8) = x;
+                    tw += qs;
+                    hw += rs;
+                    if (hw >= p.G) {
+                        hw -= p.G;
+                        ++tw;
+                    }
                 }
                 __syncwarp();
             }
@@ -531,12 +558,16 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                 if (!(ok = mbar_wait(full(sv), (gv / NS) & 1))) break;
                 if (SRC != kPaged8 && i == n - 1 && last_keys < kKeys && !(ok = mbar_wait(v_fixed, 0))) break;
                 for (int t = 0; ok && t < halves; ++t) {
-                    if (!(ok = mbar_wait(p_full(t), i & 1))) break;
-                    tc_fence_after_sync();
+                    // the first 64 keys' products run while the other probabilities are computed
+                    for (int h = 0; ok && h < 2; ++h) {
+                        if (!(ok = mbar_wait(p_full(t, h), i & 1))) break;
+                        tc_fence_after_sync();
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k,
-                                    umma_desc_mn_sw128(slot(sv) + k * 2048, P::kBlock), id_o, i > 0 || k > 0);
+                        for (int k = 4 * h; k < 4 * h + 4; ++k)
+                            umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k,
+                                        umma_desc_mn_sw128(slot(sv) + k * 2048, P::kBlock), id_o, i > 0 || k > 0);
+                    }
+                    if (!ok) break;
                     umma_commit(pv_done(t));
                     if (i + 1 < n) {
                         if (t == 0 && !(ok = mbar_wait(full(sk), (gk / NS) & 1))) break;
@@ -628,13 +659,10 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     uint32_t e[C];
 #pragma unroll
                     for (int x = 0; x < C; ++x) {
-                        const int r = r0 + x * (128 / C);
-                        e[x] = 0;
-                        if (r < keys) {
-                            const int id = p.table[(int64_t)u.b * p.table_cols + ((kb + r) >> p.log2_page)];
-                            if (id >= 0 && id < p.num_pages)
-                                e[x] = exps[((int64_t)id * p.Hkv + u.hk) * p.page_size + ((kb + r) & (p.page_size - 1))];
-                        }
+                        const int key = min(kb + r0 + x * (128 / C), u.len - 1);
+                        const int id = p.table[(int64_t)u.b * p.table_cols + (key >> p.log2_page)];
+                        const bool in = id >= 0 && id < p.num_pages;
+                        e[x] = exps[((int64_t)(in ? id : 0) * p.Hkv + u.hk) * p.page_size + (key & (p.page_size - 1))];
                     }
                     if (!(ok = warp_wait(st_full(st), (g / NST) & 1))) break;
                     if (g >= NS && !(ok = warp_wait(empty(s), (g / NS - 1) & 1))) break;

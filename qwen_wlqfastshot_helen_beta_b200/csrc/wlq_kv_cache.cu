@@ -115,15 +115,13 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kv_write_kernel(const RopeP
         const int kind = h < p.Hq ? 0 : (h < p.Hq + p.Hkv ? 1 : 2);  // q, k, v
         const int hh = kind == 0 ? h : (kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv);
         float a[8], b[8];
-        if (ok) {
+        {
             const uint16_t* src = kind == 0   ? p.q + tok * p.q_tok + hh * p.q_head
                                   : kind == 1 ? p.k + tok * p.k_tok + hh * p.k_head
                                               : p.v + tok * p.v_tok + hh * p.v_head;
-            unpack8<T>(ldg_stream_v4(src + 8 * ca), a);
-            unpack8<T>(ldg_stream_v4(src + 8 * cb), b);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+            if (!ok) src = p.q + tok * p.q_tok;
+            unpack8<T>(keep_if(ok, ldg16(src + (ok ? 8 * ca : 0))), a);
+            unpack8<T>(keep_if(ok, ldg16(src + (ok ? 8 * cb : 0))), b);
         }
         if (kind != 2) {
             if (p.interleaved) {
@@ -237,23 +235,21 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const KvReadParam
             const int h = __umulhi((uint32_t)e, p.chunk_magic);
             const int c = e - h * (p.D >> 3);
             const int64_t r = base[tk];
-            uint4 o = make_uint4(0u, 0u, 0u, 0u);
-            if (r >= 0) {
-                const int64_t row = r + (int64_t)h * p.page_size;
-                if constexpr (QUANT) {
-                    const uint2 q = ldg_stream_v2(src + row * p.D + 8 * c);
-                    const float s = exp2_biased(exps[row]);
-                    float f[8];
-                    e4m3x4_to_f32(q.x, f);
-                    e4m3x4_to_f32(q.y, f + 4);
+            const int64_t row = r < 0 ? 0 : r + (int64_t)h * p.page_size;
+            uint4 o;
+            if constexpr (QUANT) {
+                const uint2 q = ldg8(src + row * p.D + 8 * c);
+                const float s = exp2_biased(__ldg(exps + row));
+                float f[8];
+                e4m3x4_to_f32(q.x, f);
+                e4m3x4_to_f32(q.y, f + 4);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] *= s;
-                    o = pack8<T>(f);
-                } else {
-                    o = ldg_stream_v4(src + (row * p.D + 8 * c) * 2);
-                }
+                for (int j = 0; j < 8; ++j) f[j] *= s;
+                o = pack8<T>(f);
+            } else {
+                o = ldg16(src + (row * p.D + 8 * c) * 2);
             }
-            *reinterpret_cast<uint4*>(dst + (int64_t)i * 8) = o;
+            *reinterpret_cast<uint4*>(dst + (int64_t)i * 8) = keep_if(r >= 0, o);
         }
     }
 }
