@@ -138,6 +138,7 @@ int wlq_prompt_attention(const void* q, const void* k, const void* v, const int3
     if (T < 0 || B < 0) return fail(WLQ_ERR_INVALID_ARG, "%s: negative size", fn);
     if ((rc = bad_dtype(fn, act_dtype)) || (rc = bad_heads(fn, Hq, Hkv))) return rc;
     if (D != 64 && D != 128) return fail(WLQ_ERR_UNSUPPORTED, "%s: head size must be 64 or 128 (got %d)", fn, D);
+    if (Hq / Hkv > 128) return fail(WLQ_ERR_UNSUPPORTED, "%s: at most 128 query heads per kv head (got %d)", fn, Hq / Hkv);
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail(WLQ_ERR_INVALID_ARG, "%s: scale must be positive and finite", fn);
     if (T == 0) return WLQ_OK;
     if (B < 1 || !cu_seqlens) return fail(WLQ_ERR_INVALID_ARG, "%s: cu_seqlens is required", fn);
@@ -175,6 +176,7 @@ int wlq_paged_attention(const void* q, const void* k_cache, const void* v_cache,
     if (T < 0 || B < 0 || table_cols < 0 || max_q < 1) return fail(WLQ_ERR_INVALID_ARG, "%s: bad size", fn);
     if ((rc = bad_dtype(fn, act_dtype)) || (rc = bad_heads(fn, Hq, Hkv))) return rc;
     if (D != 64 && D != 128) return fail(WLQ_ERR_UNSUPPORTED, "%s: head size must be 64 or 128 (got %d)", fn, D);
+    if (Hq / Hkv > 128) return fail(WLQ_ERR_UNSUPPORTED, "%s: at most 128 query heads per kv head (got %d)", fn, Hq / Hkv);
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail(WLQ_ERR_INVALID_ARG, "%s: scale must be positive and finite", fn);
     if ((rc = bad_cache(fn, k_cache, v_cache, k_exp, v_exp, num_pages, page_size))) return rc;
     if (T == 0) return WLQ_OK;

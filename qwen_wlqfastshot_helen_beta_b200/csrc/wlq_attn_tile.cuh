@@ -10,22 +10,23 @@
 // and the sum is fp32), and after the first tiles the accumulator is hardly
 // ever touched.
 //
-// The rows of a CTA are the new tokens of one sequence times the G query
-// heads of one kv head, token-major, so that a short prompt or a chunk of few
-// tokens fills its tiles whatever G is, and every row of a tile needs about
-// the same keys.
+// A tile's 128 rows are whole tokens of one sequence times the G query heads
+// of one kv head, token-major (128 / G tokens, rounded down), so that a short
+// prompt or a chunk of few tokens fills its tiles whatever G is, every row of
+// a tile needs about the same keys, and q comes and the output goes as one
+// TMA box of tokens x heads.
 //
 // Roles (one CTA per SM):
 //   warps 0..3, 4..7  softmax of rows 0..127 and 128..255, a thread per row:
 //                     scores TMEM -> registers, maximum, exponentials, the
 //                     16-bit probabilities back into TMEM over the scores;
-//                     they load q at the start and write the output at the end
+//                     the output through the q tile's shared memory
 //   warp 8            issues the MMAs: S = Q K^T (both from shared memory),
 //                     O += P V (P from TMEM).  The order P0 V, S0, P1 V, S1
 //                     lets the tensor cores work on one half's tiles while
 //                     the other half's softmax runs
-//   warp 9            TMA producer of the k and v tiles: packed rows, or one
-//                     copy per page
+//   warp 9            TMA producer of q and of the k and v tiles: packed rows,
+//                     or one copy per page
 //   warps 12..15      8-bit caches: the pages' codes land in a staging ring
 //                     and are written as the 16-bit tiles the MMAs read,
 //                     code * 2^e, which is exact
@@ -46,11 +47,12 @@ constexpr int kRows = 256;    // query rows of one CTA
 constexpr int kKeys = 128;    // keys of one tile
 
 struct TileParams {
-    CUtensorMap tm_k, tm_v;
+    CUtensorMap tm_q, tm_o, tm_k, tm_v;
     AttnParams a;
-    float* part;  // [split CTAs][kRows][D] unnormalised outputs of a part of the keys
+    float* part;  // [split CTAs][D / 4][kRows][4] unnormalised outputs of a part of the keys
     float* stat;  // [split CTAs][kRows][2] their row maxima (times c) and sums
     int sms;
+    int nt;       // tokens of a tile: 128 / G
 };
 
 template <int D, int SRC>
@@ -80,20 +82,20 @@ struct TilePlan {
 // What one CTA works on.
 struct Unit {
     int b, hk;        // sequence, kv head
-    int row0, rows;   // its first row in the sequence, rows of the sequence
+    int tok0, n;      // its first token in the sequence, tokens of the sequence
     int first;        // first query token of the sequence in q
-    int past;         // keys a row of the first token does not count itself: row r sees keys <= past + r / G
+    int past;         // token t sees keys <= past + t
     int len;          // keys of the sequence
     int tile0, tiles; // key tiles [tile0, tile0 + tiles)
     int slot;         // partial result slot, or -1: the whole row is here
 };
 
 struct Seq {
-    int rows, tiles, rtiles, len, n, first;
+    int tiles, rtiles, len, n, first;
 };
 
 template <bool PAGED>
-__device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
+__device__ __forceinline__ Seq seq_of(const AttnParams& p, int nt, int b) {
     Seq s;
     if (p.cu) {
         s.first = p.cu[b];
@@ -106,44 +108,63 @@ __device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
     if (s.first < 0 || s.n < 0 || (int64_t)s.first + s.n > p.T) s.n = 0;
     s.len = s.n;
     if (PAGED) s.len = (int)max((int64_t)0, min((int64_t)p.kv_lens[b], p.table_cols << p.log2_page));
-    s.rows = s.n * p.G;
-    s.rtiles = (s.rows + kRows - 1) / kRows;
+    s.rtiles = (s.n + 2 * nt - 1) / (2 * nt);
     s.tiles = (s.len + kKeys - 1) / kKeys;
     return s;
 }
 
-// Parts of a sequence's keys: as many CTAs as fill the device once, shared
-// out in proportion to the keys, none with less than 4 tiles.
-__device__ __forceinline__ int splits_of(const Seq& s, int64_t work, int sms) {
-    if (s.rtiles == 0) return 0;
-    const int most = (int)min((int64_t)s.tiles * sms / max(work, (int64_t)1), (int64_t)s.tiles / 4);
-    return max(1, most);
-}
+constexpr int kPartsPerSm = 3;  // CTAs that hold a part of their rows' keys, at most
 
-// Key tiles times row tiles of all sequences (paged form), by one warp.
-__device__ __forceinline__ int64_t total_work(const AttnParams& p, int lane) {
-    int64_t w = 0;
-    for (int b = lane; b < p.B; b += 32) {
-        const Seq s = seq_of<true>(p, b);
-        w += (int64_t)s.rtiles * s.tiles;
+// Key tiles of one part (paged form), found by one warp: a sequence with more
+// tiles is shared by several CTAs.  Up to 32 sequences: of 16 sizes the one
+// with the least waves of CTAs times a part's duration (its tiles, about 3
+// more for starting and ending, and once 6 for joining the parts).  More
+// sequences: an even share of all tiles.
+__device__ __forceinline__ int tiles_per_part(const AttnParams& p, int nt, int sms, int lane) {
+    if (p.B > 32) {
+        int64_t w = 0;
+        for (int b = lane; b < p.B; b += 32) {
+            const Seq s = seq_of<true>(p, nt, b);
+            w += (int64_t)s.rtiles * s.tiles;
+        }
+        return (int)max((int64_t)4, (warp_sum(w) * p.Hkv + sms - 1) / sms);
     }
-    return warp_sum(w) * p.Hkv;
+    Seq s{};
+    if (lane < p.B) s = seq_of<true>(p, nt, lane);
+    const int most = __reduce_max_sync(0xffffffffu, s.rtiles ? s.tiles : 0);
+    const int units = s.rtiles * p.Hkv;
+    int best = most, cost = 0x7fffffff;
+    for (int parts = 1; parts <= 64; parts += parts < 8 ? 1 : parts / 4) {
+        const int per = (most + parts - 1) / parts;
+        if (parts > 1 && per < 4) break;
+        const int sp = (s.tiles + per - 1) / max(per, 1);
+        const int ctas = __reduce_add_sync(0xffffffffu, units * max(sp, 1));
+        const int shared = __reduce_add_sync(0xffffffffu, sp > 1 ? units * sp : 0);
+        if (shared > kPartsPerSm * sms) break;
+        const int c = (ctas + sms - 1) / sms * (per + 3) + (shared ? 6 : 0);
+        if (c < cost) {
+            cost = c;
+            best = per;
+        }
+    }
+    return max(best, 1);
 }
+__device__ __forceinline__ int parts_of(const Seq& s, int per) { return s.rtiles ? max(1, (s.tiles + per - 1) / per) : 0; }
 
 // The work of CTA c, found by one warp: sequences in order, row tiles from
 // the last (the longest, where the mask is causal) to the first, then parts
 // of the keys, then heads.  False if there is none.
 template <bool PAGED>
-__device__ __forceinline__ bool find_unit(const AttnParams& p, int sms, int c, int lane, Unit& u) {
-    const int64_t work = PAGED ? total_work(p, lane) : 0;
+__device__ __forceinline__ bool find_unit(const AttnParams& p, int nt, int sms, int c, int lane, Unit& u) {
+    const int per = PAGED ? tiles_per_part(p, nt, sms, lane) : 0;
     int before = 0, slots = 0;  // CTAs of earlier sequences, those of them that hold parts
     for (int b0 = 0; b0 < p.B; b0 += 32) {
         const int b = b0 + lane;
         Seq s{};
         int sp = 0;
         if (b < p.B) {
-            s = seq_of<PAGED>(p, b);
-            sp = PAGED ? splits_of(s, work, sms) : (s.rtiles ? 1 : 0);
+            s = seq_of<PAGED>(p, nt, b);
+            sp = PAGED ? parts_of(s, per) : (s.rtiles ? 1 : 0);
         }
         const int mine = s.rtiles * sp * p.Hkv, part = sp > 1 ? mine : 0;
         const int cum = warp_scan(mine, lane), pcum = warp_scan(part, lane);
@@ -153,7 +174,6 @@ __device__ __forceinline__ bool find_unit(const AttnParams& p, int sms, int c, i
             const int x = c - before - __shfl_sync(0xffffffffu, cum - mine, l);  // CTA within the sequence
             const int slot0 = slots + __shfl_sync(0xffffffffu, pcum - part, l);
             sp = __shfl_sync(0xffffffffu, sp, l);
-            s.rows = __shfl_sync(0xffffffffu, s.rows, l);
             s.rtiles = __shfl_sync(0xffffffffu, s.rtiles, l);
             s.tiles = __shfl_sync(0xffffffffu, s.tiles, l);
             s.len = __shfl_sync(0xffffffffu, s.len, l);
@@ -163,18 +183,16 @@ __device__ __forceinline__ bool find_unit(const AttnParams& p, int sms, int c, i
             u.hk = x % p.Hkv;
             const int y = x / p.Hkv;
             const int part_no = y % sp;
-            u.row0 = (s.rtiles - 1 - y / sp) * kRows;
-            u.rows = s.rows;
+            u.tok0 = (s.rtiles - 1 - y / sp) * 2 * nt;
+            u.n = s.n;
             u.first = s.first;
             u.len = s.len;
             u.past = s.len - s.n;
-            // keys the last row of the tile sees
-            const int last = (min(u.row0 + kRows, s.rows) - 1) / p.G;
-            const int seen = p.causal ? max(0, min(s.len, u.past + last + 1)) : s.len;
+            // keys the last token sees
+            const int seen = p.causal ? max(0, min(s.len, u.past + min(u.tok0 + 2 * nt, s.n))) : s.len;
             const int need = (seen + kKeys - 1) / kKeys;
-            const int per = (s.tiles + sp - 1) / sp;
-            u.tile0 = min(need, part_no * per);
-            u.tiles = min(need, u.tile0 + per) - u.tile0;
+            u.tile0 = sp > 1 ? min(need, part_no * per) : 0;
+            u.tiles = (sp > 1 ? min(need, u.tile0 + per) : need) - u.tile0;
             u.slot = sp > 1 ? slot0 + x : -1;
             return true;
         }
@@ -223,6 +241,28 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_wait() {  // until this thread's stores have read their source
+    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+// Barrier of one half's 128 softmax threads; whether `v` holds for any.
+__device__ __forceinline__ bool bar_or_half(int t, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v), "r"(1 + t)
+        : "memory");
+    return r != 0;
+}
 
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ uint64_t f2_pack(float a, float b) {
@@ -278,14 +318,14 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
         Unit u;
-        const bool any = find_unit<kPagedSrc>(p, tp.sms, (int)blockIdx.x, lane, u);
+        const bool any = find_unit<kPagedSrc>(p, tp.nt, tp.sms, (int)blockIdx.x, lane, u);
         if (lane == 0) {
             su = u;
             work_here = any;
         }
     }
     if (threadIdx.x == 32) {
-        mbar_init(q_full, 8);
+        mbar_init(q_full, 1);
         mbar_init(v_fixed, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(s_full(t), 1);
@@ -302,8 +342,10 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
             mbar_init(st_empty(s), 4);
         }
         mbar_fence_init();
+        tma_prefetch_desc(&tp.tm_q);
         tma_prefetch_desc(&tp.tm_k);
         tma_prefetch_desc(&tp.tm_v);
+        tma_prefetch_desc(&tp.tm_o);
     }
     __syncthreads();
     if (!work_here) return;
@@ -317,7 +359,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sgen + P::kBarOff + (tmem_slot - bars));
     const Unit u = su;
     const int n = u.tiles;
-    const int halves = u.row0 + kRowsT < u.rows ? 2 : 1;
+    const int halves = u.tok0 + tp.nt < u.n ? 2 : 1;
     const int key0 = u.tile0 * kKeys;
     // keys past the sequence's end in the last tile here
     const int last_keys = min(kKeys, u.len - (key0 + (n - 1) * kKeys));
@@ -328,39 +370,16 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
     if (warp < 8) {
         // ------------------------------------------------------- softmax
         const int t = warp >> 2;
-        const int r = threadIdx.x;           // row of the CTA
-        const int row = u.row0 + r;          // row of the sequence
-        // q rows, 16 bytes a lane, a row's chunks next to one another; all of a thread's loads in flight together
-        {
-            constexpr int C = D / 8, S = 128 / C;  // chunks of a row; rows of one round
-            const int ch = (int)(threadIdx.x & 127) % C, r0 = (int)(threadIdx.x & 127) / C;
-            int tk = (u.row0 + t * kRowsT + r0) / p.G, hh = u.row0 + t * kRowsT + r0 - tk * p.G;
-            const int qs = S / p.G, rs = S - qs * p.G;
-            uint4 v[C];
-#pragma unroll
-            for (int i = 0; i < C; ++i) {
-                const bool in = u.row0 + t * kRowsT + r0 + i * S < u.rows;
-                v[i] = keep_if(in, ldg16(p.q + (int64_t)(u.first + (in ? tk : 0)) * p.q_tok +
-                                         (u.hk * p.G + hh) * p.q_head + ch * 8));
-                tk += qs;
-                hh += rs;
-                if (hh >= p.G) {
-                    hh -= p.G;
-                    ++tk;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < C; ++i) sts128(sb + t * P::kTileBytes + tile_chunk(r0 + i * S, ch), v[i]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        }
+        const int r = threadIdx.x & 127;  // row of the tile
+        const int tok = u.tok0 + t * tp.nt + r / p.G;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * D + lanes;
         const float c = p.scale_log2;
         // the row's last visible key, and the first one any row of the half cannot see
-        const int lim = p.causal ? min(u.len - 1, u.past + row / p.G) : u.len - 1;
-        const int lim0 = p.causal ? min(u.len - 1, u.past + (u.row0 + t * kRowsT) / p.G) : u.len - 1;
+        const int lim = p.causal ? min(u.len - 1, u.past + tok) : u.len - 1;
+        const int lim0 = p.causal ? min(u.len - 1, u.past + u.tok0 + t * tp.nt) : u.len - 1;
+        // rows past the tile's tokens or the sequence compute whatever is there, and have no say in the others'
+        const bool mine = r < tp.nt * p.G && tok < u.n;
         float m = -INFINITY;
         uint64_t l2 = f2_pack(0.f, 0.f);
         bool ok = true;
@@ -389,7 +408,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     mx[k] = fmaxf(mx[k], __uint_as_float(s[k][31]));
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
+                if (__any_sync(0xffffffffu, mine && (top - m) * c > 8.f)) {
                     const float mn = fmaxf(m, top);
                     const float f = mn == m ? 1.f : ex2((m - mn) * c);
                     m = mn;
@@ -438,90 +457,102 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
             float l = la + lb;
             if (n > 0 && ok) ok = warp_wait(pv_done(t), (n - 1) & 1);
             tc_fence_after_sync();
-            const bool mine = row < u.rows;
             const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-            float* pdst = u.slot < 0 ? nullptr : tp.part + ((int64_t)u.slot * kRows + r) * D;
+            float4* pdst = u.slot < 0 ? nullptr
+                                      : reinterpret_cast<float4*>(tp.part) + (int64_t)u.slot * (D / 4) * kRows + t * kRowsT + r;
+            const uint32_t tile = sb + t * P::kTileBytes;  // this half's q, which no MMA reads any more
             float bad = 0.f;
 #pragma unroll 1
-            for (int k = 0; k < D / 32; ++k) {
-                uint32_t o[32];
+            for (int k = 0; k < D / 64; ++k) {
+                uint32_t o[2][32];
                 if (n > 0) {
-                    tmem_ld_32x32b_x32(to + 32 * k, o);
+                    tmem_ld_32x32b_x32(to + 64 * k, o[0]);
+                    tmem_ld_32x32b_x32(to + 64 * k + 32, o[1]);
                     tmem_ld_wait();
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = 0u;
+                    for (int j = 0; j < 32; ++j) o[0][j] = o[1][j] = 0u;
                 }
-                float f[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    f[j] = __uint_as_float(o[j]);
-                    bad = fmaf(f[j], 0.f, bad);  // NaN where a value is not finite
-                }
-                if (mine && pdst) {
+                for (int y = 0; y < 2; ++y) {
+                    float f[32];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        *reinterpret_cast<float4*>(pdst + 32 * k + 4 * j) =
-                            make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-                } else {
-                    // through this half's q tile, which no MMA reads any more
+                    for (int j = 0; j < 32; ++j) {
+                        f[j] = __uint_as_float(o[y][j]);
+                        bad = fmaf(f[j], 0.f, bad);  // NaN where a value is not finite
+                    }
+                    if (pdst) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        sts128(sb + t * P::kTileBytes + tile_chunk(r & 127, 4 * k + j),
-                               make_uint4(pack2<T>(f[8 * j] * inv, f[8 * j + 1] * inv),
-                                          pack2<T>(f[8 * j + 2] * inv, f[8 * j + 3] * inv),
-                                          pack2<T>(f[8 * j + 4] * inv, f[8 * j + 5] * inv),
-                                          pack2<T>(f[8 * j + 6] * inv, f[8 * j + 7] * inv)));
-                }
-                __syncwarp();
-            }
-            if (!pdst) {
-                // a warp's 32 rows, their 16-byte chunks next to one another
-                constexpr int C = D / 8, S = 32 / C;
-                const int ch = lane % C, rw = (r & ~31) + lane / C;
-                int tw = (u.row0 + rw) / p.G, hw = u.row0 + rw - tw * p.G;
-                const int qs = S / p.G, rs = S - qs * p.G;
+                        for (int j = 0; j < 8; ++j)
+                            pdst[(16 * k + 8 * y + j) * kRows] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                    } else {
 #pragma unroll
-                for (int i = 0; i < C; ++i) {
-                    const uint4 x = lds128(sb + t * P::kTileBytes + tile_chunk((rw + i * S) & 127, ch));
-                    if (u.row0 + rw + i * S < u.rows)
-                        *reinterpret_cast<uint4*>(p.out + (int64_t)(u.first + tw) * p.o_tok +
-                                                  (u.hk * p.G + hw) * p.o_head + ch * 8) = x;
-                    tw += qs;
-                    hw += rs;
-                    if (hw >= p.G) {
-                        hw -= p.G;
-                        ++tw;
+                        for (int j = 0; j < 4; ++j)
+                            sts128(tile + tile_chunk(r, 8 * k + 4 * y + j),
+                                   make_uint4(pack2<T>(f[8 * j] * inv, f[8 * j + 1] * inv),
+                                              pack2<T>(f[8 * j + 2] * inv, f[8 * j + 3] * inv),
+                                              pack2<T>(f[8 * j + 4] * inv, f[8 * j + 5] * inv),
+                                              pack2<T>(f[8 * j + 6] * inv, f[8 * j + 7] * inv)));
                     }
                 }
-                __syncwarp();
             }
-            if (mine && pdst) {
-                float* st = tp.stat + ((int64_t)u.slot * kRows + r) * 2;
-                st[0] = m * c;
-                st[1] = l;
-            }
+            if (pdst)
+                *reinterpret_cast<float2*>(tp.stat + ((int64_t)u.slot * kRows + t * kRowsT + r) * 2) = make_float2(m * c, l);
             // rows that values behind the mask may have spoilt
             const bool masked = key0 + n * kKeys - 1 > lim;
             unsigned again = __ballot_sync(0xffffffffu, ok && mine && masked && bad != bad);
+            if (!pdst) {
+                fence_proxy_async_smem();
+                const bool plain = bar_or_half(t, again != 0 || !ok) || u.tok0 + (t + 1) * tp.nt > u.n;
+                if (!plain) {
+                    if (r == 0) {
+#pragma unroll
+                        for (int h = 0; h < P::kHalves; ++h)
+                            tma_store_3d(&tp.tm_o, tile + h * P::kBlock, h * 64, u.hk * p.G, u.first + u.tok0 + t * tp.nt);
+                        tma_store_wait();
+                    }
+                } else {
+                    // the sequence ends inside the tile (or rows follow): a warp's 32 rows, chunk by chunk
+                    constexpr int C = D / 8, S = 32 / C;
+                    const int ch = lane % C, rw = (r & ~31) + lane / C;
+                    int tw = rw / p.G, hw = rw - tw * p.G;
+                    const int qs = S / p.G, rs = S - qs * p.G;
+#pragma unroll
+                    for (int i = 0; i < C; ++i) {
+                        const uint4 x = lds128(tile + tile_chunk(rw + i * S, ch));
+                        if (tw < tp.nt && u.tok0 + t * tp.nt + tw < u.n)
+                            *reinterpret_cast<uint4*>(p.out + (int64_t)(u.first + u.tok0 + t * tp.nt + tw) * p.o_tok +
+                                                      (u.hk * p.G + hw) * p.o_head + ch * 8) = x;
+                        tw += qs;
+                        hw += rs;
+                        if (hw >= p.G) {
+                            hw -= p.G;
+                            ++tw;
+                        }
+                    }
+                }
+            }
+            __syncwarp();
             while (again) {
                 const int x = __ffs(again) - 1;
                 again &= again - 1;
-                const int rx = __shfl_sync(0xffffffffu, row, x);
+                const int rx = (r & ~31) + x, tx = __shfl_sync(0xffffffffu, tok, x), hx = rx % p.G;
                 const int j1 = __shfl_sync(0xffffffffu, lim, x) + 1;
                 float o[D / 32], mx, lx;
-                row_alone<T, D, SRC>(p, RowOf{u.b, u.hk, u.first}, rx, key0, min(j1, key0 + n * kKeys), lane, o, mx, lx);
-                const int tx = rx / p.G, hx = u.hk * p.G + (rx - tx * p.G);
+                row_alone<T, D, SRC>(p, RowOf{u.b, u.hk, u.first}, tx * p.G + hx, key0, min(j1, key0 + n * kKeys), lane, o, mx, lx);
                 if (u.slot < 0) {
                     const float ix = lx > 0.f ? 1.f / lx : (lx == lx ? 0.f : lx);
-                    uint16_t* d = p.out + (int64_t)(u.first + tx) * p.o_tok + hx * p.o_head + lane * (D / 32);
+                    uint16_t* d = p.out + (int64_t)(u.first + tx) * p.o_tok + (u.hk * p.G + hx) * p.o_head + lane * (D / 32);
 #pragma unroll
                     for (int j = 0; j < D / 32; j += 2)
                         *reinterpret_cast<uint32_t*>(d + j) = pack2<T>(o[j] * ix, o[j + 1] * ix);
                 } else {
-                    const int64_t at = (int64_t)u.slot * kRows + (rx - u.row0);
+                    const int64_t at = (int64_t)u.slot * kRows + t * kRowsT + rx;
 #pragma unroll
-                    for (int j = 0; j < D / 32; ++j) tp.part[at * D + lane * (D / 32) + j] = o[j];
+                    for (int j = 0; j < D / 32; ++j) {
+                        const int d = lane * (D / 32) + j;
+                        tp.part[(((int64_t)u.slot * (D / 4) + (d >> 2)) * kRows + t * kRowsT + rx) * 4 + (d & 3)] = o[j];
+                    }
                     if (lane == 0) {
                         tp.stat[at * 2] = mx;
                         tp.stat[at * 2 + 1] = lx;
@@ -590,6 +621,14 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
         constexpr int NR = SRC == kPaged8 ? NST : NS;
         auto rfull = [&](int s) { return SRC == kPaged8 ? st_full(s) : full(s); };
         auto rempty = [&](int s) { return SRC == kPaged8 ? st_empty(s) : empty(s); };
+        if (lane == 0 && n > 0) {
+            mbar_arrive_expect_tx(q_full, halves * P::kHalves * tp.nt * p.G * 128);
+            for (int t = 0; t < halves; ++t)
+#pragma unroll
+                for (int h = 0; h < P::kHalves; ++h)
+                    tma_load_3d(sb + t * P::kTileBytes + h * P::kBlock, &tp.tm_q, q_full, h * 64, u.hk * p.G,
+                                u.first + u.tok0 + t * tp.nt);
+        }
         for (int i = 0; i < n && ok; ++i) {
             const int kb = key0 + i * kKeys;
             int z = 0, pages = 1;
@@ -641,6 +680,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
             }
         }
         // no copy may still be landing when the CTA exits
+        if (n > 0) mbar_wait(q_full, 0);
         for (int j = g > NR ? g - NR : 0; j < g; ++j) mbar_wait(rfull(j % NR), (j / NR) & 1);
     } else if constexpr (SRC == kPaged8) {
         if (warp >= 12) {
@@ -706,26 +746,24 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
     }
 }
 
-// Joins the parts of the sequences whose keys several CTAs shared: block x
-// takes 256 / gridDim.y rows of the x-th such row tile, a warp per row.  The
+// Joins the parts of the sequences whose keys several CTAs shared: block (x,
+// y) takes 16 columns of the x-th such 256-row tile, a row per thread.  The
 // parts are added in the order of the keys.
-constexpr int kJoinThreads = 256;
-
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) attn_tile_join_kernel(const __grid_constant__ TileParams tp) {
+__global__ void __launch_bounds__(kRows) attn_tile_join_kernel(const __grid_constant__ TileParams tp) {
     const AttnParams& p = tp.a;
     __shared__ int sh[6];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        const int64_t work = total_work(p, lane);
+        const int per = tiles_per_part(p, tp.nt, tp.sms, lane);
         int before = 0, slots = 0, found = 0;
         for (int b0 = 0; b0 < p.B && !found; b0 += 32) {
             const int b = b0 + lane;
             Seq s{};
             int sp = 0;
             if (b < p.B) {
-                s = seq_of<true>(p, b);
-                sp = splits_of(s, work, tp.sms);
+                s = seq_of<true>(p, tp.nt, b);
+                sp = parts_of(s, per);
             }
             const int mine = sp > 1 ? s.rtiles * p.Hkv : 0;
             const int cum = warp_scan(mine, lane), scum = warp_scan(mine * sp, lane);
@@ -737,8 +775,8 @@ __global__ void __launch_bounds__(kJoinThreads) attn_tile_join_kernel(const __gr
                     const int hk = x % p.Hkv, rt = x / p.Hkv;
                     sh[0] = slots + scum - mine * sp + rt * sp * p.Hkv + hk;  // slot of the first part
                     sh[1] = sp;
-                    sh[2] = (s.rtiles - 1 - rt) * kRows;
-                    sh[3] = s.rows;
+                    sh[2] = (s.rtiles - 1 - rt) * 2 * tp.nt;
+                    sh[3] = s.n;
                     sh[4] = s.first;
                     sh[5] = hk;
                 }
@@ -751,29 +789,38 @@ __global__ void __launch_bounds__(kJoinThreads) attn_tile_join_kernel(const __gr
     __syncthreads();
     const int sp = sh[1];
     if (sp == 0) return;
-    const int slot = sh[0], row0 = sh[2], rows = sh[3], first = sh[4], hk = sh[5];
-    constexpr int E = D / 32;
-    for (int r = blockIdx.y * 8 + warp; r < min(kRows, rows - row0); r += gridDim.y * 8) {
-        float m = -INFINITY, l = 0.f, o[E];
-        for (int s = 0; s < sp; ++s) m = fmaxf(m, tp.stat[((int64_t)(slot + s * p.Hkv) * kRows + r) * 2]);
-        const float ref = m == -INFINITY ? 0.f : m;
+    const int slot = sh[0], first = sh[4], hk = sh[5];
+    const int r = threadIdx.x, rt = r & (kRowsT - 1), tk = sh[2] + (r >> 7) * tp.nt + rt / p.G, h = hk * p.G + rt % p.G;
+    if (rt >= tp.nt * p.G || tk >= sh[3]) return;
+    float m = -INFINITY, l = 0.f, o[16];
+    for (int s = 0; s < sp; ++s) m = fmaxf(m, tp.stat[((int64_t)(slot + s * p.Hkv) * kRows + r) * 2]);
+    const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[j] = 0.f;
-        for (int s = 0; s < sp; ++s) {
-            const int64_t at = (int64_t)(slot + s * p.Hkv) * kRows + r;
-            const float2 st = *reinterpret_cast<const float2*>(tp.stat + at * 2);
-            const float f = exp2f(st.x - ref);
-            l += st.y * f;
-            if (st.x == -INFINITY && st.y == 0.f) continue;  // a part the row saw nothing of
+    for (int j = 0; j < 16; ++j) o[j] = 0.f;
+#pragma unroll 2
+    for (int s = 0; s < sp; ++s) {
+        const int64_t at = slot + s * p.Hkv;
+        const float2 st = *reinterpret_cast<const float2*>(tp.stat + (at * kRows + r) * 2);
+        float4 v[4];
 #pragma unroll
-            for (int j = 0; j < E; ++j) o[j] += tp.part[at * D + lane * E + j] * f;
+        for (int j = 0; j < 4; ++j)
+            v[j] = reinterpret_cast<const float4*>(tp.part)[(at * (D / 4) + blockIdx.y * 4 + j) * kRows + r];
+        const float f = exp2f(st.x - ref);
+        l += st.y * f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // (a part the row saw nothing of has weight 0)
+            o[4 * j] += v[j].x * f;
+            o[4 * j + 1] += v[j].y * f;
+            o[4 * j + 2] += v[j].z * f;
+            o[4 * j + 3] += v[j].w * f;
         }
-        const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-        const int tk = (row0 + r) / p.G, h = hk * p.G + (row0 + r) % p.G;
-        uint16_t* d = p.out + (int64_t)(first + tk) * p.o_tok + h * p.o_head + lane * E;
-#pragma unroll
-        for (int j = 0; j < E; j += 2) *reinterpret_cast<uint32_t*>(d + j) = pack2<T>(o[j] * inv, o[j + 1] * inv);
     }
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    uint4* d = reinterpret_cast<uint4*>(p.out + (int64_t)(first + tk) * p.o_tok + h * p.o_head + blockIdx.y * 16);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        d[j] = make_uint4(pack2<T>(o[8 * j] * inv, o[8 * j + 1] * inv), pack2<T>(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                          pack2<T>(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack2<T>(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
 }
 
 template <typename T, int D, int SRC>
@@ -782,13 +829,17 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
     TileParams tp;
     tp.a = a;
     tp.sms = device_sm_count();
+    tp.nt = kRowsT / a.G;
     int rc;
-    constexpr bool f16 = ActTraits<T>::kIsF16;
-    const CUtensorMapDataType dt = SRC == kPaged8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                   : f16          ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUtensorMapDataType act = ActTraits<T>::kIsF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    // the strides of a single head or token are never used
+    const uint64_t qt = a.T == 1 ? D * 2 : a.q_tok * 2, qh = a.Hq == 1 ? D * 2 : a.q_head * 2;
+    const uint64_t ot = a.T == 1 ? D * 2 : a.o_tok * 2, oh = a.Hq == 1 ? D * 2 : a.o_head * 2;
+    if ((rc = encode_3d(&tp.tm_q, act, a.q, D, a.Hq, a.T, qh, qt, 64, a.G, tp.nt, CU_TENSOR_MAP_SWIZZLE_128B, "q")) ||
+        (rc = encode_3d(&tp.tm_o, act, a.out, D, a.Hq, a.T, oh, ot, 64, a.G, tp.nt, CU_TENSOR_MAP_SWIZZLE_128B, "out")))
+        return rc;
+    const CUtensorMapDataType dt = SRC == kPaged8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : act;
     if constexpr (SRC == kPacked) {
-        // a single kv head's stride is never used
         const uint64_t kh = a.Hkv == 1 ? D * 2 : a.k_head * 2, vh = a.Hkv == 1 ? D * 2 : a.v_head * 2;
         const uint64_t kt = a.T == 1 ? D * 2 : a.k_tok * 2, vt = a.T == 1 ? D * 2 : a.v_tok * 2;
         if ((rc = encode_3d(&tp.tm_k, dt, a.k, D, a.Hkv, a.T, kh, kt, 64, 1, kKeys, CU_TENSOR_MAP_SWIZZLE_128B, "k")) ||
@@ -804,8 +855,8 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
             return rc;
     }
     tp.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + WLQ_ATTENTION_ZERO_BYTES);
-    tp.stat = tp.part + (size_t)tp.sms * kRows * D;
-    const int64_t grid = (a.T * a.G / kRows + a.B) * a.Hkv + (SRC == kPacked ? 0 : tp.sms);
+    tp.stat = tp.part + (size_t)kPartsPerSm * tp.sms * kRows * D;
+    const int64_t grid = (a.T / (2 * tp.nt) + a.B) * a.Hkv + (SRC == kPacked ? 0 : kPartsPerSm * tp.sms);
     if (grid > 0x7fffffff) return fail(WLQ_ERR_UNSUPPORTED, "attention: %lld row tiles in one call", (long long)grid);
     static const cudaError_t attr = cudaFuncSetAttribute(attn_tile_kernel<T, D, SRC>,
                                                          cudaFuncAttributeMaxDynamicSharedMemorySize, P::kAlloc);
@@ -813,7 +864,7 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
     attn_tile_kernel<T, D, SRC><<<(unsigned)grid, P::kThreads, P::kAlloc, stream>>>(tp);
     if ((rc = check_cuda(cudaGetLastError(), "attn_tile_kernel"))) return rc;
     if constexpr (SRC != kPacked) {
-        attn_tile_join_kernel<T, D><<<dim3(tp.sms / 2, 8), kJoinThreads, 0, stream>>>(tp);
+        attn_tile_join_kernel<T, D><<<dim3(kPartsPerSm * tp.sms / 2, D / 16), kRows, 0, stream>>>(tp);
         rc = check_cuda(cudaGetLastError(), "attn_tile_join_kernel");
     }
     return rc;
