@@ -19,9 +19,14 @@ from typing import Optional, Tuple
 import numpy as np
 import torch
 
-from ._lib import WLQ_DTYPE_BF16, WLQ_DTYPE_F16, WLQ_LUT_F16, WLQ_LUT_PREPACKED, check, lib
+from . import _calls
+from ._lib import (WLQ_DTYPE_BF16, WLQ_DTYPE_F16, WLQ_LUT_F16, WLQ_LUT_PREPACKED, WLQError, check, lib)
 
 _NONE = None
+
+_calls.setup(tuple(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+    "wlq_rope_kv_write", "wlq_kv_read", "wlq_prompt_attention", "wlq_paged_attention_workspace_bytes",
+    "wlq_paged_attention", "wlq_last_error")), WLQError)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -368,53 +373,9 @@ def prepack_outliers(q_packed, lut_c, chunk_offsets, chunk_cols, chunk_vals, N, 
 # -------------------------------------------------------------- attention ---
 # The operators between the qkv and the o projection of a served layer
 # (wlq_rope_kv_write ... wlq_paged_attention in include/wlq_b200.h say what
-# they compute).  Tensors of heads are [tokens, heads, head_size] views with
+# they compute; csrc/torch/calls.cpp checks the arguments and keeps the
+# workspaces).  Tensors of heads are [tokens, heads, head_size] views with
 # contiguous heads, such as the parts of one qkv projection's output.
-
-def _heads(name, nm, t, dtype, dev, heads=None, D=None):
-    """Checks one [T, heads, D] tensor; its token and head strides."""
-    _require(t.is_cuda and t.device == dev, lambda: f"{name}: {nm} must be on {dev}")
-    _require(t.dtype == dtype, lambda: f"{name}: {nm} must be {dtype}, got {t.dtype}")
-    _require(t.dim() == 3, lambda: f"{name}: {nm} must be [tokens, heads, head_size], got {tuple(t.shape)}")
-    st = t.stride()
-    _require(st[2] == 1 or t.shape[2] == 1, lambda: f"{name}: the values of a head of {nm} must be contiguous")
-    _require((heads is None or t.shape[1] == heads) and (D is None or t.shape[2] == D),
-             lambda: f"{name}: {nm} must be [tokens, {heads}, {D}], got {tuple(t.shape)}")
-    return st[0], st[1]
-
-
-def _vector(name, nm, t, dtype, dev, n=None):
-    _require(t is not None and t.is_cuda and t.device == dev, lambda: f"{name}: {nm} must be on {dev}")
-    _require(t.dtype == dtype and t.is_contiguous(), lambda: f"{name}: {nm} must be contiguous {dtype}")
-    _require(n is None or t.numel() == n, lambda: f"{name}: {nm} must have {n} values, got {t.numel()}")
-
-
-def _cache_checks(name, k_cache, v_cache, k_exp, v_exp, act, dev):
-    """(pages, kv_heads, page_size, D) of a paged cache."""
-    _require(k_cache.dim() == 4 and k_cache.shape == v_cache.shape,
-             lambda: f"{name}: k_cache and v_cache must be [pages, kv_heads, page_size, head_size], got "
-                     f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    want = act if k_exp is None else torch.float8_e4m3fn
-    for nm, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _require(t.device == dev and t.is_contiguous(), lambda: f"{name}: {nm} must be contiguous on {dev}")
-        _require(t.dtype == want, lambda: f"{name}: {nm} must be {want}, got {t.dtype}"
-                 + (" (an 8-bit cache needs k_exp and v_exp)" if k_exp is None else ""))
-    _require((k_exp is None) == (v_exp is None), lambda: f"{name}: give k_exp and v_exp, or neither")
-    if k_exp is not None:
-        for nm, t in (("k_exp", k_exp), ("v_exp", v_exp)):
-            _require(t.device == dev and t.dtype == torch.uint8 and t.is_contiguous() and
-                     t.shape == k_cache.shape[:3], lambda: f"{name}: {nm} must be contiguous uint8 "
-                     f"{tuple(k_cache.shape[:3])} on {dev}")
-    return k_cache.shape
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _raw_stream(dev):
-    return torch._C._cuda_getCurrentRawStream(dev.index)
-
 
 def rope_kv_write(q, k, v, positions, cos_sin, slots, k_cache, v_cache, q_out, k_out=None, k_exp=None, v_exp=None,
                   interleaved=False):
@@ -423,94 +384,21 @@ def rope_kv_write(q, k, v, positions, cos_sin, slots, k_cache, v_cache, q_out, k
     optional k_out [T, Hkv, D]; positions and slots int64 [T] (slot = page *
     page_size + offset, negative for a padding token); cos_sin float32
     [positions, rot] (rope_table makes one)."""
-    name, dev, act = "rope_kv_write", q.device, q.dtype
-    dt = _act_dtype(q)
-    _require(q.is_cuda, lambda: f"{name}: q must be a CUDA tensor")
-    pages, Hkv, ps, D = _cache_checks(name, k_cache, v_cache, k_exp, v_exp, act, dev)
-    sq, sk, sv = (_heads(name, "q", q, act, dev, None, D), _heads(name, "k", k, act, dev, Hkv, D),
-                  _heads(name, "v", v, act, dev, Hkv, D))
-    T, Hq = q.shape[0], q.shape[1]
-    so = _heads(name, "q_out", q_out, act, dev, Hq, D)
-    ko = (0, 0) if k_out is None else _heads(name, "k_out", k_out, act, dev, Hkv, D)
-    _require(k.shape[0] == T and v.shape[0] == T and q_out.shape[0] == T and (k_out is None or k_out.shape[0] == T),
-             lambda: f"{name}: q, k, v, q_out and k_out must have the same number of tokens")
-    _vector(name, "positions", positions, torch.int64, dev, T)
-    _vector(name, "slots", slots, torch.int64, dev, T)
-    _vector(name, "cos_sin", cos_sin, torch.float32, dev)
-    _require(cos_sin.dim() == 2, lambda: f"{name}: cos_sin must be [positions, rot]")
-    with _DeviceGuard(dev):
-        rc = lib.wlq_rope_kv_write(q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(),
-                                   slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _addr(k_exp),
-                                   _addr(v_exp), q_out.data_ptr(), _addr(k_out), *sq, *sk, *sv, *so, *ko, T,
-                                   cos_sin.shape[0], pages, Hq, Hkv, D, cos_sin.shape[1], ps, 1 if interleaved else 0,
-                                   dt, _raw_stream(dev))
-    check(rc, "wlq_rope_kv_write")
+    _calls.rope_kv_write(q, k, v, positions, cos_sin, slots, k_cache, v_cache, q_out, k_out, k_exp, v_exp, interleaved)
 
 
 def kv_read(k_cache, v_cache, block_table, cu_lens, k_out, v_out, k_exp=None, v_exp=None):
     """The cached k and v of whole sequences as packed rows (wlq_kv_read):
     k_out, v_out [T, Hkv, D] contiguous; block_table int32 [B, pages],
     cu_lens int32 [B + 1]."""
-    name, dev, act = "kv_read", k_out.device, k_out.dtype
-    dt = _act_dtype(k_out)
-    _require(k_out.is_cuda, lambda: f"{name}: k_out must be a CUDA tensor")
-    pages, Hkv, ps, D = _cache_checks(name, k_cache, v_cache, k_exp, v_exp, act, dev)
-    for nm, t in (("k_out", k_out), ("v_out", v_out)):
-        _heads(name, nm, t, act, dev, Hkv, D)
-        _require(t.is_contiguous() and t.shape == k_out.shape, lambda: f"{name}: {nm} must be contiguous, of k_out's shape")
-    _vector(name, "block_table", block_table, torch.int32, dev)
-    _vector(name, "cu_lens", cu_lens, torch.int32, dev)
-    _require(block_table.dim() == 2 and cu_lens.numel() == block_table.shape[0] + 1,
-             lambda: f"{name}: block_table must be [B, pages] and cu_lens [B + 1]")
-    with _DeviceGuard(dev):
-        rc = lib.wlq_kv_read(k_cache.data_ptr(), v_cache.data_ptr(), _addr(k_exp), _addr(v_exp),
-                             block_table.data_ptr(), cu_lens.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-                             k_out.shape[0], block_table.shape[0], pages, block_table.shape[1], Hkv, D, ps, dt,
-                             _raw_stream(dev))
-    check(rc, "wlq_kv_read")
+    _calls.kv_read(k_cache, v_cache, block_table, cu_lens, k_out, v_out, k_exp, v_exp)
 
 
 def prompt_attention(q, k, v, cu_seqlens, out, scale=None, causal=True):
     """Attention of packed prompts over their own k and v
     (wlq_prompt_attention): q, out [T, Hq, D], k, v [T, Hkv, D], cu_seqlens
     int32 [B + 1]; scale defaults to D ** -0.5."""
-    name, dev, act = "prompt_attention", q.device, q.dtype
-    dt = _act_dtype(q)
-    _require(q.is_cuda, lambda: f"{name}: q must be a CUDA tensor")
-    sq = _heads(name, "q", q, act, dev)
-    T, Hq, D = q.shape
-    sk = _heads(name, "k", k, act, dev, None, D)
-    Hkv = k.shape[1]
-    sv, so = _heads(name, "v", v, act, dev, Hkv, D), _heads(name, "out", out, act, dev, Hq, D)
-    _require(k.shape[0] == T and v.shape[0] == T and out.shape[0] == T,
-             lambda: f"{name}: q, k, v and out must have the same number of tokens")
-    _vector(name, "cu_seqlens", cu_seqlens, torch.int32, dev)
-    with _DeviceGuard(dev):
-        rc = lib.wlq_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr(),
-                                      *sq, *sk, *sv, *so, T, cu_seqlens.numel() - 1, Hq, Hkv, D,
-                                      D ** -0.5 if scale is None else float(scale), 1 if causal else 0, dt,
-                                      _raw_stream(dev))
-    check(rc, "wlq_prompt_attention")
-
-
-# Workspaces of paged_attention, one per device and stream (calls on several
-# streams may overlap), grown when a call needs more and kept for the process.
-_ATTN_WS = {}
-_ATTN_ZERO_BYTES = 256 * 1024  # WLQ_ATTENTION_ZERO_BYTES
-
-
-def attention_workspace(dev, stream, nbytes):
-    """This stream's workspace.  While a CUDA graph is captured the graph gets
-    one of its own, from its memory pool: a replay may overlap later calls on
-    the stream that captured it."""
-    capturing = torch.cuda.is_current_stream_capturing()
-    ws = None if capturing else _ATTN_WS.get((dev.index, stream))
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        ws[:_ATTN_ZERO_BYTES].zero_()
-        if not capturing:
-            _ATTN_WS[(dev.index, stream)] = ws
-    return ws
+    _calls.prompt_attention(q, k, v, cu_seqlens, out, scale, causal)
 
 
 def paged_attention(q, k_cache, v_cache, block_table, kv_lens, out, cu_q=None, max_q=1, k_exp=None, v_exp=None,
@@ -521,30 +409,7 @@ def paged_attention(q, k_cache, v_cache, block_table, kv_lens, out, cu_q=None, m
     cu_q int32 [B + 1] the sequences' rows of q and max_q an upper bound of
     their number (None and 1: one new token per sequence); scale defaults to
     D ** -0.5."""
-    name, dev, act = "paged_attention", q.device, q.dtype
-    dt = _act_dtype(q)
-    _require(q.is_cuda, lambda: f"{name}: q must be a CUDA tensor")
-    pages, Hkv, ps, D = _cache_checks(name, k_cache, v_cache, k_exp, v_exp, act, dev)
-    sq = _heads(name, "q", q, act, dev, None, D)
-    T, Hq = q.shape[0], q.shape[1]
-    so = _heads(name, "out", out, act, dev, Hq, D)
-    _require(out.shape[0] == T, lambda: f"{name}: out must have {T} tokens")
-    _vector(name, "block_table", block_table, torch.int32, dev)
-    _require(block_table.dim() == 2, lambda: f"{name}: block_table must be [B, pages]")
-    B = block_table.shape[0]
-    _vector(name, "kv_lens", kv_lens, torch.int32, dev, B)
-    if cu_q is not None:
-        _vector(name, "cu_q", cu_q, torch.int32, dev, B + 1)
-    max_q = int(max_q)
-    with _DeviceGuard(dev):
-        stream = _raw_stream(dev)
-        ws = attention_workspace(dev, stream, lib.wlq_paged_attention_workspace_bytes(Hq, Hkv, D, max_q))
-        rc = lib.wlq_paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _addr(k_exp), _addr(v_exp),
-                                     block_table.data_ptr(), kv_lens.data_ptr(), _addr(cu_q), out.data_ptr(), *sq,
-                                     *so, T, B, Hq, Hkv, D, ps, pages, block_table.shape[1], max_q,
-                                     D ** -0.5 if scale is None else float(scale), dt, ws.data_ptr(), ws.numel(),
-                                     stream)
-    check(rc, "wlq_paged_attention")
+    _calls.paged_attention(q, k_cache, v_cache, block_table, kv_lens, out, cu_q, max_q, k_exp, v_exp, scale)
 
 
 def init_workspaces(max_N, max_K, device):
