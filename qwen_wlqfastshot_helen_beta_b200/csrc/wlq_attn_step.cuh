@@ -4,7 +4,8 @@
 // HBM-bound: the cache is read once.  The key tiles of all sequences and kv
 // heads, 64 keys each, form one list that is shared out evenly over the CTAs
 // whatever the sequences' lengths are; a CTA walks its share, one segment per
-// (sequence, kv head) it touches.  Where a segment is only a part, its
+// (sequence, kv head) it touches.  Few tiles are shared out by equal parts of
+// each sequence instead, one per CTA.  Where a segment is only a part, its
 // unnormalised output and statistics go to the workspace, and the CTA that
 // delivers a (sequence, kv head)'s last part adds the parts up in the order
 // of the keys: one launch, and results that do not depend on timing.
@@ -49,7 +50,7 @@ struct StepPlan {
     static constexpr int kSide = kStepKeys * D * (Q8 ? 1 : 2);  // k or v of a tile
     static constexpr int kStage = 2 * kSide + (Q8 ? 1024 : 0);  // 8-bit: the rows' scales behind them
     static constexpr int kMerge = 2 * kRowsMax * D * 4;         // two warps' outputs
-    static constexpr int kStat = 4 * kRowsMax * 4 * 4;
+    static constexpr int kStat = 5 * kRowsMax * 4 * 4;           // the warps' statistics, then the segment's
     static constexpr int kCtas = NT == 1 ? 3 : 2;               // per SM
     static constexpr int kFit = ((kCtas == 3 ? 74 : 112) * 1024 - 1024 - 256 - kMerge - kStat) / kStage;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
@@ -80,16 +81,23 @@ __device__ __forceinline__ StepSeq step_seq(const AttnParams& p, int b, int rows
     return s;
 }
 
+// a * b / c (rounded up by `up`), in 32 bits where the product fits: a 64-bit
+// division takes several times as long, and a cut needs a handful.
+__device__ __forceinline__ int mul_div(uint32_t a, uint32_t b, uint32_t c, bool up) {
+    const uint64_t x = (uint64_t)a * b + (up ? c - 1 : 0u);
+    return (x >> 32) == 0 ? (int)((uint32_t)x / c) : (int)(x / c);
+}
+
 // The list's G - 1 cuts, at even distances; a cut within `slack` tiles of a
 // sequence's (and kv head's) end moves there, so that a part is worth the
 // joining it costs.
 struct StepCuts {
     int total, G, slack;
-    __device__ __forceinline__ int raw(int c) const { return (int)((int64_t)c * total / G); }
+    __device__ __forceinline__ int raw(int c) const { return mul_div(c, total, G, false); }
     // the cuts inside tiles [base, base + n): c in [lo, hi]
     __device__ __forceinline__ void inside(int base, int n, int& lo, int& hi) const {
-        lo = (int)(((int64_t)(base + slack + 1) * G + total - 1) / total);
-        hi = (int)(((int64_t)(base + n - slack) * G + total - 1) / total) - 1;
+        lo = mul_div(base + slack + 1, G, total, true);
+        hi = n > slack ? mul_div(base + n - slack, G, total, true) - 1 : lo - 1;
     }
     __device__ __forceinline__ int moved(int at, int base, int n) const {
         return at - base <= slack ? base : (base + n - at <= slack ? base + n : at);
@@ -103,8 +111,14 @@ struct StepWalk {
     StepSeq s;
     // the segment: kv head, tiles [t0, t1) of the sequence, list index of tile 0
     int hk, t0, t1, base;
+    int parts, part;  // parts > 0: the segment is all there is, part number `part` of its sequence and kv head
 
     __device__ __forceinline__ bool next(const AttnParams& p, int rows_max) {
+        if (parts) {
+            const bool first = it == 0;
+            it = 1;
+            return first;
+        }
         if (it >= it1) return false;
         while (it >= cum + s.tiles * p.Hkv) {
             cum += s.tiles * p.Hkv;
@@ -118,6 +132,9 @@ struct StepWalk {
         return true;
     }
 };
+
+// Parts of about T tiles.
+__device__ __forceinline__ int parts_of(int tiles, int T) { return tiles ? max(1, (tiles + (T >> 1)) / T) : 0; }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
     uint32_t d;
@@ -191,110 +208,86 @@ __device__ __forceinline__ void store_row(const AttnParams& p, int hk, int first
     for (int j = 0; j < E; j += 2) *reinterpret_cast<uint32_t*>(d + j) = pack2<T>(a[j] * f, a[j + 1] * f);
 }
 
-// Adds up the parts of one (sequence, kv head), by the four consumer warps: a
-// quarter of the parts per warp, all loads of a few parts in flight together,
-// the statistics of row r in lane r.  Every sum has a fixed order.  Part 0 is
-// CTA c0's last, part i > 0 the first of CTA c0 + i.
+// Adds up the parts of one (sequence, kv head), by the four consumer warps, a
+// row per warp and round: the parts' statistics in a lane each, the outputs of
+// eight parts in flight together.  The sums have a fixed order.  Part 0 is CTA
+// c0's last, part i > 0 the first of CTA c0 + i.
 template <typename T, int D, int NT>
-__device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int hk, int first, int c0, int parts,
-                                           float* merge, float* wstat, int warp, int lane) {
-    constexpr int RM = 8 * NT, E = D / 32, U = 2 / NT;
-    float a[RM][E], a1 = -INFINITY, a0 = -INFINITY, sum = 0.f;
+__device__ __forceinline__ void join_parts(const StepParams& sp, int rows, int hk, int first, int c0, int parts, int warp,
+                                           int lane) {
+    constexpr int RM = 8 * NT, E = D / 32, U = 8;
+    for (int rb = warp; rb < rows; rb += 8) {  // rows rb, rb + 4
+        float a[2][E], a1[2], a0[2], sum[2];
 #pragma unroll
-    for (int r = 0; r < RM; ++r)
+        for (int z = 0; z < 2; ++z) {
+            a1[z] = a0[z] = -INFINITY;
+            sum[z] = 0.f;
 #pragma unroll
-        for (int j = 0; j < E; ++j) a[r][j] = 0.f;
-    for (int i0 = warp; i0 < parts; i0 += 4 * U) {
-        float4 x[U];
-        float v[U][RM][E];
+            for (int j = 0; j < E; ++j) a[z][j] = 0.f;
+        }
+        for (int p0 = 0; p0 < parts; p0 += 32) {
+            const int n = min(32, parts - p0), mine = p0 + min(lane, n - 1);
+            float4 x[2];
+            float f[2];
 #pragma unroll
-        for (int y = 0; y < U; ++y) {
-            // past the last part: the last one, without weight; past the last row: whatever the slot holds, not used
-            const int i = min(i0 + 4 * y, parts - 1);
-            const int64_t at = (int64_t)(2 * (c0 + i) + (i == 0)) * RM;
-            x[y] = ldcg4(sp.stat + (at + (lane & (RM - 1))) * 4);
+            for (int z = 0; z < 2; ++z)
+                x[z] = ldcg4(sp.stat + ((int64_t)(2 * (c0 + mine) + (mine == 0)) * RM + min(rb + 4 * z, RM - 1)) * 4);
+            for (int i0 = 0; i0 < n; i0 += U) {
+                float4 v[2][U];
 #pragma unroll
-            for (int r = 0; r < RM; ++r)
+                for (int z = 0; z < 2; ++z)
 #pragma unroll
-                for (int j = 0; j < E; j += 2) {
-                    const float2 t = ldcg2(sp.part + (at + r) * D + lane * E + j);
-                    v[y][r][j] = t.x, v[y][r][j + 1] = t.y;
+                    for (int y = 0; y < U; ++y) {
+                        const int i = p0 + min(i0 + y, n - 1);
+                        const float* src =
+                            sp.part + ((int64_t)(2 * (c0 + i) + (i == 0)) * RM + min(rb + 4 * z, RM - 1)) * D + lane * E;
+                        if constexpr (E == 4) {
+                            v[z][y] = ldcg4(src);
+                        } else {
+                            const float2 t = ldcg2(src);
+                            v[z][y] = make_float4(t.x, t.y, 0.f, 0.f);
+                        }
+                    }
+                if (i0 == 0) {  // (with the outputs on their way)
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        if (lane >= n) x[z] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+                        float b1 = fmaxf(a1[z], x[z].x), b0 = fmaxf(a0[z], x[z].y);
+#pragma unroll
+                        for (int d = 16; d; d >>= 1) {
+                            b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, d));
+                            b0 = fmaxf(b0, __shfl_xor_sync(0xffffffffu, b0, d));
+                        }
+                        const float keep = rescale(a1[z], b1);
+                        f[z] = rescale(x[z].x, b1);
+                        sum[z] = sum[z] * rescale(a0[z], b0) + x[z].z * rescale(x[z].y, b0);  // per lane, added up at the end
+                        a1[z] = b1, a0[z] = b0;
+#pragma unroll
+                        for (int j = 0; j < E; ++j) a[z][j] *= keep;
+                    }
                 }
-        }
 #pragma unroll
-        for (int y = 0; y < U; ++y)
-            if (i0 + 4 * y >= parts || lane >= rows) x[y] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
-        float b1 = a1, b0 = a0;
+                for (int z = 0; z < 2; ++z)
 #pragma unroll
-        for (int y = 0; y < U; ++y) b1 = fmaxf(b1, x[y].x), b0 = fmaxf(b0, x[y].y);
-        const float keep = rescale(a1, b1);
-        sum *= rescale(a0, b0);
-        a1 = b1, a0 = b0;
-        float f[U];
-#pragma unroll
-        for (int y = 0; y < U; ++y) {
-            f[y] = rescale(x[y].x, a1);
-            sum += x[y].z * rescale(x[y].y, a0);
-        }
-#pragma unroll
-        for (int r = 0; r < RM; ++r) {
-            const float k = __shfl_sync(0xffffffffu, keep, r);
-#pragma unroll
-            for (int j = 0; j < E; ++j) a[r][j] *= k;
-#pragma unroll
-            for (int y = 0; y < U; ++y) {
-                const float g = __shfl_sync(0xffffffffu, f[y], r);
-#pragma unroll
-                for (int j = 0; j < E; ++j) a[r][j] += g == 0.f ? 0.f : v[y][r][j] * g;
+                    for (int y = 0; y < U; ++y) {
+                        const float g = __shfl_sync(0xffffffffu, f[z], min(i0 + y, 31));
+                        if (i0 + y < n) {
+                            a[z][0] += v[z][y].x * g;
+                            a[z][1] += v[z][y].y * g;
+                            if constexpr (E == 4) {
+                                a[z][2] += v[z][y].z * g;
+                                a[z][3] += v[z][y].w * g;
+                            }
+                        }
+                    }
             }
         }
-    }
-    if (lane < RM) *reinterpret_cast<float4*>(wstat + (warp * RM + lane) * 4) = make_float4(a1, a0, sum, 0.f);
-    bar_sync_step();
-    float4 st[4];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) st[y] = *reinterpret_cast<const float4*>(wstat + (y * RM + (lane & (RM - 1))) * 4);
-    const float t1 = fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x));
-    const float t0 = fmaxf(fmaxf(st[0].y, st[1].y), fmaxf(st[2].y, st[3].y));
-    float all = 0.f;
+        for (int z = 0; z < 2; ++z) {
+            const int r = rb + 4 * z;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) all += st[y].z * rescale(st[y].y, t0);
-    const float fw = rescale(st[warp].x, t1);
-#pragma unroll
-    for (int r = 0; r < RM; ++r) {
-        const float k = __shfl_sync(0xffffffffu, fw, r);
-#pragma unroll
-        for (int j = 0; j < E; ++j) a[r][j] *= k;
-    }
-    auto put = [&](int y) {
-#pragma unroll
-        for (int r = 0; r < RM; ++r)
-#pragma unroll
-            for (int j = 0; j < E; j += 2)
-                *reinterpret_cast<float2*>(merge + (y * RM + r) * D + lane * E + j) = make_float2(a[r][j], a[r][j + 1]);
-    };
-    auto add = [&](int y) {
-#pragma unroll
-        for (int r = 0; r < RM; ++r)
-#pragma unroll
-            for (int j = 0; j < E; j += 2) {
-                const float2 t = *reinterpret_cast<const float2*>(merge + (y * RM + r) * D + lane * E + j);
-                a[r][j] += t.x;
-                a[r][j + 1] += t.y;
-            }
-    };
-    if (warp >= 2) put(warp - 2);
-    bar_sync_step();
-    if (warp < 2) add(warp);
-    if (warp == 1) put(1);
-    bar_sync_step();
-    if (warp == 0) {
-        add(1);
-#pragma unroll
-        for (int r = 0; r < RM; ++r) {
-            const float4 x = make_float4(__shfl_sync(0xffffffffu, t1, r), __shfl_sync(0xffffffffu, t0, r),
-                                         __shfl_sync(0xffffffffu, all, r), 0.f);
-            if (r < rows) store_row<T, E>(sp.a, hk, first, r, lane, a[r], x);
+            for (int d = 16; d; d >>= 1) sum[z] += __shfl_xor_sync(0xffffffffu, sum[z], d);
+            if (r < rows) store_row<T, E>(sp.a, hk, first, r, lane, a[z], make_float4(a1[z], a0[z], sum[z], 0.f));
         }
     }
 }
@@ -306,7 +299,7 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
     constexpr int NS = P::kStages, KK = D / 16, RM = P::kRowsMax;
     const AttnParams& p = sp.a;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int plan[7];
+    __shared__ int plan[10];
     __shared__ uint32_t last_part;
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sb = (raw + 1023u) & ~1023u;
@@ -328,32 +321,65 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
         tma_prefetch_desc(&sp.tm_v);
     }
     if (warp == 0) {
-        int total = 0, units = 0;
+        int total = 0, units = 0, tiles0 = 0;  // tiles0: of this lane's sequence among the first 32
         for (int b0 = 0; b0 < p.B; b0 += 32) {
             const int tiles = b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
+            if (b0 == 0) tiles0 = tiles;
             total += tiles;
             units += tiles > 0;
         }
-        total = (int)warp_sum(total) * p.Hkv;
-        units = (int)warp_sum(units) * p.Hkv;
-        // CTAs with work.  n tiles of a (sequence, kv head) in P parts take n / P * 0.75 us and, for P > 1, 3 us + P *
-        // 0.05 us to be joined: least at P = sqrt(15 n), and worth it from 6 tiles on.  P is a whole number, so that
-        // sequences of one length are cut alike, unless every CTA has 16 tiles or more.
+        total = __reduce_add_sync(0xffffffffu, total) * p.Hkv;
+        units = __reduce_add_sync(0xffffffffu, units) * p.Hkv;
+        // n tiles of a (sequence, kv head) in P parts take n / P * 0.75 us and, for P > 1, 3 us + P * 0.05 us to be
+        // joined: least at P = sqrt(15 n), and worth it from 6 tiles on.  Where such parts, T tiles each, are no more
+        // than the CTAs, every CTA has one: a sequence's parts are alike, whatever the other sequences' lengths are.
         const int grid = (int)gridDim.x;
-        const float n = (float)total / (float)max(units, 1);
-        int P = n < 6.f ? 1 : (int)fminf(n, sqrtf(15.f * n));
-        if (units * P > grid) P = max(1, grid / max(units, 1));
+        int T = 0, parts = 0, part = 0, hk = 0;
+        if (total / grid < 16 && units <= grid) {
+            const float n = (float)total / (float)max(units, 1);
+            T = n < 6.f ? 6 : max(1, (int)(n / fminf(n, sqrtf(15.f * n)) + 0.5f));
+            for (int tries = 0; tries < 6; ++tries) {
+                int sum = parts_of(tiles0, T);
+                for (int b0 = 32; b0 < p.B; b0 += 32)
+                    sum += b0 + lane < p.B ? parts_of(step_seq(p, b0 + lane, RM).tiles, T) : 0;
+                sum = __reduce_add_sync(0xffffffffu, sum) * p.Hkv;
+                if (sum <= grid) break;
+                T = tries == 5 ? 0 : mul_div(T, sum, grid, false) + 1;  // 0: shared out evenly after all
+            }
+        }
+        // Otherwise the list of tiles is cut evenly; a part is worth 4 tiles or more.
         StepCuts cuts;
         cuts.total = total;
-        cuts.G = max(1, min(total, total / grid >= 16 ? grid : min(grid, units * P)));
-        cuts.slack = P == 1 ? 4 : min(total / cuts.G / 2, 8);
+        cuts.G = max(1, min(total, grid));
+        cuts.slack = min(max(total / cuts.G / 2, 4), 8);
         // this CTA's first tile and the next one's, each with the sequence it lies in
         int first = 0, cum0 = 0, at = total, end = total;
-        if ((int)blockIdx.x < cuts.G) {
+        if (T) {
+            at = end = 0;
+            int before = 0;
+            for (int b0 = 0; b0 < p.B; b0 += 32) {
+                const int tiles = b0 == 0 ? tiles0 : b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
+                const int ps = parts_of(tiles, T), cum = before + warp_scan(ps * p.Hkv, lane);
+                const unsigned hit = __ballot_sync(0xffffffffu, (int)blockIdx.x < cum);
+                if (hit) {
+                    const int l = __ffs(hit) - 1;
+                    first = b0 + l;
+                    parts = __shfl_sync(0xffffffffu, ps, l);
+                    const int n = __shfl_sync(0xffffffffu, tiles, l);
+                    const int x = (int)blockIdx.x - __shfl_sync(0xffffffffu, cum - ps * p.Hkv, l);
+                    hk = x / parts;
+                    part = x - hk * parts;
+                    at = part * n / parts;
+                    end = (part + 1) * n / parts;
+                    break;
+                }
+                before = __shfl_sync(0xffffffffu, cum, 31);
+            }
+        } else if ((int)blockIdx.x < cuts.G) {
             const int r0 = cuts.raw(blockIdx.x), r1 = cuts.raw(blockIdx.x + 1);
             int before = 0;
             for (int b0 = 0; b0 < p.B && before <= r1; b0 += 32) {
-                const int tiles = b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
+                const int tiles = b0 == 0 ? tiles0 : b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
                 const int mine = tiles * p.Hkv, cum = before + warp_scan(mine, lane) - mine;
                 // (sequences' tiles are disjoint: one lane of one round at most has either)
                 const bool h0 = r0 >= cum && r0 < cum + mine, h1 = r1 >= cum && r1 < cum + mine;
@@ -385,6 +411,9 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
             plan[4] = cuts.slack;
             plan[5] = at;
             plan[6] = end;
+            plan[7] = parts;
+            plan[8] = part;
+            plan[9] = hk;
         }
     }
     __syncthreads();
@@ -392,6 +421,8 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
     w.it = plan[5];
     w.it1 = plan[6];
     if (w.it >= w.it1) return;
+    w.parts = plan[7];
+    w.part = plan[8];
     StepCuts cuts;
     cuts.total = plan[0];
     cuts.G = plan[3];
@@ -399,6 +430,12 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
     w.b = plan[1];
     w.cum = plan[2];
     w.s = step_seq(p, w.b, RM);
+    if (w.parts) {
+        w.t0 = w.it;
+        w.t1 = w.it1;
+        w.hk = plan[9];
+        w.it = 0;
+    }
 
     if (warp == 4) {
         // ------------------------------------------------------ producer
@@ -761,79 +798,91 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
         if (warp < 2) add_from(warp);
         if (warp == 1) out_to(1);
         bar_sync_step();
-        const bool whole = w.t0 == 0 && w.t1 == s.tiles;
-        constexpr int E = D / 32;
-        // its parts: the one a CTA ends its share with (slot 1), then those that begin with a cut (slot 0)
-        int c_lo, c_hi;
-        cuts.inside(w.base, s.tiles, c_lo, c_hi);
         if (warp == 0) {
             add_from(1);
             unsigned bad = 0;  // rows with a value that is not finite
+            if (s.n > 1) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float x = 0.f;
+#pragma unroll
+                        for (int k = 0; k < KK; ++k) x = fmaf(o[k][nt][i], 0.f, fmaf(o[k][nt][2 + i], 0.f, x));
+                        if (x != x) bad |= 1u << (8 * nt + 2 * tq + i);
+                    }
+                bad = __reduce_or_sync(0xffffffffu, bad);
+            }
+            out_to(0);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = 8 * nt + 2 * tq + i;
-                    float x = 0.f;
-#pragma unroll
-                    for (int k = 0; k < KK; ++k)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float v = o[k][nt][2 * h + i];
-                            const int d = Q8 ? gq * (D / 8) + 2 * k + h : 16 * k + gq + 8 * h;
-                            merge[r * D + d] = v;
-                            x = fmaf(v, 0.f, x);
-                        }
-                    if (x != x) bad |= 1u << r;
+                for (int i = 0; i < 2; ++i)
                     if (gq == 0)
-                        *reinterpret_cast<float4*>(wstat + r * 4) = make_float4(m1[nt][i], m0[nt][i], l[nt][i], 0.f);
-                }
-            bad = __reduce_or_sync(0xffffffffu, bad);
-            __syncwarp();
-            // with several new tokens, keys a row does not see may have spoilt it
-            if (s.n > 1 && bad) {
-                for (int r = 0; r < s.rows; ++r) {
-                    const int seen = min(s.len, past + r / p.G + 1);
-                    if (!((bad >> r) & 1) || seen >= w.t1 * kStepKeys) continue;
-                    float a[E], m, sum;
-                    row_alone<T, D, Q8 ? kPaged8 : kPaged>(p, RowOf{w.b, w.hk, s.first}, r, w.t0 * kStepKeys, seen, lane, a,
-                                                           m, sum);
+                        *reinterpret_cast<float4*>(wstat + (4 * RM + 8 * nt + 2 * tq + i) * 4) =
+                            make_float4(m1[nt][i], m0[nt][i], l[nt][i], __uint_as_float(bad));
+        }
+        bar_sync_step();
+        // a row per warp and round, E values of it per lane
+        const bool whole = w.t0 == 0 && w.t1 == s.tiles;
+        constexpr int E = D / 32;
+        const int slot = 2 * (int)blockIdx.x + (w.t0 == 0);
+        for (int rb = warp; rb < s.rows; rb += 8) {  // rows rb, rb + 4
+            float4 x[2];
+            float a[2][E];
 #pragma unroll
-                    for (int j = 0; j < E; ++j) merge[r * D + lane * E + j] = a[j];
-                    if (lane == 0) *reinterpret_cast<float4*>(wstat + r * 4) = make_float4(m, m, sum, 0.f);
+            for (int y = 0; y < 2; ++y) {
+                const int r = min(rb + 4 * y, RM - 1);
+                x[y] = *reinterpret_cast<const float4*>(wstat + (4 * RM + r) * 4);
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    // where warp 0's lane and register of (row r, value d) went
+                    const int d = lane * E + j;
+                    const int k = Q8 ? (d % (D / 8)) >> 1 : d >> 4, gl = Q8 ? d / (D / 8) : d & 7, h = Q8 ? d & 1 : (d >> 3) & 1;
+                    a[y][j] = merge[((k * NT + (r >> 3)) * 32 + gl * 4 + ((r & 7) >> 1)) * 4 + 2 * h + (r & 1)];
                 }
-                __syncwarp();
             }
-            const int slot = 2 * (int)blockIdx.x + (w.t0 == 0);
-            for (int r = 0; r < s.rows; ++r) {
-                const float4 x = *reinterpret_cast<const float4*>(wstat + r * 4);
-                float a[E];
 #pragma unroll
-                for (int j = 0; j < E; ++j) a[j] = merge[r * D + lane * E + j];
+            for (int y = 0; y < 2; ++y) {
+                const int r = rb + 4 * y;
+                if (r >= s.rows) break;
+                // with several new tokens, keys a row does not see may have spoilt it
+                if (s.n > 1 && ((__float_as_uint(x[y].w) >> r) & 1)) {
+                    const int seen = min(s.len, past + r / p.G + 1);
+                    if (seen < w.t1 * kStepKeys) {
+                        row_alone<T, D, Q8 ? kPaged8 : kPaged>(p, RowOf{w.b, w.hk, s.first}, r, w.t0 * kStepKeys, seen, lane,
+                                                               a[y], x[y].x, x[y].z);
+                        x[y].y = x[y].x;
+                    }
+                }
                 if (whole) {
-                    store_row<T, E>(p, w.hk, s.first, r, lane, a, x);
+                    store_row<T, E>(p, w.hk, s.first, r, lane, a[y], x[y]);
                 } else {
                     float* d = sp.part + ((int64_t)slot * RM + r) * D + lane * E;
 #pragma unroll
-                    for (int j = 0; j < E; j += 2) *reinterpret_cast<float2*>(d + j) = make_float2(a[j], a[j + 1]);
-                    if (lane == 0) *reinterpret_cast<float4*>(sp.stat + ((int64_t)slot * RM + r) * 4) = x;
-                }
-            }
-            if (!whole) {
-                __syncwarp();
-                if (lane == 0) {
-                    uint32_t* n = sp.arrived + w.b * p.Hkv + w.hk;
-                    const bool last = add_acq_rel(n, 1u) == (uint32_t)(c_hi - c_lo + 1);
-                    if (last) *n = 0u;  // every part is here: nobody else looks at it in this call
-                    last_part = last;
+                    for (int j = 0; j < E; j += 2) *reinterpret_cast<float2*>(d + j) = make_float2(a[y][j], a[y][j + 1]);
+                    if (lane == 0) *reinterpret_cast<float4*>(sp.stat + ((int64_t)slot * RM + r) * 4) = x[y];
                 }
             }
         }
+        // its parts: the one a CTA ends its share with (slot 1), then those that begin with a cut (slot 0)
         if (!whole) {
-            bar_sync_step();
-            if (last_part) {
-                join_parts<T, D, NT>(sp, s.rows, w.hk, s.first, c_lo - 1, c_hi - c_lo + 2, merge, wstat, warp, lane);
+            int c0 = (int)blockIdx.x - w.part, parts = w.parts;
+            if (!parts) {
+                int hi;
+                cuts.inside(w.base, s.tiles, c0, hi);
+                --c0;
+                parts = hi - c0 + 1;
             }
+            bar_sync_step();
+            if (threadIdx.x == 0) {
+                uint32_t* n = sp.arrived + w.b * p.Hkv + w.hk;
+                const bool last = add_acq_rel(n, 1u) == (uint32_t)(parts - 1);
+                if (last) *n = 0u;  // every part is here: nobody else looks at it in this call
+                last_part = last;
+            }
+            bar_sync_step();
+            if (last_part) join_parts<T, D, NT>(sp, s.rows, w.hk, s.first, c0, parts, warp, lane);
         }
     }
 }
