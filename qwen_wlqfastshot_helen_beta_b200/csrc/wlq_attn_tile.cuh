@@ -61,7 +61,7 @@ struct TilePlan {
     static constexpr int kBlock = kKeys * 128;       // bytes of one block
     static constexpr int kTileBytes = kBlock * kHalves;
     static constexpr int kQBytes = 2 * kTileBytes;
-    static constexpr int kStageBytes = kKeys * D;    // 8-bit codes of one tile
+    static constexpr int kStageBytes = kKeys * D + kKeys;  // 8-bit codes of one tile and their rows' scales
     static constexpr int kStages = SRC == kPaged8 ? 3 : 0;
     static constexpr int kBudget = 227 * 1024 - 2048 - kQBytes - kStages * kStageBytes;
     static constexpr int kFit = kBudget / kTileBytes;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
             mbar_init(empty(s), 1);
         }
         for (int s = 0; s < NST; ++s) {
-            mbar_init(st_full(s), 1);
+            mbar_init(st_full(s), 33);  // the producer's bytes; its lanes' copies of the scales
             mbar_init(st_empty(s), 4);
         }
         mbar_fence_init();
@@ -629,17 +629,19 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     tma_load_3d(sb + t * P::kTileBytes + h * P::kBlock, &tp.tm_q, q_full, h * 64, u.hk * p.G,
                                 u.first + u.tok0 + t * tp.nt);
         }
+        int ids = 0;  // paged: the page of this lane's 16 keys of a window of 4 tiles; one outside the pool reads as zeros
         for (int i = 0; i < n && ok; ++i) {
             const int kb = key0 + i * kKeys;
-            int z = 0, pages = 1;
+            int id = 0, y = 0, keys = kKeys;
             if constexpr (kPagedSrc) {
-                // this lane's page of the tile; one outside the pool reads as zeros
-                const int ps = p.page_size;
-                pages = (min(kKeys, u.len - kb) + ps - 1) >> p.log2_page;
-                if (lane < pages) {
-                    const int id = p.table[(int64_t)u.b * p.table_cols + (kb >> p.log2_page) + lane];
-                    z = (id >= 0 && id < p.num_pages ? id : (int)p.num_pages) * p.Hkv + u.hk;
+                if ((i & 3) == 0) {
+                    const int key = min(kb + lane * 16, u.len - 1);
+                    ids = p.table[(int64_t)u.b * p.table_cols + (key >> p.log2_page)];
+                    if (ids < 0 || ids >= p.num_pages) ids = (int)p.num_pages;
                 }
+                id = __shfl_sync(0xffffffffu, ids, 8 * (i & 3) + (lane & 7));
+                y = (kb + (lane & 7) * 16) & (p.page_size - 1);
+                keys = (min(kKeys, u.len - kb) + p.page_size - 1) & -p.page_size;  // whole pages
             }
             for (int kv = 0; kv < 2 && ok; ++kv, ++g) {
                 const int s = g % NR, use = g / NR;
@@ -653,16 +655,22 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                             tma_load_3d(slot(s) + h * P::kBlock, map, rfull(s), h * 64, u.hk, u.first + kb);
                     }
                 } else {
-                    const int ps = p.page_size;
-                    if (lane == 0) mbar_arrive_expect_tx(rfull(s), pages * ps * (SRC == kPaged8 ? D : 2 * D));
+                    if (lane == 0) mbar_arrive_expect_tx(rfull(s), keys * (SRC == kPaged8 ? D : 2 * D));
                     __syncwarp();
-                    if (lane < pages) {
+                    if constexpr (SRC == kPaged8) {
+                        const bool in = id < p.num_pages;
+                        const int64_t row = ((int64_t)(in ? id : 0) * p.Hkv + u.hk) * p.page_size + y;
+                        if (lane < 8) cp_async16(stage(s) + kKeys * D + lane * 16, (kv ? p.v_exp : p.k_exp) + row, in);
+                        cp_async_arrive(rfull(s));
+                    }
+                    if (lane * 16 < keys && y == 0) {  // a page begins here (tiles begin with a page)
+                        const int z = id * p.Hkv + u.hk;
                         if constexpr (SRC == kPaged8) {
-                            tma_load_3d(stage(s) + lane * ps * D, map, rfull(s), 0, 0, z);
+                            tma_load_3d(stage(s) + lane * 16 * D, map, rfull(s), 0, 0, z);
                         } else {
 #pragma unroll
                             for (int h = 0; h < P::kHalves; ++h)
-                                tma_load_3d(slot(s) + h * P::kBlock + lane * ps * 128, map, rfull(s), h * 64, 0, z);
+                                tma_load_3d(slot(s) + h * P::kBlock + lane * 16 * 128, map, rfull(s), h * 64, 0, z);
                         }
                     }
                 }
@@ -694,16 +702,6 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                 const int keys = min(kKeys, u.len - kb);
                 for (int kv = 0; kv < 2 && ok; ++kv) {
                     const int g = 2 * i + kv, st = g % NST, s = g % NS;
-                    // the rows' scales, before the waits
-                    const uint8_t* exps = kv ? p.v_exp : p.k_exp;
-                    uint32_t e[C];
-#pragma unroll
-                    for (int x = 0; x < C; ++x) {
-                        const int key = min(kb + r0 + x * (128 / C), u.len - 1);
-                        const int id = p.table[(int64_t)u.b * p.table_cols + (key >> p.log2_page)];
-                        const bool in = id >= 0 && id < p.num_pages;
-                        e[x] = exps[((int64_t)(in ? id : 0) * p.Hkv + u.hk) * p.page_size + (key & (p.page_size - 1))];
-                    }
                     if (!(ok = warp_wait(st_full(st), (g / NST) & 1))) break;
                     if (g >= NS && !(ok = warp_wait(empty(s), (g / NS - 1) & 1))) break;
 #pragma unroll
@@ -712,7 +710,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                         uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
                         if (r < keys) {
                             const uint4 q = lds128(stage(st) + r * D + ch * 16);
-                            const float sc = exp2_biased(e[x]);
+                            const float sc = exp2_biased(lds8(stage(st) + kKeys * D + r));
                             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
                             uint32_t o[8];
 #pragma unroll
@@ -725,8 +723,10 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                             lo = make_uint4(o[0], o[1], o[2], o[3]);
                             hi = make_uint4(o[4], o[5], o[6], o[7]);
                         }
-                        sts128(slot(s) + tile_chunk(r, 2 * ch), lo);
-                        sts128(slot(s) + tile_chunk(r, 2 * ch + 1), hi);
+                        // (the two column blocks' lanes write their chunks in opposite order: no bank twice)
+                        const int odd = (ch >> 2) & 1;
+                        sts128(slot(s) + tile_chunk(r, 2 * ch + odd), odd ? hi : lo);
+                        sts128(slot(s) + tile_chunk(r, 2 * ch + 1 - odd), odd ? lo : hi);
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
