@@ -16,7 +16,7 @@ size_t attention_workspace_bytes(int Hq, int Hkv, int D, int max_q) {
     // two parts per CTA of the step kernel (three CTAs per SM with 8 rows, two with 16), three CTAs' parts per SM of the tile
     // kernel
     const size_t rows = few_rows(max_q, Hq / Hkv) ? 2 * 2 * sms * kFewRows : 3 * sms * 256;
-    return WLQ_ATTENTION_ZERO_BYTES + rows * (D + 4) * sizeof(float);
+    return WLQ_ATTENTION_ZERO_BYTES + 64 * 1024 /* the tile kernel's list of joins */ + rows * (D + 4) * sizeof(float);
 }
 
 int launch_attention(const AttnParams& p, bool f16, cudaStream_t stream) {

@@ -49,6 +49,7 @@ constexpr int kKeys = 128;    // keys of one tile
 struct TileParams {
     CUtensorMap tm_q, tm_o, tm_k, tm_v;
     AttnParams a;
+    int* joins;   // number of row tiles that several CTAs share, then a Join for each
     float* part;  // [split CTAs][D / 4][kRows][4] unnormalised outputs of a part of the keys
     float* stat;  // [split CTAs][kRows][2] their row maxima (times c) and sums
     int sms;
@@ -77,6 +78,12 @@ struct TilePlan {
     static_assert(2 * kRegsSoftmax + (kThreads / 128 - 2) * kRegsOther == 65536 / kThreads / 8 * 8 * (kThreads / 128),
                   "register shares");
     static_assert(kSlots >= 3, "k and v tiles in flight");
+};
+
+// A row tile whose keys several CTAs share: the first part's slot (the next
+// ones follow Hkv apart), the parts, and the rows.
+struct alignas(8) Join {
+    int slot, parts, tok0, n, first, hk;
 };
 
 // What one CTA works on.
@@ -113,6 +120,7 @@ __device__ __forceinline__ Seq seq_of(const AttnParams& p, int nt, int b) {
     return s;
 }
 
+constexpr int kJoinListBytes = 64 * 1024;  // (at least two parts each: at most 3 * 148 / 2 entries)
 constexpr int kPartsPerSm = 3;  // CTAs that hold a part of their rows' keys, at most
 
 // Key tiles of one part (paged form), found by one warp: a sequence with more
@@ -200,6 +208,31 @@ __device__ __forceinline__ bool find_unit(const AttnParams& p, int nt, int sms, 
         slots += __shfl_sync(0xffffffffu, pcum, 31);
     }
     return false;
+}
+
+// The list of joins, written by one warp of CTA 0.
+__device__ __forceinline__ void list_joins(const AttnParams& p, int nt, int sms, int lane, int* out) {
+    const int per = tiles_per_part(p, nt, sms, lane);
+    Join* list = reinterpret_cast<Join*>(out + 2);
+    int count = 0, slots = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+        const int b = b0 + lane;
+        Seq s{};
+        int sp = 0;
+        if (b < p.B) {
+            s = seq_of<true>(p, nt, b);
+            sp = parts_of(s, per);
+        }
+        const int mine = sp > 1 ? s.rtiles * p.Hkv : 0;
+        const int at = count + warp_scan(mine, lane) - mine, slot = slots + warp_scan(mine * sp, lane) - mine * sp;
+        for (int x = 0; x < mine; ++x) {
+            const int rt = x / p.Hkv, hk = x - rt * p.Hkv;
+            list[at + x] = Join{slot + rt * sp * p.Hkv + hk, sp, (s.rtiles - 1 - rt) * 2 * nt, s.n, s.first, hk};
+        }
+        count = __shfl_sync(0xffffffffu, at + mine, 31);
+        slots = __shfl_sync(0xffffffffu, slot + mine * sp, 31);
+    }
+    if (lane == 0) out[0] = count;
 }
 
 // ------------------------------------------------------------ tcgen05 extras
@@ -348,7 +381,10 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
         tma_prefetch_desc(&tp.tm_o);
     }
     __syncthreads();
-    if (!work_here) return;
+    if (!work_here) {
+        if (kPagedSrc && blockIdx.x == 0 && threadIdx.x == 0) tp.joins[0] = 0;
+        return;
+    }
     if (warp == 8) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
@@ -484,7 +520,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     if (pdst) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            pdst[(16 * k + 8 * y + j) * kRows] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                            if (mine) pdst[(16 * k + 8 * y + j) * kRows] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
@@ -688,8 +724,12 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
             }
         }
         // no copy may still be landing when the CTA exits
-        if (n > 0) mbar_wait(q_full, 0);
+        if (n > 0) warp_wait(q_full, 0);
         for (int j = g > NR ? g - NR : 0; j < g; ++j) mbar_wait(rfull(j % NR), (j / NR) & 1);
+    } else if (warp == 10) {
+        if constexpr (kPagedSrc) {
+            if (blockIdx.x == 0) list_joins(p, tp.nt, tp.sms, lane, tp.joins);
+        }
     } else if constexpr (SRC == kPaged8) {
         if (warp >= 12) {
             // ------------------------------------------- codes -> 16-bit tiles
@@ -746,81 +786,87 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
     }
 }
 
-// Joins the parts of the sequences whose keys several CTAs shared: block (x,
-// y) takes 16 columns of the x-th such 256-row tile, a row per thread.  The
-// parts are added in the order of the keys.
+// Joins the parts of the row tiles whose keys several CTAs shared.  A piece of
+// work is 32 rows (a lane each) of 16 columns.  Few parts: a piece per warp.
+// Many: the parts of a piece go to the block's eight warps in turn, whose sums
+// are then added in the warps' order.  Either way the order of the sums does
+// not depend on timing.
+constexpr int kJoinWarps = 8;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kRows) attn_tile_join_kernel(const __grid_constant__ TileParams tp) {
+__global__ void __launch_bounds__(32 * kJoinWarps) attn_tile_join_kernel(const __grid_constant__ TileParams tp) {
     const AttnParams& p = tp.a;
-    __shared__ int sh[6];
+    __shared__ float sh[kJoinWarps][18][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) {
-        const int per = tiles_per_part(p, tp.nt, tp.sms, lane);
-        int before = 0, slots = 0, found = 0;
-        for (int b0 = 0; b0 < p.B && !found; b0 += 32) {
-            const int b = b0 + lane;
-            Seq s{};
-            int sp = 0;
-            if (b < p.B) {
-                s = seq_of<true>(p, tp.nt, b);
-                sp = parts_of(s, per);
-            }
-            const int mine = sp > 1 ? s.rtiles * p.Hkv : 0;
-            const int cum = warp_scan(mine, lane), scum = warp_scan(mine * sp, lane);
-            const unsigned hit = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + cum);
-            if (hit) {
-                found = 1;
-                if (lane == __ffs(hit) - 1) {
-                    const int x = (int)blockIdx.x - before - (cum - mine);
-                    const int hk = x % p.Hkv, rt = x / p.Hkv;
-                    sh[0] = slots + scum - mine * sp + rt * sp * p.Hkv + hk;  // slot of the first part
-                    sh[1] = sp;
-                    sh[2] = (s.rtiles - 1 - rt) * 2 * tp.nt;
-                    sh[3] = s.n;
-                    sh[4] = s.first;
-                    sh[5] = hk;
+    constexpr int kPieces = (kRows / 32) * (D / 16), kGroups = kPieces / kJoinWarps;
+    const int groups = tp.joins[0] * kGroups;
+    for (int i = blockIdx.x; i < groups; i += gridDim.x) {
+        const Join j = reinterpret_cast<const Join*>(tp.joins + 2)[i / kGroups];
+        const bool many = j.parts > kJoinWarps;
+        for (int q = 0; q < (many ? kJoinWarps : 1); ++q) {
+            // the 16 columns vary fastest: a group of 8 pieces shares its rows' statistics
+            const int piece = (i % kGroups) * kJoinWarps + (many ? q : warp);
+            const int rg = piece / (D / 16), col = piece % (D / 16);
+            const int r = rg * 32 + lane, rt = r & (kRowsT - 1), tk = j.tok0 + (r >> 7) * tp.nt + rt / p.G;
+            const bool mine = rt < tp.nt * p.G && tk < j.n;
+            if (!__any_sync(0xffffffffu, mine)) continue;  // many: the same for all warps
+            float m = -INFINITY, l = 0.f, o[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[x] = 0.f;
+#pragma unroll 2
+            for (int s = many ? warp : 0; s < j.parts; s += many ? kJoinWarps : 1) {
+                const int64_t at = j.slot + s * p.Hkv;
+                const float2 st = *reinterpret_cast<const float2*>(tp.stat + (at * kRows + r) * 2);
+                float4 v[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    v[x] = reinterpret_cast<const float4*>(tp.part)[(at * (D / 4) + col * 4 + x) * kRows + r];
+                const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.f : mn;
+                const float keep = exp2f(m - ref), f = exp2f(st.x - ref);
+                m = mn;
+                l = l * keep + st.y * f;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    o[4 * x] = o[4 * x] * keep + v[x].x * f;
+                    o[4 * x + 1] = o[4 * x + 1] * keep + v[x].y * f;
+                    o[4 * x + 2] = o[4 * x + 2] * keep + v[x].z * f;
+                    o[4 * x + 3] = o[4 * x + 3] * keep + v[x].w * f;
                 }
             }
-            before += __shfl_sync(0xffffffffu, cum, 31);
-            slots += __shfl_sync(0xffffffffu, scum, 31);
+            uint16_t* out = p.out + (int64_t)(j.first + tk) * p.o_tok + (j.hk * p.G + rt % p.G) * p.o_head + col * 16;
+            if (!many) {
+                const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+                if (mine)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        reinterpret_cast<uint4*>(out)[x] =
+                            make_uint4(pack2<T>(o[8 * x] * inv, o[8 * x + 1] * inv), pack2<T>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
+                                       pack2<T>(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
+                                       pack2<T>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+                continue;
+            }
+            sh[warp][16][lane] = m;
+            sh[warp][17][lane] = l;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) sh[warp][x][lane] = o[x];
+            __syncthreads();
+            float all = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int y = 0; y < kJoinWarps; ++y) all = fmaxf(all, sh[y][16][lane]);
+            const float ref = all == -INFINITY ? 0.f : all;
+            float a[2] = {0.f, 0.f};  // this warp's two of the 16 columns
+#pragma unroll
+            for (int y = 0; y < kJoinWarps; ++y) {
+                const float f = exp2f(sh[y][16][lane] - ref);
+                sum += sh[y][17][lane] * f;
+                a[0] += sh[y][2 * warp][lane] * f;
+                a[1] += sh[y][2 * warp + 1][lane] * f;
+            }
+            const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+            if (mine) *reinterpret_cast<uint32_t*>(out + 2 * warp) = pack2<T>(a[0] * inv, a[1] * inv);
+            __syncthreads();
         }
-        if (!found && lane == 0) sh[1] = 0;
     }
-    __syncthreads();
-    const int sp = sh[1];
-    if (sp == 0) return;
-    const int slot = sh[0], first = sh[4], hk = sh[5];
-    const int r = threadIdx.x, rt = r & (kRowsT - 1), tk = sh[2] + (r >> 7) * tp.nt + rt / p.G, h = hk * p.G + rt % p.G;
-    if (rt >= tp.nt * p.G || tk >= sh[3]) return;
-    float m = -INFINITY, l = 0.f, o[16];
-    for (int s = 0; s < sp; ++s) m = fmaxf(m, tp.stat[((int64_t)(slot + s * p.Hkv) * kRows + r) * 2]);
-    const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] = 0.f;
-#pragma unroll 2
-    for (int s = 0; s < sp; ++s) {
-        const int64_t at = slot + s * p.Hkv;
-        const float2 st = *reinterpret_cast<const float2*>(tp.stat + (at * kRows + r) * 2);
-        float4 v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[j] = reinterpret_cast<const float4*>(tp.part)[(at * (D / 4) + blockIdx.y * 4 + j) * kRows + r];
-        const float f = exp2f(st.x - ref);
-        l += st.y * f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // (a part the row saw nothing of has weight 0)
-            o[4 * j] += v[j].x * f;
-            o[4 * j + 1] += v[j].y * f;
-            o[4 * j + 2] += v[j].z * f;
-            o[4 * j + 3] += v[j].w * f;
-        }
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    uint4* d = reinterpret_cast<uint4*>(p.out + (int64_t)(first + tk) * p.o_tok + h * p.o_head + blockIdx.y * 16);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-        d[j] = make_uint4(pack2<T>(o[8 * j] * inv, o[8 * j + 1] * inv), pack2<T>(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
-                          pack2<T>(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack2<T>(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
 }
 
 template <typename T, int D, int SRC>
@@ -854,7 +900,9 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
             (rc = encode_3d(&tp.tm_v, dt, a.v_cache, D, ps, pg, D * es, ps * D * es, box, ps, 1, sw, "v_cache")))
             return rc;
     }
-    tp.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + WLQ_ATTENTION_ZERO_BYTES);
+    tp.joins = reinterpret_cast<int*>(static_cast<uint8_t*>(a.ws) + WLQ_ATTENTION_ZERO_BYTES);
+    static_assert(sizeof(Join) == 24, "the list's entries");
+    tp.part = reinterpret_cast<float*>(tp.joins) + kJoinListBytes / 4;
     tp.stat = tp.part + (size_t)kPartsPerSm * tp.sms * kRows * D;
     const int64_t grid = (a.T / (2 * tp.nt) + a.B) * a.Hkv + (SRC == kPacked ? 0 : kPartsPerSm * tp.sms);
     if (grid > 0x7fffffff) return fail(WLQ_ERR_UNSUPPORTED, "attention: %lld row tiles in one call", (long long)grid);
@@ -864,7 +912,7 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
     attn_tile_kernel<T, D, SRC><<<(unsigned)grid, P::kThreads, P::kAlloc, stream>>>(tp);
     if ((rc = check_cuda(cudaGetLastError(), "attn_tile_kernel"))) return rc;
     if constexpr (SRC != kPacked) {
-        attn_tile_join_kernel<T, D><<<dim3(kPartsPerSm * tp.sms / 2, D / 16), kRows, 0, stream>>>(tp);
+        attn_tile_join_kernel<T, D><<<4 * tp.sms, 32 * kJoinWarps, 0, stream>>>(tp);
         rc = check_cuda(cudaGetLastError(), "attn_tile_join_kernel");
     }
     return rc;
