@@ -29,7 +29,7 @@
 //                     us for a prompt of 8192 tokens and 28 heads, 439 so)
 //   warp 9            TMA producer of q and of the k and v tiles: packed rows,
 //                     or one copy per page
-//   warps 12..15      8-bit caches: the pages' codes land in a staging ring
+//   warps 12..19      8-bit caches: the pages' codes land in a staging ring
 //                     and are written as the 16-bit tiles the MMAs read,
 //                     code * 2^e, which is exact
 //
@@ -47,6 +47,7 @@ namespace {
 constexpr int kRowsT = 128;   // query rows of one tile (MMA M)
 constexpr int kRows = 256;    // query rows of one CTA
 constexpr int kKeys = 128;    // keys of one tile
+constexpr int kConvWarps = 8; // warps that turn codes into 16-bit tiles
 
 struct TileParams {
     CUtensorMap tm_q, tm_o, tm_k, tm_v;
@@ -65,7 +66,7 @@ struct TilePlan {
     static constexpr int kTileBytes = kBlock * kHalves;
     static constexpr int kQBytes = 2 * kTileBytes;
     static constexpr int kStageBytes = kKeys * D + kKeys;  // 8-bit codes of one tile and their rows' scales
-    static constexpr int kStages = SRC == kPaged8 ? 3 : 0;
+    static constexpr int kStages = SRC == kPaged8 ? 2 : 0;
     static constexpr int kBudget = 227 * 1024 - 2048 - kQBytes - kStages * kStageBytes;
     static constexpr int kFit = kBudget / kTileBytes;
     static constexpr int kSlots = kFit > 8 ? 8 : kFit;
@@ -74,9 +75,9 @@ struct TilePlan {
     static constexpr int kBarOff = kStageOff + kStages * kStageBytes;
     static constexpr int kAlloc = kBarOff + 512 + 1024;  // barriers, alignment slack
     // registers a thread: the softmax groups hold a row's 128 scores; the
-    // groups' shares add up to what the block is launched with (168 x 3, 128 x 4)
-    static constexpr int kThreads = SRC == kPaged8 ? 512 : 384;
-    static constexpr int kRegsSoftmax = SRC == kPaged8 ? 184 : 208, kRegsOther = SRC == kPaged8 ? 72 : 88;
+    // groups' shares add up to what the block is launched with (168 x 3, 96 x 5)
+    static constexpr int kThreads = SRC == kPaged8 ? 640 : 384;
+    static constexpr int kRegsSoftmax = SRC == kPaged8 ? 168 : 208, kRegsOther = SRC == kPaged8 ? 48 : 88;
     static_assert(2 * kRegsSoftmax + (kThreads / 128 - 2) * kRegsOther == 65536 / kThreads / 8 * 8 * (kThreads / 128),
                   "register shares");
     static_assert(kSlots >= 3, "k and v tiles in flight");
@@ -369,12 +370,12 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
             mbar_init(pv_done(t), 1);
         }
         for (int s = 0; s < NS; ++s) {
-            mbar_init(full(s), SRC == kPaged8 ? 4 : 1);
+            mbar_init(full(s), SRC == kPaged8 ? kConvWarps : 1);
             mbar_init(empty(s), 1);
         }
         for (int s = 0; s < NST; ++s) {
             mbar_init(st_full(s), 33);  // the producer's bytes; its lanes' copies of the scales
-            mbar_init(st_empty(s), 4);
+            mbar_init(st_empty(s), kConvWarps);
         }
         mbar_fence_init();
         tma_prefetch_desc(&tp.tm_q);
@@ -744,7 +745,8 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
     } else if constexpr (SRC == kPaged8) {
         if (warp >= 12) {
             // ------------------------------------------- codes -> 16-bit tiles
-            constexpr int C = D / 16;  // 16-code chunks of a row
+            constexpr int C = D / 16;             // 16-code chunks of a row
+            constexpr int R = 32 * kConvWarps / C;  // rows of one round
             const int tid = threadIdx.x - 384;
             const int ch = tid % C, r0 = tid / C;
             bool ok = true;
@@ -756,8 +758,8 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     if (!(ok = warp_wait(st_full(st), (g / NST) & 1))) break;
                     if (g >= NS && !(ok = warp_wait(empty(s), (g / NS - 1) & 1))) break;
 #pragma unroll
-                    for (int x = 0; x < C; ++x) {
-                        const int r = r0 + x * (128 / C);
+                    for (int x = 0; x < kKeys / R; ++x) {
+                        const int r = r0 + x * R;
                         uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
                         if (r < keys) {
                             const uint4 q = lds128(stage(st) + r * D + ch * 16);
