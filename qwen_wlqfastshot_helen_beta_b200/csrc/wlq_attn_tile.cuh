@@ -5,10 +5,9 @@
 // M_i), c = scale log2(e), the sums taken tile by tile with a running
 // reference M_i; both sums carry the same factor, so M_i only has to keep the
 // exponentials in range.  It is raised, and the output accumulator rescaled,
-// only when a row's maximum has grown by more than 2^8: the probabilities
-// then stay below 256, no precision is lost (they are floating-point numbers
-// and the sum is fp32), and after the first tiles the accumulator is hardly
-// ever touched.
+// only when a probability would pass 2^14 (fp16 ends at 2^16): no precision is
+// lost, they are floating-point numbers and the sum is fp32, and after the
+// first tiles the accumulator is hardly ever touched.
 //
 // A tile's 128 rows are whole tokens of one sequence times the G query heads
 // of one kv head, token-major (128 / G tokens, rounded down), so that a short
@@ -47,6 +46,7 @@ namespace {
 constexpr int kRowsT = 128;   // query rows of one tile (MMA M)
 constexpr int kRows = 256;    // query rows of one CTA
 constexpr int kKeys = 128;    // keys of one tile
+constexpr float kGrow = 14.f; // powers of two a row's maximum may pass its reference by
 constexpr int kConvWarps = 8; // warps that turn codes into 16-bit tiles
 
 struct TileParams {
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     mx[k] = fmaxf(mx[k], __uint_as_float(s[k][31]));
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if (__any_sync(0xffffffffu, mine && (top - m) * c > 8.f)) {
+                if (__any_sync(0xffffffffu, mine && (top - m) * c > kGrow)) {
                     const float mn = fmaxf(m, top);
                     const float f = mn == m ? 1.f : ex2((m - mn) * c);
                     m = mn;
@@ -623,21 +623,25 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     const uint32_t off = (k >> 2) * kBlock16 + (k & 3) * 2;
                     umma_f16(tmem + t * 128, q0 + off, k0 + off, id_s, k > 0);
                 }
-                umma_commit(s_full(t));
             };
             const int nh = halves;
             const bool fix = SRC != kPaged8 && last_keys < kKeys;
             bool ok = mbar_wait(q_full, 0) && mbar_wait(full(0), 0);
             tc_fence_after_sync();
-            for (int t = 0; ok && t < nh; ++t) issue_s(t, 0);
+            for (int t = 0; ok && t < nh; ++t) {
+                issue_s(t, 0);
+                umma_commit(s_full(t));
+            }
             // tiles arrive as K0 V0 K1 V1 ...
             int sv = 1 % NS, sk = 2 % NS, pv = 0, pk = 2 / NS & 1;  // slots of V_i and K_i+1, their phases
+            auto arrived = [&](int i) {
+                return mbar_wait(full(sv), pv) && (i + 1 < n ? mbar_wait(full(sk), pk) : !fix || mbar_wait(v_fixed, 0));
+            };
+            ok = ok && arrived(0);
             for (int i = 0; ok && i < n; ++i) {
                 const bool more = i + 1 < n;
-                if (!(ok = mbar_wait(full(sv), pv))) break;
-                if (fix && !more && !(ok = mbar_wait(v_fixed, 0))) break;
-                if (more && !(ok = mbar_wait(full(sk), pk))) break;
                 const uint64_t v0 = dv + (uint32_t)sv * kTile16;
+                const int slot_k = sk;
                 for (int t = 0; ok && t < nh; ++t) {
                     const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * D;
                     // the first 64 keys' products run while the other probabilities are computed
@@ -652,13 +656,16 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     if (!ok) break;
                     // one commit a tile (the next scores, over P in TMEM: the MMAs of a thread run in order); the
                     // slots are handed back by the softmax that sees it: a commit holds the issuing thread up until
-                    // the MMAs before it are nearly done
-                    if (more) issue_s(t, sk);
-                    else umma_commit(pv_done(t));
+                    // the MMAs before it are nearly done, so the next tiles' arrival is looked at before it
+                    if (more) issue_s(t, slot_k);
+                    if (t + 1 == nh) {
+                        sv += 2, sk += 2;
+                        if (sv >= NS) sv -= NS, pv ^= 1;
+                        if (sk >= NS) sk -= NS, pk ^= 1;
+                        if (more) ok = arrived(i + 1);
+                    }
+                    umma_commit(more ? s_full(t) : pv_done(t));
                 }
-                sv += 2, sk += 2;
-                if (sv >= NS) sv -= NS, pv ^= 1;
-                if (sk >= NS) sk -= NS, pk ^= 1;
             }
         }
         __syncwarp();
