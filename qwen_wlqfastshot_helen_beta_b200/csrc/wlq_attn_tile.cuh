@@ -52,7 +52,7 @@ constexpr int kConvWarps = 8; // warps that turn codes into 16-bit tiles
 struct TileParams {
     CUtensorMap tm_q, tm_o, tm_k, tm_v;
     AttnParams a;
-    int* joins;   // number of row tiles that several CTAs share, then a Join for each
+    int* joins;   // numbers of row tiles that several CTAs share (few parts, many), then a Join for each
     float* part;  // [split CTAs][D / 4][kRows][4] unnormalised outputs of a part of the keys
     float* stat;  // [split CTAs][kRows][2] their row maxima (times c) and sums
     int sms;
@@ -213,11 +213,15 @@ __device__ __forceinline__ bool find_unit(const AttnParams& p, int nt, int sms, 
     return false;
 }
 
-// The list of joins, written by one warp of CTA 0.
+// The lists of joins, written by one warp of CTA 0: those of up to
+// kJoinWarps parts from the front, the others from the back.
+constexpr int kJoinWarps = 8;
+constexpr int kMaxJoins = (kJoinListBytes - 8) / (int)sizeof(Join);
+
 __device__ __forceinline__ void list_joins(const AttnParams& p, int nt, int sms, int lane, int* out) {
     const int per = tiles_per_part(p, nt, sms, lane);
     Join* list = reinterpret_cast<Join*>(out + 2);
-    int count = 0, slots = 0;
+    int few = 0, many = 0, slots = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
         const int b = b0 + lane;
         Seq s{};
@@ -227,15 +231,22 @@ __device__ __forceinline__ void list_joins(const AttnParams& p, int nt, int sms,
             sp = parts_of(s, per);
         }
         const int mine = sp > 1 ? s.rtiles * p.Hkv : 0;
-        const int at = count + warp_scan(mine, lane) - mine, slot = slots + warp_scan(mine * sp, lane) - mine * sp;
+        const int nf = sp <= kJoinWarps ? mine : 0, nm = mine - nf;
+        const int at_f = few + warp_scan(nf, lane) - nf, at_m = many + warp_scan(nm, lane) - nm;
+        const int slot = slots + warp_scan(mine * sp, lane) - mine * sp;
         for (int x = 0; x < mine; ++x) {
             const int rt = x / p.Hkv, hk = x - rt * p.Hkv;
-            list[at + x] = Join{slot + rt * sp * p.Hkv + hk, sp, (s.rtiles - 1 - rt) * 2 * nt, s.n, s.first, hk};
+            list[nf ? at_f + x : kMaxJoins - 1 - (at_m + x)] =
+                Join{slot + rt * sp * p.Hkv + hk, sp, (s.rtiles - 1 - rt) * 2 * nt, s.n, s.first, hk};
         }
-        count = __shfl_sync(0xffffffffu, at + mine, 31);
+        few = __shfl_sync(0xffffffffu, at_f + nf, 31);
+        many = __shfl_sync(0xffffffffu, at_m + nm, 31);
         slots = __shfl_sync(0xffffffffu, slot + mine * sp, 31);
     }
-    if (lane == 0) out[0] = count;
+    if (lane == 0) {
+        out[0] = few;
+        out[1] = many;
+    }
 }
 
 // ------------------------------------------------------------ tcgen05 extras
@@ -383,12 +394,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
         tma_prefetch_desc(&tp.tm_v);
         tma_prefetch_desc(&tp.tm_o);
     }
-    __syncthreads();
-    if (!work_here) {
-        if (kPagedSrc && blockIdx.x == 0 && threadIdx.x == 0) tp.joins[0] = 0;
-        return;
-    }
-    if (warp == 8) {
+    if (warp == 8) {  // beside the search
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -396,6 +402,11 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sgen + P::kBarOff + (tmem_slot - bars));
+    if (!work_here) {
+        if (kPagedSrc && blockIdx.x == 0 && threadIdx.x < 2) tp.joins[threadIdx.x] = 0;
+        if (warp == 8) tmem_dealloc(tmem, 512);
+        return;
+    }
     const Unit& u = su;  // read where it is used: its fields would take the softmax threads' registers
     const int n = u.tiles;
     const int halves = u.tok0 + tp.nt < u.n ? 2 : 1;
@@ -807,85 +818,82 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
 }
 
 // Joins the parts of the row tiles whose keys several CTAs shared.  A piece of
-// work is 32 rows (a lane each) of 16 columns.  Few parts: a piece per warp.
-// Many: the parts of a piece go to the block's eight warps in turn, whose sums
-// are then added in the warps' order.  Either way the order of the sums does
+// work is 32 rows (a lane each) of 16 columns.  Up to eight parts: a piece per
+// warp.  More: a piece per block, its parts go to the eight warps in turn, and
+// the warps' sums are added in their order.  Either way the order of the sums does
 // not depend on timing.
-constexpr int kJoinWarps = 8;
-
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) attn_tile_join_kernel(const __grid_constant__ TileParams tp) {
     const AttnParams& p = tp.a;
     __shared__ float sh[kJoinWarps][18][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kPieces = (kRows / 32) * (D / 16), kGroups = kPieces / kJoinWarps;
-    const int groups = tp.joins[0] * kGroups;
-    for (int i = blockIdx.x; i < groups; i += gridDim.x) {
-        const Join j = reinterpret_cast<const Join*>(tp.joins + 2)[i / kGroups];
-        const bool many = j.parts > kJoinWarps;
-        for (int q = 0; q < (many ? kJoinWarps : 1); ++q) {
-            // the 16 columns vary fastest: a group of 8 pieces shares its rows' statistics
-            const int piece = (i % kGroups) * kJoinWarps + (many ? q : warp);
-            const int rg = piece / (D / 16), col = piece % (D / 16);
-            const int r = rg * 32 + lane, rt = r & (kRowsT - 1), tk = j.tok0 + (r >> 7) * tp.nt + rt / p.G;
-            const bool mine = rt < tp.nt * p.G && tk < j.n;
-            if (!__any_sync(0xffffffffu, mine)) continue;  // many: the same for all warps
-            float m = -INFINITY, l = 0.f, o[16];
+    const int groups = tp.joins[0] * kGroups, items = groups + tp.joins[1] * kPieces;
+    const Join* list = reinterpret_cast<const Join*>(tp.joins + 2);
+    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+        const bool many = i >= groups;
+        const Join j = list[many ? kMaxJoins - 1 - (i - groups) / kPieces : i / kGroups];
+        // the 16 columns vary fastest: a group of 8 pieces shares its rows' statistics
+        const int piece = many ? (i - groups) % kPieces : (i % kGroups) * kJoinWarps + warp;
+        const int rg = piece / (D / 16), col = piece % (D / 16);
+        const int r = rg * 32 + lane, rt = r & (kRowsT - 1), tk = j.tok0 + (r >> 7) * tp.nt + rt / p.G;
+        const bool mine = rt < tp.nt * p.G && tk < j.n;
+        if (!__any_sync(0xffffffffu, mine)) continue;  // many: the same for all warps
+        float m = -INFINITY, l = 0.f, o[16];
 #pragma unroll
-            for (int x = 0; x < 16; ++x) o[x] = 0.f;
+        for (int x = 0; x < 16; ++x) o[x] = 0.f;
 #pragma unroll 2
-            for (int s = many ? warp : 0; s < j.parts; s += many ? kJoinWarps : 1) {
-                const int64_t at = j.slot + s * p.Hkv;
-                const float2 st = *reinterpret_cast<const float2*>(tp.stat + (at * kRows + r) * 2);
-                float4 v[4];
+        for (int s = many ? warp : 0; s < j.parts; s += many ? kJoinWarps : 1) {
+            const int64_t at = j.slot + s * p.Hkv;
+            const float2 st = *reinterpret_cast<const float2*>(tp.stat + (at * kRows + r) * 2);
+            float4 v[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    v[x] = reinterpret_cast<const float4*>(tp.part)[(at * (D / 4) + col * 4 + x) * kRows + r];
-                const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.f : mn;
-                const float keep = exp2f(m - ref), f = exp2f(st.x - ref);
-                m = mn;
-                l = l * keep + st.y * f;
+            for (int x = 0; x < 4; ++x)
+                v[x] = reinterpret_cast<const float4*>(tp.part)[(at * (D / 4) + col * 4 + x) * kRows + r];
+            const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.f : mn;
+            const float keep = exp2f(m - ref), f = exp2f(st.x - ref);
+            m = mn;
+            l = l * keep + st.y * f;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    o[4 * x] = o[4 * x] * keep + v[x].x * f;
-                    o[4 * x + 1] = o[4 * x + 1] * keep + v[x].y * f;
-                    o[4 * x + 2] = o[4 * x + 2] * keep + v[x].z * f;
-                    o[4 * x + 3] = o[4 * x + 3] * keep + v[x].w * f;
-                }
+            for (int x = 0; x < 4; ++x) {
+                o[4 * x] = o[4 * x] * keep + v[x].x * f;
+                o[4 * x + 1] = o[4 * x + 1] * keep + v[x].y * f;
+                o[4 * x + 2] = o[4 * x + 2] * keep + v[x].z * f;
+                o[4 * x + 3] = o[4 * x + 3] * keep + v[x].w * f;
             }
-            uint16_t* out = p.out + (int64_t)(j.first + tk) * p.o_tok + (j.hk * p.G + rt % p.G) * p.o_head + col * 16;
-            if (!many) {
-                const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-                if (mine)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        reinterpret_cast<uint4*>(out)[x] =
-                            make_uint4(pack2<T>(o[8 * x] * inv, o[8 * x + 1] * inv), pack2<T>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
-                                       pack2<T>(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
-                                       pack2<T>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
-                continue;
-            }
-            sh[warp][16][lane] = m;
-            sh[warp][17][lane] = l;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) sh[warp][x][lane] = o[x];
-            __syncthreads();
-            float all = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int y = 0; y < kJoinWarps; ++y) all = fmaxf(all, sh[y][16][lane]);
-            const float ref = all == -INFINITY ? 0.f : all;
-            float a[2] = {0.f, 0.f};  // this warp's two of the 16 columns
-#pragma unroll
-            for (int y = 0; y < kJoinWarps; ++y) {
-                const float f = exp2f(sh[y][16][lane] - ref);
-                sum += sh[y][17][lane] * f;
-                a[0] += sh[y][2 * warp][lane] * f;
-                a[1] += sh[y][2 * warp + 1][lane] * f;
-            }
-            const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-            if (mine) *reinterpret_cast<uint32_t*>(out + 2 * warp) = pack2<T>(a[0] * inv, a[1] * inv);
-            __syncthreads();
         }
+        uint16_t* out = p.out + (int64_t)(j.first + tk) * p.o_tok + (j.hk * p.G + rt % p.G) * p.o_head + col * 16;
+        if (!many) {
+            const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+            if (mine)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    reinterpret_cast<uint4*>(out)[x] =
+                        make_uint4(pack2<T>(o[8 * x] * inv, o[8 * x + 1] * inv), pack2<T>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
+                                   pack2<T>(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
+                                   pack2<T>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+            continue;
+        }
+        sh[warp][16][lane] = m;
+        sh[warp][17][lane] = l;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sh[warp][x][lane] = o[x];
+        __syncthreads();
+        float all = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int y = 0; y < kJoinWarps; ++y) all = fmaxf(all, sh[y][16][lane]);
+        const float ref = all == -INFINITY ? 0.f : all;
+        float a[2] = {0.f, 0.f};  // this warp's two of the 16 columns
+#pragma unroll
+        for (int y = 0; y < kJoinWarps; ++y) {
+            const float f = exp2f(sh[y][16][lane] - ref);
+            sum += sh[y][17][lane] * f;
+            a[0] += sh[y][2 * warp][lane] * f;
+            a[1] += sh[y][2 * warp + 1][lane] * f;
+        }
+        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+        if (mine) *reinterpret_cast<uint32_t*>(out + 2 * warp) = pack2<T>(a[0] * inv, a[1] * inv);
+        __syncthreads();
     }
 }
 

@@ -43,6 +43,13 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
     return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
 }
 
+// 16 bytes that this kernel may write later (q_out may be q): not by the read-only path
+__device__ __forceinline__ uint4 ld16(const void* p) {
+    uint4 r;
+    asm("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
@@ -51,19 +58,21 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 
 // A warp takes one token (its cos/sin values stay in registers) and walks
 // part of the token's heads, 32 / G rows at a time, kAhead such steps' loads in
-// flight: G lanes share a row, each with two 8-value chunks that hold both
+// flight, then the next token: G lanes share a row, each with two 8-value chunks that hold both
 // members of its pairs.  Few tokens spread their heads over several warps
 // (`parts`), so that a decoding step is one round of loads.
 constexpr int kAhead = 3;
+constexpr int kRopeCtas = 4;  // per SM (at most 128 registers a thread)
 
 template <typename T, bool QUANT, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads) rope_kv_write_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeCtas) rope_kv_write_kernel(const RopeParams p) {
     const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
-    const int64_t tok = w / p.parts;
+    const int64_t w0 = (int64_t)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
+    const int64_t step = (int64_t)gridDim.x * (kRopeThreads / 32) / p.parts;  // tokens of a round
+    const int part = (int)(w0 % p.parts);
+    int64_t tok = w0 / p.parts;
     if (tok >= p.T) return;
-    const int64_t pos = p.positions[tok];
-    const int64_t slot = p.slots[tok];
+    int64_t next_pos = p.positions[tok], next_slot = p.slots[tok];
     const int G = p.lanes_per_row, rows = 32 / G;
     const int l = lane & (G - 1), sub = lane / G;
     const bool live = 16 * l < p.D;  // D / 16 lanes work where G is rounded up
@@ -81,7 +90,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kv_write_kernel(const RopeP
     }
     if (!live) ca = cb = 0;
     const int heads = p.Hq + 2 * p.Hkv;
-    const int part = (int)(w - tok * p.parts), stride = p.parts * rows;
+    const int stride = p.parts * rows;
     uint4 xa[kAhead], xb[kAhead];
     auto load = [&](int h0) {
 #pragma unroll
@@ -90,123 +99,130 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kv_write_kernel(const RopeP
             const uint16_t* src = h < p.Hq           ? p.q + tok * p.q_tok + h * p.q_head
                                   : h < p.Hq + p.Hkv ? p.k + tok * p.k_tok + (h - p.Hq) * p.k_head
                                                      : p.v + tok * p.v_tok + (h - p.Hq - p.Hkv) * p.v_head;
-            xa[u] = ldg16(src + 8 * ca);
-            xb[u] = ldg16(src + 8 * cb);
+            xa[u] = ld16(src + 8 * ca);
+            xb[u] = ld16(src + 8 * cb);
         }
     };
-    load(part * rows);
-    if (pos < 0 || pos >= p.table_rows) {
-        if (lane == 0) atomicOr(&g_position_error, 1u);
-        return;
-    }
-    const bool store = slot >= 0 && slot < p.num_pages * p.page_size;  // a negative slot: a padding token
-    const int64_t page = store ? slot / p.page_size : 0;
-    const int off = store ? (int)(slot - page * p.page_size) : 0;
-
-    // interleaved: 4 pairs of each chunk; halves: 8 pairs across the chunks
-    float cs[8], sn[8];
-    const float* row = p.cos_sin + pos * p.rot;
-    const bool turn_a = live && ca < nrot, turn_b = live && cb < nrot;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
-    {
-        const int ia = INTER ? 4 * ca : 8 * ca, ib = INTER ? 4 * cb : 8 * ca + 4;
-        if (turn_a) {
-            const float4 c = *reinterpret_cast<const float4*>(row + ia);
-            const float4 s = *reinterpret_cast<const float4*>(row + p.rot / 2 + ia);
-            cs[0] = c.x, cs[1] = c.y, cs[2] = c.z, cs[3] = c.w;
-            sn[0] = s.x, sn[1] = s.y, sn[2] = s.z, sn[3] = s.w;
+    for (; tok < p.T; tok += step) {
+        load(part * rows);
+        const int64_t pos = next_pos, slot = next_slot;
+        if (tok + step < p.T) {  // the next token's, while this one is worked on
+            next_pos = p.positions[tok + step];
+            next_slot = p.slots[tok + step];
         }
-        if (turn_b) {
-            const float4 c = *reinterpret_cast<const float4*>(row + ib);
-            const float4 s = *reinterpret_cast<const float4*>(row + p.rot / 2 + ib);
-            cs[4] = c.x, cs[5] = c.y, cs[6] = c.z, cs[7] = c.w;
-            sn[4] = s.x, sn[5] = s.y, sn[6] = s.z, sn[7] = s.w;
+        if (pos < 0 || pos >= p.table_rows) {
+            if (lane == 0) atomicOr(&g_position_error, 1u);
+            continue;
         }
-    }
+        const bool store = slot >= 0 && slot < p.num_pages * p.page_size;  // a negative slot: a padding token
+        const int64_t page = store ? slot / p.page_size : 0;
+        const int off = store ? (int)(slot - page * p.page_size) : 0;
 
-    for (int h0 = part * rows; h0 < heads; h0 += kAhead * stride) {
-        if (h0 != part * rows) load(h0);
+        // interleaved: 4 pairs of each chunk; halves: 8 pairs across the chunks
+        float cs[8], sn[8];
+        const float* row = p.cos_sin + pos * p.rot;
+        const bool turn_a = live && ca < nrot, turn_b = live && cb < nrot;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (h0 + u * stride >= heads) break;  // uniform over the warp
-            const int h = h0 + u * stride + sub;
-            const bool ok = live && h < heads;
-            const int kind = h < p.Hq ? 0 : (h < p.Hq + p.Hkv ? 1 : 2);  // q, k, v
-            const int hh = kind == 0 ? h : (kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv);
-            float a[8], b[8];
-            unpack8<T>(keep_if(ok, xa[u]), a);
-            unpack8<T>(keep_if(ok, xb[u]), b);
-            if (kind != 2) {
-                if (INTER) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], t = b[2 * i + 1];
-                        if (turn_a) {
-                            a[2 * i] = x * cs[i] - y * sn[i];
-                            a[2 * i + 1] = y * cs[i] + x * sn[i];
-                        }
-                        if (turn_b) {
-                            b[2 * i] = z * cs[4 + i] - t * sn[4 + i];
-                            b[2 * i + 1] = t * cs[4 + i] + z * sn[4 + i];
-                        }
-                    }
-                } else if (turn_a) {  // both chunks are rotated, or neither
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float x = a[i], y = b[i];
-                        a[i] = x * cs[i] - y * sn[i];
-                        b[i] = y * cs[i] + x * sn[i];
-                    }
-                }
+        for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
+        {
+            const int ia = INTER ? 4 * ca : 8 * ca, ib = INTER ? 4 * cb : 8 * ca + 4;
+            if (turn_a) {
+                const float4 c = *reinterpret_cast<const float4*>(row + ia);
+                const float4 s = *reinterpret_cast<const float4*>(row + p.rot / 2 + ia);
+                cs[0] = c.x, cs[1] = c.y, cs[2] = c.z, cs[3] = c.w;
+                sn[0] = s.x, sn[1] = s.y, sn[2] = s.z, sn[3] = s.w;
             }
-            uint16_t* d = kind == 0   ? p.q_out + tok * p.qo_tok + hh * p.qo_head
-                          : kind == 1 ? p.k_out + tok * p.ko_tok + hh * p.ko_head
-                                      : nullptr;
-            if (ok && (kind == 0 || (kind == 1 && p.k_out))) {
-                *reinterpret_cast<uint4*>(d + 8 * ca) = pack8<T>(a);
-                *reinterpret_cast<uint4*>(d + 8 * cb) = pack8<T>(b);
+            if (turn_b) {
+                const float4 c = *reinterpret_cast<const float4*>(row + ib);
+                const float4 s = *reinterpret_cast<const float4*>(row + p.rot / 2 + ib);
+                cs[4] = c.x, cs[5] = c.y, cs[6] = c.z, cs[7] = c.w;
+                sn[4] = s.x, sn[5] = s.y, sn[6] = s.z, sn[7] = s.w;
             }
-            if (!store || h0 + u * stride + rows <= p.Hq) continue;  // uniform over the warp
-            const int64_t crow = (page * p.Hkv + hh) * p.page_size + off;
-            if constexpr (QUANT) {
-                if (ActTraits<T>::kIsF16) {
-                    // the largest e4m3 grid value below 65504, so that what is read back stays finite in fp16
+        }
+
+        for (int h0 = part * rows; h0 < heads; h0 += kAhead * stride) {
+            if (h0 != part * rows) load(h0);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        a[i] = fminf(fmaxf(a[i], -61440.f), 61440.f);
-                        b[i] = fminf(fmaxf(b[i], -61440.f), 61440.f);
+            for (int u = 0; u < kAhead; ++u) {
+                if (h0 + u * stride >= heads) break;  // uniform over the warp
+                const int h = h0 + u * stride + sub;
+                const bool ok = live && h < heads;
+                const int kind = h < p.Hq ? 0 : (h < p.Hq + p.Hkv ? 1 : 2);  // q, k, v
+                const int hh = kind == 0 ? h : (kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv);
+                float a[8], b[8];
+                unpack8<T>(keep_if(ok, xa[u]), a);
+                unpack8<T>(keep_if(ok, xb[u]), b);
+                if (kind != 2) {
+                    if (INTER) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], t = b[2 * i + 1];
+                            if (turn_a) {
+                                a[2 * i] = x * cs[i] - y * sn[i];
+                                a[2 * i + 1] = y * cs[i] + x * sn[i];
+                            }
+                            if (turn_b) {
+                                b[2 * i] = z * cs[4 + i] - t * sn[4 + i];
+                                b[2 * i + 1] = t * cs[4 + i] + z * sn[4 + i];
+                            }
+                        }
+                    } else if (turn_a) {  // both chunks are rotated, or neither
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float x = a[i], y = b[i];
+                            a[i] = x * cs[i] - y * sn[i];
+                            b[i] = y * cs[i] + x * sn[i];
+                        }
                     }
                 }
-                float top = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(a[i]), fabsf(b[i])));
-                for (int x = 1; x < G; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                // top = m 2^x with m in [1, 2) and 448 = 1.75 * 2^8
-                const uint32_t bits = __float_as_uint(top);
-                const int e = max(1, (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));  // + 127
-                const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-                if (ok && kind != 0) {
-                    uint8_t* c8 = reinterpret_cast<uint8_t*>(kind == 1 ? p.k_cache : p.v_cache) + crow * p.D;
-                    *reinterpret_cast<uint2*>(c8 + 8 * ca) =
-                        make_uint2(e4m3x4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv),
-                                   e4m3x4(a[4] * inv, a[5] * inv, a[6] * inv, a[7] * inv));
-                    *reinterpret_cast<uint2*>(c8 + 8 * cb) =
-                        make_uint2(e4m3x4(b[0] * inv, b[1] * inv, b[2] * inv, b[3] * inv),
-                                   e4m3x4(b[4] * inv, b[5] * inv, b[6] * inv, b[7] * inv));
-                    if (l == 0) (kind == 1 ? p.k_exp : p.v_exp)[crow] = (uint8_t)e;
+                uint16_t* d = kind == 0   ? p.q_out + tok * p.qo_tok + hh * p.qo_head
+                              : kind == 1 ? p.k_out + tok * p.ko_tok + hh * p.ko_head
+                                          : nullptr;
+                if (ok && (kind == 0 || (kind == 1 && p.k_out))) {
+                    *reinterpret_cast<uint4*>(d + 8 * ca) = pack8<T>(a);
+                    *reinterpret_cast<uint4*>(d + 8 * cb) = pack8<T>(b);
                 }
-            } else if (ok && kind != 0) {
-                uint16_t* c16 = reinterpret_cast<uint16_t*>(kind == 1 ? p.k_cache : p.v_cache) + crow * p.D;
-                *reinterpret_cast<uint4*>(c16 + 8 * ca) = pack8<T>(a);
-                *reinterpret_cast<uint4*>(c16 + 8 * cb) = pack8<T>(b);
+                if (!store || h0 + u * stride + rows <= p.Hq) continue;  // uniform over the warp
+                const int64_t crow = (page * p.Hkv + hh) * p.page_size + off;
+                if constexpr (QUANT) {
+                    if (ActTraits<T>::kIsF16) {
+                        // the largest e4m3 grid value below 65504, so that what is read back stays finite in fp16
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            a[i] = fminf(fmaxf(a[i], -61440.f), 61440.f);
+                            b[i] = fminf(fmaxf(b[i], -61440.f), 61440.f);
+                        }
+                    }
+                    float top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(a[i]), fabsf(b[i])));
+                    for (int x = 1; x < G; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    // top = m 2^x with m in [1, 2) and 448 = 1.75 * 2^8
+                    const uint32_t bits = __float_as_uint(top);
+                    const int e = max(1, (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));  // + 127
+                    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+                    if (ok && kind != 0) {
+                        uint8_t* c8 = reinterpret_cast<uint8_t*>(kind == 1 ? p.k_cache : p.v_cache) + crow * p.D;
+                        *reinterpret_cast<uint2*>(c8 + 8 * ca) =
+                            make_uint2(e4m3x4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv),
+                                       e4m3x4(a[4] * inv, a[5] * inv, a[6] * inv, a[7] * inv));
+                        *reinterpret_cast<uint2*>(c8 + 8 * cb) =
+                            make_uint2(e4m3x4(b[0] * inv, b[1] * inv, b[2] * inv, b[3] * inv),
+                                       e4m3x4(b[4] * inv, b[5] * inv, b[6] * inv, b[7] * inv));
+                        if (l == 0) (kind == 1 ? p.k_exp : p.v_exp)[crow] = (uint8_t)e;
+                    }
+                } else if (ok && kind != 0) {
+                    uint16_t* c16 = reinterpret_cast<uint16_t*>(kind == 1 ? p.k_cache : p.v_cache) + crow * p.D;
+                    *reinterpret_cast<uint4*>(c16 + 8 * ca) = pack8<T>(a);
+                    *reinterpret_cast<uint4*>(c16 + 8 * cb) = pack8<T>(b);
+                }
             }
         }
     }
 }
 
 // A CTA reads back `tokens` consecutive rows of the packed output, all heads
-// of k then of v: the first threads look the rows' cache slots up, then every
+// of k or of v: the first threads look the rows' cache slots up, then every
 // thread moves 16 values per item (16 codes or 32 bytes in, one 32-byte store
 // out), four items' loads in flight.  Rows outside the table or the pool are
 // zeros.
@@ -236,50 +252,49 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const KvReadParam
     const int per = p.Hkv * (p.D >> 4);  // items of one token
     const int n = nt * per;
     constexpr int U = 4;
-    for (int which = 0; which < 2; ++which) {
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(which ? p.v_cache : p.k_cache);
-        const uint8_t* exps = which ? p.v_exp : p.k_exp;
-        uint16_t* dst = (which ? p.v_out : p.k_out) + t0 * per * 16;
-        for (int i0 = threadIdx.x; i0 < n; i0 += U * kReadThreads) {
-            Words8 w[U];
-            uint32_t e[U];
-            bool in[U];
+    const int which = blockIdx.y;  // k, v
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(which ? p.v_cache : p.k_cache);
+    const uint8_t* exps = which ? p.v_exp : p.k_exp;
+    uint16_t* dst = (which ? p.v_out : p.k_out) + t0 * per * 16;
+    for (int i0 = threadIdx.x; i0 < n; i0 += U * kReadThreads) {
+        Words8 w[U];
+        uint32_t e[U];
+        bool in[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = min(i0 + u * kReadThreads, n - 1);
-                const int tk = p.per_magic ? __umulhi((uint32_t)i, p.per_magic) : i;
-                const int x = i - tk * per;
-                const int h = p.chunk_magic ? __umulhi((uint32_t)x, p.chunk_magic) : x;
-                const int64_t r = base[tk];
-                in[u] = r >= 0;
-                const int64_t row = in[u] ? r + (int64_t)h * p.page_size : 0;
-                const int64_t at = row * p.D + 16 * (x - h * (p.D >> 4));
-                if constexpr (QUANT) {
-                    const uint4 q = ldg16(src + at);
-                    w[u].w[0] = q.x, w[u].w[1] = q.y, w[u].w[2] = q.z, w[u].w[3] = q.w;
-                    e[u] = __ldg(exps + row);
-                } else {
-                    w[u] = ldg32(src + at * 2);
+        for (int u = 0; u < U; ++u) {
+            const int i = min(i0 + u * kReadThreads, n - 1);
+            const int tk = p.per_magic ? __umulhi((uint32_t)i, p.per_magic) : i;
+            const int x = i - tk * per;
+            const int h = p.chunk_magic ? __umulhi((uint32_t)x, p.chunk_magic) : x;
+            const int64_t r = base[tk];
+            in[u] = r >= 0;
+            const int64_t row = in[u] ? r + (int64_t)h * p.page_size : 0;
+            const int64_t at = row * p.D + 16 * (x - h * (p.D >> 4));
+            if constexpr (QUANT) {
+                const uint4 q = ldg16(src + at);
+                w[u].w[0] = q.x, w[u].w[1] = q.y, w[u].w[2] = q.z, w[u].w[3] = q.w;
+                e[u] = __ldg(exps + row);
+            } else {
+                w[u] = ldg32(src + at * 2);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            Words8 o = w[u];
+            if constexpr (QUANT) {
+                const float s = exp2_biased(e[u]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float f[4];
+                    e4m3x4_to_f32(w[u].w[j], f);
+                    o.w[2 * j] = pack2<T>(f[0] * s, f[1] * s);
+                    o.w[2 * j + 1] = pack2<T>(f[2] * s, f[3] * s);
                 }
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                Words8 o = w[u];
-                if constexpr (QUANT) {
-                    const float s = exp2_biased(e[u]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float f[4];
-                        e4m3x4_to_f32(w[u].w[j], f);
-                        o.w[2 * j] = pack2<T>(f[0] * s, f[1] * s);
-                        o.w[2 * j + 1] = pack2<T>(f[2] * s, f[3] * s);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o.w[j] = in[u] ? o.w[j] : 0u;
-                const int i = i0 + u * kReadThreads;
-                if (i < n) stg32(dst + (int64_t)i * 16, o);
-            }
+            for (int j = 0; j < 8; ++j) o.w[j] = in[u] ? o.w[j] : 0u;
+            const int i = i0 + u * kReadThreads;
+            if (i < n) stg32(dst + (int64_t)i * 16, o);
         }
     }
 }
@@ -295,9 +310,11 @@ int launch_rope_kv_write(RopeParams& p, bool f16, bool quant, cudaStream_t strea
     const int steps = (p.Hq + 2 * p.Hkv + 32 / p.lanes_per_row - 1) / (32 / p.lanes_per_row);
     // enough warps for 16 per SM before a warp walks several steps
     const int64_t want = (int64_t)device_sm_count() * 16;
-    p.parts = (int)std::min<int64_t>(steps, std::max<int64_t>(1, (want + p.T - 1) / p.T));
-    const int64_t warps = p.T * p.parts;
-    const unsigned grid = (unsigned)((warps + kRopeThreads / 32 - 1) / (kRopeThreads / 32));
+    const int64_t resident = (int64_t)device_sm_count() * kRopeCtas;
+    p.parts = (int)std::min(std::min<int64_t>(steps, resident), std::max<int64_t>(1, (want + p.T - 1) / p.T));
+    // CTAs that fit at once; their warps walk the tokens (a multiple of `parts` warps: the same part each time)
+    const int64_t warps = p.T * p.parts, per = kRopeThreads / 32;
+    const unsigned grid = (unsigned)std::min((warps + per - 1) / per, resident / p.parts * p.parts);
     auto run = [&](auto kernel) { kernel<<<grid, kRopeThreads, 0, stream>>>(p); };
     auto typed = [&](auto t) {
         using T = decltype(t);
@@ -315,7 +332,7 @@ int launch_kv_read(KvReadParams& p, bool f16, bool quant, cudaStream_t stream) {
     p.tokens = p.T >= (int64_t)device_sm_count() * 2 * kReadTokens ? kReadTokens : 8;
     p.per_magic = magic_u32((uint32_t)(p.Hkv * (p.D >> 4)));
     p.chunk_magic = magic_u32((uint32_t)(p.D >> 4));
-    const unsigned grid = (unsigned)((p.T + p.tokens - 1) / p.tokens);
+    const dim3 grid((unsigned)((p.T + p.tokens - 1) / p.tokens), 2);
     if (f16)
         quant ? kv_read_kernel<__half, true><<<grid, kReadThreads, 0, stream>>>(p)
               : kv_read_kernel<__half, false><<<grid, kReadThreads, 0, stream>>>(p);
