@@ -6,7 +6,12 @@ custom ops (the reference schema with optional trailing arguments for
 per-group codebooks, the prepacked layout and ``lora_A``, the DoRA matrix A
 given in place of h = A x so the decode GEMV computes h itself; ``out``
 mutated, fake implementations for CUDA-graph capture and torch.compile),
-``init_workspaces`` and the ``register`` vLLM plugin entry point.  ``WLQFastShotConfig`` / ``WLQLinearMethod`` import vLLM
+``init_workspaces`` and the ``register`` vLLM plugin entry point.  The attention
+operators between the projections (rotary positions with a paged cache's write,
+its read-back, attention of prompts and over the cache) are in ``_C`` and, with
+the same arguments, torch ops of the same namespace; ``attention`` has their
+tables and caches, ``attention_block`` runs them with the linears.
+``WLQFastShotConfig`` / ``WLQLinearMethod`` import vLLM
 and are loaded on first access.
 """
 from __future__ import annotations
@@ -98,6 +103,78 @@ def _register_ops():
         return None
 
 
+def _register_attention_ops():
+    """The attention operators as torch ops (the same arguments as the _C
+    functions, outputs and caches mutated in place), for graphs and
+    torch.compile; eager callers that count microseconds call _C."""
+
+    @torch.library.custom_op("wlq_fastShot::rope_kv_write",
+                             mutates_args={"k_cache", "v_cache", "q_out", "k_out", "k_exp", "v_exp"})
+    def _rope(
+        q: torch.Tensor,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        positions: torch.Tensor,
+        cos_sin: torch.Tensor,
+        slots: torch.Tensor,
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        q_out: torch.Tensor,
+        k_out: Optional[torch.Tensor] = None,
+        k_exp: Optional[torch.Tensor] = None,
+        v_exp: Optional[torch.Tensor] = None,
+        interleaved: bool = False,
+    ) -> None:
+        _C.rope_kv_write(q, k, v, positions, cos_sin, slots, k_cache, v_cache, q_out, k_out, k_exp, v_exp, interleaved)
+
+    @torch.library.custom_op("wlq_fastShot::kv_read", mutates_args={"k_out", "v_out"})
+    def _read(
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        block_table: torch.Tensor,
+        cu_lens: torch.Tensor,
+        k_out: torch.Tensor,
+        v_out: torch.Tensor,
+        k_exp: Optional[torch.Tensor] = None,
+        v_exp: Optional[torch.Tensor] = None,
+    ) -> None:
+        _C.kv_read(k_cache, v_cache, block_table, cu_lens, k_out, v_out, k_exp, v_exp)
+
+    @torch.library.custom_op("wlq_fastShot::prompt_attention", mutates_args={"out"})
+    def _prompt(
+        q: torch.Tensor,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        cu_seqlens: torch.Tensor,
+        out: torch.Tensor,
+        scale: Optional[float] = None,
+        causal: bool = True,
+    ) -> None:
+        _C.prompt_attention(q, k, v, cu_seqlens, out, scale, causal)
+
+    @torch.library.custom_op("wlq_fastShot::paged_attention", mutates_args={"out"})
+    def _paged(
+        q: torch.Tensor,
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        block_table: torch.Tensor,
+        kv_lens: torch.Tensor,
+        out: torch.Tensor,
+        cu_q: Optional[torch.Tensor] = None,
+        max_q: int = 1,
+        k_exp: Optional[torch.Tensor] = None,
+        v_exp: Optional[torch.Tensor] = None,
+        scale: Optional[float] = None,
+    ) -> None:
+        _C.paged_attention(q, k_cache, v_cache, block_table, kv_lens, out, cu_q, max_q, k_exp, v_exp, scale)
+
+    def _fake(*args, **kwargs):
+        return None
+
+    for op in (_rope, _read, _prompt, _paged):
+        op.register_fake(_fake)
+
+
 def _ops_registered() -> bool:
     try:
         return torch._C._dispatch_has_kernel_for_dispatch_key("wlq_fastShot::gemv", "CompositeExplicitAutograd") or \
@@ -108,6 +185,7 @@ def _ops_registered() -> bool:
 
 if not _ops_registered():
     _register_ops()
+    _register_attention_ops()
 
 
 def init_workspaces(max_N: int, max_K: int, device: torch.device):

@@ -1,0 +1,118 @@
+"""The attention operators without a GPU: refusals of the C ABI and of the
+Python calls, rotary tables, the cache's tensors."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+P = 1 << 20  # a 16-byte aligned address that is never used
+
+
+def lib():
+    from qwen_wlqfastshot_helen_beta_b200._lib import lib
+    return lib
+
+
+def rope(T=1, rows=8, pages=4, Hq=4, Hkv=2, D=64, rot=64, page=16, dtype=1, ke=None, ve=None, q=P, cs=P, tok=256):
+    return lib().wlq_rope_kv_write(q, P, P, P, cs, P, P, P, ke, ve, P, None, tok, 64, 128, 64, 128, 64, 256, 64, 0, 0, T,
+                                   rows, pages, Hq, Hkv, D, rot, page, 0, dtype, None)
+
+
+def prompt(T=2, B=1, Hq=4, Hkv=2, D=64, scale=0.1, dtype=1, tok=256, out=P):
+    return lib().wlq_prompt_attention(P, P, P, P, out, tok, 64, 128, 64, 128, 64, 256, 64, T, B, Hq, Hkv, D, scale, 1,
+                                      dtype, None)
+
+
+def paged(T=2, B=2, Hq=4, Hkv=2, D=64, page=16, max_q=1, scale=0.1, ke=None, ve=None, cu=None, cols=4):
+    return lib().wlq_paged_attention(P, P, P, ke, ve, P, P, cu, P, 256, 64, 256, 64, T, B, Hq, Hkv, D, page, 8, cols,
+                                     max_q, scale, 1, None, 0, None)
+
+
+def read(T=1, B=1, Hkv=2, D=64, page=16, ke=None, ve=None, out=P):
+    return lib().wlq_kv_read(P, P, ke, ve, P, P, out, P, T, B, 8, 4, Hkv, D, page, 1, None)
+
+
+@pytest.mark.parametrize("call,code,word", [
+    (lambda: rope(T=-1), 1, b"T=-1"), (lambda: rope(rows=0), 1, b"table rows"), (lambda: rope(dtype=5), 2, b"act_dtype"),
+    (lambda: rope(Hq=5), 1, b"heads"), (lambda: rope(D=72), 2, b"head size"), (lambda: rope(D=512), 2, b"head size"),
+    (lambda: rope(rot=40), 2, b"rotated"), (lambda: rope(rot=80), 2, b"rotated"), (lambda: rope(page=8), 2, b"page_size"),
+    (lambda: rope(page=48), 2, b"page_size"), (lambda: rope(ke=P), 1, b"k_exp"), (lambda: rope(q=P + 8), 3, b"aligned"),
+    (lambda: rope(tok=250), 3, b"aligned"), (lambda: rope(cs=P + 4), 3, b"cos_sin"), (lambda: rope(cs=None), 1, b"cos_sin"),
+    (lambda: prompt(D=80), 2, b"head size"), (lambda: prompt(scale=0.0), 1, b"scale"),
+    (lambda: prompt(scale=float("nan")), 1, b"scale"), (lambda: prompt(scale=float("inf")), 1, b"scale"),
+    (lambda: prompt(Hq=6, Hkv=4), 1, b"heads"), (lambda: prompt(Hq=129, Hkv=1), 2, b"128 query heads"),
+    (lambda: prompt(out=None), 1, b"out"), (lambda: prompt(out=P + 2), 3, b"aligned"), (lambda: prompt(B=0), 1, b"cu_seqlens"),
+    (lambda: paged(D=96), 2, b"head size"), (lambda: paged(T=3), 1, b"without cu_q"), (lambda: paged(max_q=2), 1, b"without cu_q"),
+    (lambda: paged(max_q=0), 1, b"size"), (lambda: paged(ke=P), 1, b"k_exp"), (lambda: paged(ke=P + 4, ve=P), 3, b"k_exp"),
+    (lambda: paged(T=70000, B=70000), 2, b"sequences"), (lambda: paged(cols=1 << 30), 2, b"too many"),
+    (lambda: read(D=20), 2, b"head size"), (lambda: read(out=None), 1, b"required"), (lambda: read(out=P + 4), 3, b"aligned"),
+    (lambda: read(ve=P), 1, b"k_exp"),
+])
+def test_refusals(call, code, word):
+    assert call() == code and word in lib().wlq_last_error()
+
+
+def test_nothing_to_do_is_no_error():
+    assert rope(T=0) == 0 and prompt(T=0, B=0) == 0 and paged(T=0, B=0) == 0 and read(T=0, B=0) == 0
+
+
+def test_python_refuses_cpu_tensors_and_wrong_arguments():
+    from qwen_wlqfastshot_helen_beta_b200 import _C, _calls
+    x = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    i = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="wlq: prompt_attention: q must be a CUDA tensor"):
+        _C.prompt_attention(x, x, x, i, x)
+    with pytest.raises(RuntimeError, match="wlq: paged_attention: q must be a tensor"):
+        _C.paged_attention(None, x, x, i, i, x)
+    with pytest.raises(RuntimeError, match="wlq: kv_read: k_out must be a CUDA tensor"):
+        _C.kv_read(x, x, i, i, x, x)
+    with pytest.raises(RuntimeError, match="wlq: rope_kv_write: q must be a CUDA tensor"):
+        _C.rope_kv_write(x, x, x, i, x, i, x, x, x)
+    with pytest.raises(TypeError):
+        _calls.kv_read(x)
+    with pytest.raises(TypeError):
+        _calls.setup((1, 2), RuntimeError)
+
+
+def test_rope_table():
+    from qwen_wlqfastshot_helen_beta_b200.attention import rope_frequencies, rope_table
+    t = rope_table(1000, 64, 1e4, device="cpu")
+    assert t.shape == (1000, 64) and t.dtype == torch.float32
+    for p, i in ((0, 0), (999, 0), (999, 31), (7, 13)):
+        a = p * 1e4 ** (-2 * i / 64)
+        assert abs(t[p, i].item() - math.cos(a)) < 6e-8 and abs(t[p, 32 + i].item() - math.sin(a)) < 6e-8
+    lin = rope_table(100, 32, 1e4, {"type": "linear", "factor": 4.0}, device="cpu")
+    assert torch.equal(lin[4::4], rope_table(25, 32, 1e4, device="cpu")[1:])  # position 4 n looks like position n
+    f, a = rope_frequencies(128, 1e6, {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768})
+    g, _ = rope_frequencies(128, 1e6)
+    assert abs(a - (0.1 * math.log(4) + 1)) < 1e-12
+    assert torch.equal(f[:10], g[:10]) and torch.allclose(f[-10:], g[-10:] / 4, rtol=1e-12)  # fast pairs kept, slow ones stretched
+    assert (f <= g).all() and (f >= g / 4 * (1 - 1e-12)).all() and (f[1:] < f[:-1]).all()
+    d, _ = rope_frequencies(64, 1e4, {"type": "dynamic", "factor": 2.0})
+    h, _ = rope_frequencies(64, 1e4)
+    assert d[0] == 1.0 and abs(d[-1] / h[-1] - 0.5) < 1e-9  # the slowest pair stretched by the factor
+    with pytest.raises(ValueError):
+        rope_frequencies(64, 1e4, {"type": "other", "factor": 2.0})
+
+
+def test_cache_tensors():
+    from qwen_wlqfastshot_helen_beta_b200.attention import PagedKVCache
+    c = PagedKVCache(5, 2, 64, 32, 8, torch.float16, "cpu")
+    k, v, ke, ve = c.tensors
+    assert k.shape == v.shape == (5, 2, 32, 64) and k.dtype == torch.float8_e4m3fn and ke.shape == (5, 2, 32)
+    assert c.nbytes() == 2 * 5 * 2 * 32 * 65
+    c = PagedKVCache(5, 2, 64, 32, 16, torch.float16, "cpu")
+    assert c.tensors[0].dtype == torch.float16 and c.tensors[2] is None and c.nbytes() == 2 * 5 * 2 * 32 * 64 * 2
+    with pytest.raises(ValueError):
+        PagedKVCache(5, 2, 64, 32, 4)
+
+
+def test_header_constants():
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = open(os.path.join(root, "include", "wlq_b200.h")).read()
+    assert re.search(r"WLQ_DEVERR_POSITION 2u", src) and re.search(r"WLQ_ATTENTION_ZERO_BYTES \(256u \* 1024u\)", src)
+    assert isinstance(lib().wlq_paged_attention_workspace_bytes(28, 4, 128, 1), int)
+    assert ctypes.sizeof(ctypes.c_size_t) == 8

@@ -484,3 +484,114 @@ def test_paged_attention_streams_and_graph():
     for i, n in enumerate([5, 700, 1]):
         k, v = R.gather(kc, ke, table, i, n), R.gather(vc, ve, table, i, n)
         R.check(out[i:i + 1], *R.attention(q[i:i + 1].double(), k, v, n, R.scale_of(D)))
+
+
+# ------------------------------------------------------- refusals, the block ---
+
+def test_refusals_on_the_gpu():
+    q = torch.zeros(3, 4, 64, device="cuda", dtype=torch.bfloat16)
+    k = torch.zeros(3, 2, 64, device="cuda", dtype=torch.bfloat16)
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    kc = torch.zeros(2, 2, 16, 64, device="cuda", dtype=torch.bfloat16)
+    tab, lens = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    f8 = kc.to(torch.float8_e4m3fn)
+    e8 = torch.zeros(2, 2, 16, dtype=torch.uint8, device="cuda")
+    i64 = torch.zeros(3, dtype=torch.int64, device="cuda")
+    cs = torch.zeros(4, 64, device="cuda")
+    bad = [
+        (lambda: C().prompt_attention(q.float(), k, k, cu, out), "float16 or bfloat16"),
+        (lambda: C().prompt_attention(q, k.half(), k, cu, out), "k must be"),
+        (lambda: C().prompt_attention(q, k[:2], k, cu, out), "k must be"),
+        (lambda: C().prompt_attention(q, k, k, cu.long(), out), "cu_seqlens must be"),
+        (lambda: C().prompt_attention(q, k, k, cu, out[:, :3]), "out must be"),
+        (lambda: C().prompt_attention(q.transpose(1, 2).contiguous().transpose(1, 2), k, k, cu, out), "contiguous"),
+        (lambda: C().prompt_attention(q, k, k, cu, out, -1.0), "scale"),
+        (lambda: C().prompt_attention(q, k, k, cu.cpu(), out), "must be on"),
+        (lambda: C().paged_attention(q, f8, f8, tab, lens, out), "8-bit cache needs"),
+        (lambda: C().paged_attention(q, f8, f8, tab, lens, out, None, 1, e8), "k_exp and v_exp"),
+        (lambda: C().paged_attention(q, kc, kc, tab, lens, out, None, 1, e8, e8), "must be"),
+        (lambda: C().paged_attention(q, kc, kc, tab[0], lens, out), "block_table"),
+        (lambda: C().paged_attention(q, kc, kc, tab, lens[:2], out), "kv_lens"),
+        (lambda: C().paged_attention(q, kc, kc, tab, lens, out, None, 4), "without cu_q"),
+        (lambda: C().paged_attention(q, kc[:, :, :10].contiguous(), kc[:, :, :10].contiguous(), tab, lens, out), "page_size"),
+        (lambda: C().paged_attention(q, kc.transpose(1, 2), kc, tab, lens, out), "k_cache"),
+        (lambda: C().kv_read(kc, kc, tab, lens, k, k), "cu_lens"),
+        (lambda: C().kv_read(kc, kc, tab[:1], cu, k[:, :1], k), "k_out"),
+        (lambda: C().rope_kv_write(q, k, k, i64.int(), cs, i64, kc, kc, out), "positions"),
+        (lambda: C().rope_kv_write(q, k, k, i64, cs[:, :24].contiguous(), i64, kc, kc, out), "rotated"),
+        (lambda: C().rope_kv_write(q, k, k, i64, cs[0], i64, kc, kc, out), "cos_sin"),
+        (lambda: C().rope_kv_write(q, k, k, i64[:2], cs, i64, kc, kc, out), "positions"),
+    ]
+    for call, word in bad:
+        with pytest.raises(RuntimeError, match=word):
+            call()
+    torch.cuda.synchronize()
+
+
+def test_torch_ops_agree_with_the_calls():
+    g = gen_of("ops")
+    T, Hq, Hkv, D, page = 20, 4, 2, 64, 16
+    q, k, v = (randn(g, T, h, D).bfloat16() for h in (Hq, Hkv, Hkv))
+    cs, pos = table_of(64, D), torch.arange(T, device="cuda")
+    table, pages = R.pages_of([T], page, g)
+    slots = table[0, pos // page].long() * page + pos % page
+    lens, cu = torch.tensor([T], dtype=torch.int32, device="cuda"), torch.tensor([0, T], dtype=torch.int32, device="cuda")
+
+    def run(ops):
+        kc, vc = (torch.zeros(pages, Hkv, page, D, device="cuda").to(torch.float8_e4m3fn) for _ in range(2))
+        ke, ve = (torch.full((pages, Hkv, page), 127, dtype=torch.uint8, device="cuda") for _ in range(2))
+        q2, k2 = torch.empty_like(q), torch.empty_like(k)
+        ops.rope_kv_write(q, k, v, pos, cs, slots, kc, vc, q2, k2, ke, ve, False)
+        a, b, ko, vo = torch.empty_like(q), torch.empty_like(q), torch.empty_like(k), torch.empty_like(k)
+        ops.prompt_attention(q2, k2, v, cu, a, None, True)
+        ops.paged_attention(q2, kc, vc, table, lens, b, cu, T, ke, ve, None)
+        ops.kv_read(kc, vc, table, cu, ko, vo, ke, ve)
+        return [q2, k2, a, b, ko, vo]
+
+    import qwen_wlqfastshot_helen_beta_b200  # noqa: F401  (registers the ops)
+    for x, y in zip(run(C()), run(torch.ops.wlq_fastShot)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("bits,tol", [(16, 2e-2), (8, 8e-2)])
+def test_attention_block(bits, tol):
+    """A prompt, a chunk and a single token through the block agree with the same tokens as one prompt: what the
+    cache holds and where it lies does not show, but for its own rounding (e4m3: up to 2^-4 of a value)."""
+    from qwen_wlqfastshot_helen_beta_b200.attention_block import synthetic_block
+    hidden, heads, kv_heads, d, page = 256, 4, 2, 64, 16
+    block = synthetic_block(hidden, heads, kv_heads, d, pages=24, page_size=page, bits=bits, max_position=256, seed=3)
+    lens = [70, 33]
+    g = gen_of("block")
+    table = torch.randperm(24, generator=g, device="cuda").to(torch.int32).view(2, 12)
+    xs = [(randn(g, n, hidden)).bfloat16() for n in lens]
+
+    def slots(s, a, b):
+        p = torch.arange(a, b, device="cuda")
+        return p, table[s, p // page].long() * page + p % page
+
+    def call(a, b, fn):  # tokens a[s] .. b[s] of both sequences
+        ps = [slots(s, a[s], b[s]) for s in range(2)]
+        cu = torch.tensor([0, b[0] - a[0], b[0] - a[0] + b[1] - a[1]], dtype=torch.int32, device="cuda")
+        x = torch.cat([xs[s][a[s]:b[s]] for s in range(2)])
+        y = fn(x, torch.cat([p for p, _ in ps]), torch.cat([q for _, q in ps]), cu)
+        return y.split([b[s] - a[s] for s in range(2)])
+
+    want = call([0, 0], lens, lambda x, p, s, cu: block.prompt(x, p, s, cu))
+    got = [[], []]
+    first, then = [40, 20], [69, 32]
+    steps = [([0, 0], first, lambda x, p, s, cu: block.prompt(x, p, s, cu))]
+
+    def extend(b):
+        kv = torch.tensor(b, dtype=torch.int32, device="cuda")
+        return lambda x, p, s, cu: block.extend(x, p, s, table, kv, cu, int((cu[1:] - cu[:-1]).max()))
+
+    steps.append((first, then, extend(then)))
+    kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    steps.append((then, lens, lambda x, p, s, cu: block.extend(x, p, s, table, kv)))
+    for a, b, fn in steps:
+        for s, y in enumerate(call(a, b, fn)):
+            got[s].append(y)
+    for s in range(2):
+        y, w = torch.cat(got[s]).float(), want[s].float()
+        assert ((y - w).norm() / w.norm()).item() <= tol
