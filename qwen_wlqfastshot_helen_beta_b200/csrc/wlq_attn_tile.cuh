@@ -330,6 +330,12 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // Byte offset of 16-byte chunk c (of 8 values) of row r in a tile: blocks of
 // 64 columns, the chunk index XORed with row % 8 inside a 128-byte row (the
 // layout TMA writes and tcgen05 reads).
@@ -463,7 +469,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                     mx[k] = __uint_as_float(s[k][0]);
 #pragma unroll
                     for (int j = 1; j < 31; j += 2)
-                        mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(s[k][j]), __uint_as_float(s[k][j + 1])));
+                        mx[k] = max3(mx[k], __uint_as_float(s[k][j]), __uint_as_float(s[k][j + 1]));
                     mx[k] = fmaxf(mx[k], __uint_as_float(s[k][31]));
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
