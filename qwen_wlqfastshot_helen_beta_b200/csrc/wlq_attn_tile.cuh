@@ -264,14 +264,44 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t 
     return d;
 }
 
-// D[tmem] (+)= A[tmem] * B[smem]: A is M x 16 16-bit values, two per column
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// One lane of a converged warp: 1 there, 0 in the others.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r;
+}
+// The MMAs and the commit of wlq_sm100.cuh, issued where `me` is set.
+__device__ __forceinline__ void umma_f16_if(uint32_t me, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(me)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]: A is M x 16 16-bit values, two per column
+__device__ __forceinline__ void umma_f16_ts_if(uint32_t me, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
+                                               uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(me)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(uint32_t me, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar), "r"(me)
         : "memory");
 }
 
@@ -626,49 +656,53 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
         }
     } else if (warp == 8) {
         // ------------------------------------------------------ MMA issue
-        if (lane == 0 && n > 0) {
+        // The whole warp runs the loop and one lane of it issues: addresses and descriptors are then the same in all
+        // lanes by construction, and stay in uniform registers, where the MMAs want them.
+        if (n > 0) {
             constexpr uint32_t fmt = ActTraits<T>::kIsF16 ? 0u : 1u;
             constexpr uint32_t id_s = umma_idesc_f16(fmt, kRowsT, kKeys);
             constexpr uint32_t id_o = umma_idesc_f16(fmt, kRowsT, D) | (1u << 16);  // V is stored with N contiguous
+            constexpr uint32_t kTile16 = P::kTileBytes >> 4, kBlock16 = P::kBlock >> 4;
             // descriptors hold addresses in units of 16 bytes: a tile's or block's offset is added to them as it is
             const uint64_t dq = umma_desc_sw128(sb), dk = umma_desc_sw128(slot(0)), dv = umma_desc_mn_sw128(slot(0), P::kBlock);
-            constexpr uint32_t kTile16 = P::kTileBytes >> 4, kBlock16 = P::kBlock >> 4;
+            const uint32_t me = elect_one();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             auto issue_s = [&](int t, int sl) {
                 const uint64_t q0 = dq + (uint32_t)t * kTile16, k0 = dk + (uint32_t)sl * kTile16;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t off = (k >> 2) * kBlock16 + (k & 3) * 2;
-                    umma_f16(tmem + t * 128, q0 + off, k0 + off, id_s, k > 0);
+                    umma_f16_if(me, tm + t * 128, q0 + off, k0 + off, id_s, k > 0);
                 }
             };
-            const int nh = halves;
+            const int nh = __shfl_sync(0xffffffffu, halves, 0), nn = __shfl_sync(0xffffffffu, n, 0);
             const bool fix = SRC != kPaged8 && last_keys < kKeys;
-            bool ok = mbar_wait(q_full, 0) && mbar_wait(full(0), 0);
+            bool ok = warp_wait(q_full, 0) && warp_wait(full(0), 0);
             tc_fence_after_sync();
             for (int t = 0; ok && t < nh; ++t) {
                 issue_s(t, 0);
-                umma_commit(s_full(t));
+                umma_commit_if(me, s_full(t));
             }
             // tiles arrive as K0 V0 K1 V1 ...
             int sv = 1 % NS, sk = 2 % NS, pv = 0, pk = 2 / NS & 1;  // slots of V_i and K_i+1, their phases
             auto arrived = [&](int i) {
-                return mbar_wait(full(sv), pv) && (i + 1 < n ? mbar_wait(full(sk), pk) : !fix || mbar_wait(v_fixed, 0));
+                return warp_wait(full(sv), pv) && (i + 1 < nn ? warp_wait(full(sk), pk) : !fix || warp_wait(v_fixed, 0));
             };
             ok = ok && arrived(0);
-            for (int i = 0; ok && i < n; ++i) {
-                const bool more = i + 1 < n;
+            for (int i = 0; ok && i < nn; ++i) {
+                const bool more = i + 1 < nn;
                 const uint64_t v0 = dv + (uint32_t)sv * kTile16;
                 const int slot_k = sk;
-                for (int t = 0; ok && t < nh; ++t) {
-                    const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * D;
+                for (int t = 0; t < nh; ++t) {
+                    const uint32_t ts = tm + t * 128, to = tm + 256 + t * D;
                     // the first 64 keys' products run while the other probabilities are computed
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (!(ok = mbar_wait(p_full(t, h), i & 1))) break;
+                        if (!(ok = warp_wait(p_full(t, h), i & 1))) break;
                         tc_fence_after_sync();
 #pragma unroll
                         for (int k = 4 * h; k < 4 * h + 4; ++k)
-                            umma_f16_ts(to, ts + 8 * k, v0 + k * 128, id_o, i > 0 || k > 0);
+                            umma_f16_ts_if(me, to, ts + 8 * k, v0 + k * 128, id_o, i > 0 || k > 0);
                     }
                     if (!ok) break;
                     // one commit a tile (the next scores, over P in TMEM: the MMAs of a thread run in order); the
@@ -681,7 +715,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                         if (sk >= NS) sk -= NS, pk ^= 1;
                         if (more) ok = arrived(i + 1);
                     }
-                    umma_commit(more ? s_full(t) : pv_done(t));
+                    umma_commit_if(me, more ? s_full(t) : pv_done(t));
                 }
             }
         }
