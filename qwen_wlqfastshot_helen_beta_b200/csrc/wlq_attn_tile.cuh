@@ -366,6 +366,41 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// 16 e4m3 codes times 2^(e - 127) as 16-bit values, exact where the type has
+// them: in fp16 by one packed product after the conversion (scales outside
+// fp16's normal range and everything in bf16 through fp32).
+template <typename T>
+__device__ __forceinline__ void codes_to_16(uint4 q, uint32_t e, uint32_t (&o)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if (ActTraits<T>::kIsF16 && e >= 113 && e <= 142) {
+        const uint32_t s16 = (e - 112) << 10;  // 2^(e - 127)
+        const uint32_t s2 = s16 | (s16 << 16);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const uint32_t h = e4m3x2_to_f16x2(y & 1 ? w[y >> 1] >> 16 : w[y >> 1]);
+            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&s2));
+            o[y] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        return;
+    }
+    const float sc = exp2_biased(e);
+    const uint64_t sc2 = f2_pack(sc, sc);
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+        const uint32_t h = e4m3x2_to_f16x2(y & 1 ? w[y >> 1] >> 16 : w[y >> 1]);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        float a, b;
+        f2_unpack(f2_mul(f2_pack(f.x, f.y), sc2), a, b);
+        o[y] = pack2<T>(a, b);
+    }
+}
+
 // Byte offset of 16-byte chunk c (of 8 values) of row r in a tile: blocks of
 // 64 columns, the chunk index XORed with row % 8 inside a 128-byte row (the
 // layout TMA writes and tcgen05 reads).
@@ -821,16 +856,8 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                         uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
                         if (r < keys) {
                             const uint4 q = lds128(stage(st) + r * D + ch * 16);
-                            const float sc = exp2_biased(lds8(stage(st) + kKeys * D + r));
-                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
                             uint32_t o[8];
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                float f[4];
-                                e4m3x4_to_f32(w[y], f);
-                                o[2 * y] = pack2<T>(f[0] * sc, f[1] * sc);
-                                o[2 * y + 1] = pack2<T>(f[2] * sc, f[3] * sc);
-                            }
+                            codes_to_16<T>(q, lds8(stage(st) + kKeys * D + r), o);
                             lo = make_uint4(o[0], o[1], o[2], o[3]);
                             hi = make_uint4(o[4], o[5], o[6], o[7]);
                         }
