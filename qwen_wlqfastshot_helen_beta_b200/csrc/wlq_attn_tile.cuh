@@ -32,6 +32,18 @@
 //                     and are written as the 16-bit tiles the MMAs read,
 //                     code * 2^e, which is exact
 //
+// What bounds it: the chain of one half, softmax (2000 cycles: scores read 200,
+// maximum 450, 128 exponentials a thread 1350) then P V and the next S (1024),
+// against 2048 cycles of MMAs for a pair of tiles; a pair takes 3300.  One
+// prompt of 8192 tokens, 28 heads over 4, D 128, bf16: 400 us, 1.2 PFLOP/s of
+// the causal products, 73 % of the measured cuBLAS burst rate (61 % of the
+// tensor pipe's cycles).  4 x 512 new tokens over 16384 cached ones: 367 us
+// from 16-bit pages; from 8-bit ones 461 us, where writing and reading the
+// 16-bit tiles beside the MMAs' operands takes the shared memory's rate.
+// Tried: a polynomial for a part of the exponentials (1.5 % faster for
+// prompts, 4 to 15 % slower over pages); exponentials before the maximum (10 %
+// slower); references that rise by 2^8 (4 % slower than by 2^14).
+//
 // Every mbarrier wait is bounded; a wait that runs out sets the device error
 // word and the CTA winds down, releasing its TMEM.
 #pragma once
@@ -80,7 +92,8 @@ struct TilePlan {
     static constexpr int kRegsSoftmax = SRC == kPaged8 ? 168 : 208, kRegsOther = SRC == kPaged8 ? 48 : 88;
     static_assert(2 * kRegsSoftmax + (kThreads / 128 - 2) * kRegsOther == 65536 / kThreads / 8 * 8 * (kThreads / 128),
                   "register shares");
-    static_assert(kSlots >= 3, "k and v tiles in flight");
+    // the next k and v tiles are waited for while this one's still hold theirs
+    static_assert(kSlots >= 4, "k and v tiles in flight");
 };
 
 // A row tile whose keys several CTAs share: the first part's slot (the next
