@@ -13,9 +13,9 @@ bool few_rows(int64_t max_q, int G) { return max_q * G <= kFewRows; }
 
 size_t attention_workspace_bytes(int Hq, int Hkv, int D, int max_q) {
     const size_t sms = device_sm_count();
-    // two parts per CTA of the step kernel (three CTAs per SM with 8 rows, two with 16), three CTAs' parts per SM of the tile
+    // two parts per CTA of the step kernel (three CTAs per SM with 8 rows, two with 16), four CTAs' parts per SM of the tile
     // kernel
-    const size_t rows = few_rows(max_q, Hq / Hkv) ? 2 * 2 * sms * kFewRows : 3 * sms * 256;
+    const size_t rows = few_rows(max_q, Hq / Hkv) ? 2 * 2 * sms * kFewRows : 4 * sms * 256;
     return WLQ_ATTENTION_ZERO_BYTES + 64 * 1024 /* the tile kernel's list of joins */ + rows * (D + 4) * sizeof(float);
 }
 

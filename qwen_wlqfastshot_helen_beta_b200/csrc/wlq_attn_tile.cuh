@@ -48,6 +48,8 @@
 // word and the CTA winds down, releasing its TMEM.
 #pragma once
 
+#include <algorithm>
+
 #include "wlq_attn_row.cuh"
 #include "wlq_internal.h"
 
@@ -136,8 +138,10 @@ __device__ __forceinline__ Seq seq_of(const AttnParams& p, int nt, int b) {
     return s;
 }
 
-constexpr int kJoinListBytes = 64 * 1024;  // (at least two parts each: at most 3 * 148 / 2 entries)
-constexpr int kPartsPerSm = 3;  // CTAs that hold a part of their rows' keys, at most
+constexpr int kJoinListBytes = 64 * 1024;  // (at least two parts each: at most 4 * 148 / 2 entries)
+constexpr int kFewTiles = 4;    // key tiles of a part, at least
+constexpr int kPartsPerSm = 4;  // CTAs an SM where rows are shared, at most
+constexpr int kLanesSeqs = 32;  // sequences whose split is searched for
 
 // Key tiles of one part (paged form), found by one warp: a sequence with more
 // tiles is shared by several CTAs.  Up to 32 sequences: of 16 sizes the one
@@ -145,13 +149,13 @@ constexpr int kPartsPerSm = 3;  // CTAs that hold a part of their rows' keys, at
 // more for starting and ending, and once 6 for joining the parts).  More
 // sequences: an even share of all tiles.
 __device__ __forceinline__ int tiles_per_part(const AttnParams& p, int nt, int sms, int lane) {
-    if (p.B > 32) {
+    if (p.B > kLanesSeqs) {
         int64_t w = 0;
         for (int b = lane; b < p.B; b += 32) {
             const Seq s = seq_of<true>(p, nt, b);
             w += (int64_t)s.rtiles * s.tiles;
         }
-        return (int)max((int64_t)4, (warp_sum(w) * p.Hkv + sms - 1) / sms);
+        return (int)max((int64_t)kFewTiles, (warp_sum(w) * p.Hkv + sms - 1) / sms);
     }
     Seq s{};
     if (lane < p.B) s = seq_of<true>(p, nt, lane);
@@ -160,11 +164,11 @@ __device__ __forceinline__ int tiles_per_part(const AttnParams& p, int nt, int s
     int best = most, cost = 0x7fffffff;
     for (int parts = 1; parts <= 64; parts += parts < 8 ? 1 : parts / 4) {
         const int per = (most + parts - 1) / parts;
-        if (parts > 1 && per < 4) break;
+        if (parts > 1 && per < kFewTiles) break;
         const int sp = (s.tiles + per - 1) / max(per, 1);
         const int ctas = __reduce_add_sync(0xffffffffu, units * max(sp, 1));
         const int shared = __reduce_add_sync(0xffffffffu, sp > 1 ? units * sp : 0);
-        if (shared > kPartsPerSm * sms) break;
+        if (shared && ctas > kPartsPerSm * sms) break;
         const int c = (ctas + sms - 1) / sms * (per + 3) + (shared ? 6 : 0);
         if (c < cost) {
             cost = c;
@@ -1012,14 +1016,22 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
     static_assert(sizeof(Join) == 24, "the list's entries");
     tp.part = reinterpret_cast<float*>(tp.joins) + kJoinListBytes / 4;
     tp.stat = tp.part + (size_t)kPartsPerSm * tp.sms * kRows * D;
-    const int64_t grid = (a.T / (2 * tp.nt) + a.B) * a.Hkv + (SRC == kPacked ? 0 : kPartsPerSm * tp.sms);
+    // the most CTAs there can be work for; those beyond what there is start, search and end: 1.7 us per 148 of them
+    int64_t grid = (a.T / (2 * tp.nt) + a.B) * a.Hkv;
+    const int64_t tiles = SRC == kPacked ? 0 : ((a.table_cols << a.log2_page) + kKeys - 1) / kKeys;
+    const bool shares = tiles > kFewTiles;
+    if (shares) {
+        // an even share: a row tile that is split has more than an SM's share, and so adds at most that many parts
+        const int64_t most = a.B > kLanesSeqs ? grid + tp.sms : std::max(grid, (int64_t)kPartsPerSm * tp.sms);
+        grid = std::min(grid * ((tiles + kFewTiles - 1) / kFewTiles), most);
+    }
     if (grid > 0x7fffffff) return fail(WLQ_ERR_UNSUPPORTED, "attention: %lld row tiles in one call", (long long)grid);
     static const cudaError_t attr = cudaFuncSetAttribute(attn_tile_kernel<T, D, SRC>,
                                                          cudaFuncAttributeMaxDynamicSharedMemorySize, P::kAlloc);
     if (attr != cudaSuccess) return check_cuda(attr, "attn_tile_kernel shared memory");
     attn_tile_kernel<T, D, SRC><<<(unsigned)grid, P::kThreads, P::kAlloc, stream>>>(tp);
     if ((rc = check_cuda(cudaGetLastError(), "attn_tile_kernel"))) return rc;
-    if constexpr (SRC != kPacked) {
+    if (shares) {
         attn_tile_join_kernel<T, D><<<4 * tp.sms, 32 * kJoinWarps, 0, stream>>>(tp);
         rc = check_cuda(cudaGetLastError(), "attn_tile_join_kernel");
     }

@@ -329,6 +329,33 @@ def test_paged_attention(lens, new, Hq, Hkv, D, page, dtype, bits):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("lens,new,Hq,Hkv,D", [
+    ([700] * 4, [700] * 4, 14, 2, 64),                                # row tiles of several waves, few key tiles
+    ([2100, 900, 1300, 33], [250, 900, 17, 20], 28, 4, 128),          # shared and whole rows together
+    ([30 + 37 * i for i in range(40)], [9 + i % 25 for i in range(40)], 28, 4, 128),  # more sequences than a warp's lanes
+], ids=["waves", "shared", "many"])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_paged_attention_many_row_tiles(lens, new, Hq, Hkv, D, bits):
+    page, g = 64, gen_of("many", D, bits, len(lens))
+    table, pages = R.pages_of(lens, page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, torch.bfloat16, bits)
+    q = randn(g, sum(new), Hq, D).to(torch.bfloat16)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0] + new, device="cuda").cumsum(0).to(torch.int32)
+    out = torch.full_like(q, float("nan"))
+    C().paged_attention(q, kc, vc, table, kv_lens, out, cu, max(new), ke, ve)
+    wide = torch.cat([table, table.new_full((len(lens), 400), -1)], 1)  # a table for longer sequences: the same results
+    again = torch.full_like(q, float("nan"))
+    C().paged_attention(q, kc, vc, wide, kv_lens, again, cu, max(new), ke, ve)
+    assert C().device_error() == 0
+    assert torch.equal(again, out)
+    at = 0
+    for i, (m, n) in enumerate(zip(lens, new)):
+        k, v = R.gather(kc, ke, table, i, m), R.gather(vc, ve, table, i, m)
+        R.check(out[at:at + n], *R.attention(q[at:at + n].double(), k, v, m - n + 1, R.scale_of(D)))
+        at += n
+
+
 @pytest.mark.parametrize("max_q", [4, 60])
 def test_paged_attention_rows_that_see_nothing(max_q):
     """Empty caches, more new tokens than cached ones, sequences without new tokens."""
