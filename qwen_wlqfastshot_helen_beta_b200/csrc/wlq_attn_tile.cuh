@@ -37,8 +37,8 @@
 // against 2048 cycles of MMAs for a pair of tiles; a pair takes 3300.  One
 // prompt of 8192 tokens, 28 heads over 4, D 128, bf16: 400 us, 1.2 PFLOP/s of
 // the causal products, 73 % of the measured cuBLAS burst rate (61 % of the
-// tensor pipe's cycles).  4 x 512 new tokens over 16384 cached ones: 367 us
-// from 16-bit pages; from 8-bit ones 461 us, where writing and reading the
+// tensor pipe's cycles).  4 x 512 new tokens over 16384 cached ones: 342 us
+// from 16-bit pages; from 8-bit ones 424 us, where writing and reading the
 // 16-bit tiles beside the MMAs' operands takes the shared memory's rate.
 // Tried: a polynomial for a part of the exponentials (1.5 % faster for
 // prompts, 4 to 15 % slower over pages); exponentials before the maximum (10 %
@@ -140,7 +140,9 @@ __device__ __forceinline__ Seq seq_of(const AttnParams& p, int nt, int b) {
 
 constexpr int kJoinListBytes = 64 * 1024;  // (at least two parts each: at most 4 * 148 / 2 entries)
 constexpr int kFewTiles = 4;    // key tiles of a part, at least
-constexpr int kPartsPerSm = 4;  // CTAs an SM where rows are shared, at most
+// CTAs an SM where rows are shared, at most (4 x 512 tokens over 1501 .. 16384
+// 8-bit ones: 213 us, 224 with three)
+constexpr int kPartsPerSm = 4;
 constexpr int kLanesSeqs = 32;  // sequences whose split is searched for
 
 // Key tiles of one part (paged form), found by one warp: a sequence with more
@@ -1016,7 +1018,8 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
     static_assert(sizeof(Join) == 24, "the list's entries");
     tp.part = reinterpret_cast<float*>(tp.joins) + kJoinListBytes / 4;
     tp.stat = tp.part + (size_t)kPartsPerSm * tp.sms * kRows * D;
-    // the most CTAs there can be work for; those beyond what there is start, search and end: 1.7 us per 148 of them
+    // the most CTAs there can be work for: those beyond what there is start, search and end, 1.7 us per 148 of them
+    // (3 x 196 tokens over 3071: 12 us, 17.4 with 3 x 148 CTAs more than row tiles)
     int64_t grid = (a.T / (2 * tp.nt) + a.B) * a.Hkv;
     const int64_t tiles = SRC == kPacked ? 0 : ((a.table_cols << a.log2_page) + kKeys - 1) / kKeys;
     const bool shares = tiles > kFewTiles;
