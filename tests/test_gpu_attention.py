@@ -176,6 +176,36 @@ def test_kv_read(lens, bits, page, Hkv, D, dtype):
         assert torch.equal(got.double(), want)  # code * 2^e needs no rounding
 
 
+@pytest.mark.parametrize("bits,D", [(8, 128), (16, 64), (16, 16)])
+@pytest.mark.parametrize("off_out,off_cache", [(8, 0), (0, 8), (8, 8), (24, 40)])
+@pytest.mark.parametrize("T", [5, 1000])
+def test_kv_read_16_byte_aligned(bits, D, off_out, off_cache, T):
+    """Outputs and caches that begin at an odd multiple of 16 bytes."""
+    page, Hkv, dtype = 16, 3, torch.bfloat16
+    g = gen_of("align", bits, D)
+    table, pages = R.pages_of([T], page, g)
+    shifted = []
+    for x in make_cache(g, pages, Hkv, page, D, dtype, bits)[:2]:
+        off = off_cache * 2 // x.element_size()  # `off_cache` in 16-bit values
+        buf = torch.empty(x.numel() + off, device="cuda", dtype=dtype if bits == 16 else torch.uint8)
+        buf = buf if bits == 16 else buf.view(torch.float8_e4m3fn)
+        shifted.append(buf[off:].view_as(x))
+        shifted[-1].view(torch.uint8).copy_(x.view(torch.uint8))
+        assert shifted[-1].data_ptr() % 32 == off_cache * 2 % 32
+    exp = [None, None]
+    if bits == 8:
+        exp = [torch.randint(118, 123, (pages, Hkv, page), generator=g, device="cuda").to(torch.uint8) for _ in range(2)]
+    outs = []
+    for _ in range(2):
+        buf = torch.full((T * Hkv * D + off_out + 8,), 7.0, device="cuda", dtype=dtype)
+        outs.append((buf, buf[off_out:off_out + T * Hkv * D].view(T, Hkv, D)))
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    C().kv_read(*shifted, table, cu, outs[0][1], outs[1][1], *exp)
+    for (buf, got), cache, e in zip(outs, shifted, exp):
+        assert torch.equal(got.double(), R.gather(cache, e, table, 0, T))
+        assert (buf[:off_out] == 7.0).all() and (buf[off_out + T * Hkv * D:] == 7.0).all()
+
+
 def test_kv_read_missing_pages_are_zeros():
     g = gen_of("missing")
     kc, vc, _, _ = make_cache(g, 3, 2, 16, 64, torch.bfloat16, 16)
