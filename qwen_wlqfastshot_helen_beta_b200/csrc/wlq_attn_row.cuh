@@ -3,6 +3,7 @@
 #pragma once
 
 #include "wlq_attn.cuh"
+#include "wlq_once.h"
 #include "wlq_sm100.cuh"
 
 namespace wlq {
@@ -132,6 +133,16 @@ __device__ __noinline__ void row_alone(const AttnParams& p, const RowOf& u, int 
         for (int i = 0; i < E; ++i) o[i] = o[i] * c + e * v[i];
         m = mn;
     }
+}
+
+// Raises a kernel's dynamic shared memory limit on the current device.
+template <typename Kernel>
+int allow_shared_memory(OncePerDevice& limit, Kernel kernel, int bytes, const char* what) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess)
+        e = limit.run(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+    return check_cuda(e, what);
 }
 
 }  // namespace

@@ -914,10 +914,10 @@ int launch_step(const AttnParams& a, cudaStream_t stream) {
     sp.arrived = static_cast<uint32_t*>(a.ws);
     sp.stat = reinterpret_cast<float*>(sp.arrived + kStepCounters);
     sp.part = sp.stat + (size_t)2 * grid * P::kRowsMax * 4;
-    static const cudaError_t attr = cudaFuncSetAttribute(attn_step_kernel<T, D, Q8, NT>,
-                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, P::kAlloc);
-    if (attr != cudaSuccess) return check_cuda(attr, "attn_step_kernel shared memory");
-    attn_step_kernel<T, D, Q8, NT><<<grid, kStepThreads, P::kAlloc, stream>>>(sp);
+    auto kernel = attn_step_kernel<T, D, Q8, NT>;
+    static OncePerDevice limit;
+    if ((rc = allow_shared_memory(limit, kernel, P::kAlloc, "attn_step_kernel shared memory"))) return rc;
+    kernel<<<grid, kStepThreads, P::kAlloc, stream>>>(sp);
     return check_cuda(cudaGetLastError(), "attn_step_kernel");
 }
 

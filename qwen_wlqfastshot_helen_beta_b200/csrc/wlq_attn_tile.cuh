@@ -1030,10 +1030,10 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
         grid = std::min(grid * ((tiles + kFewTiles - 1) / kFewTiles), most);
     }
     if (grid > 0x7fffffff) return fail(WLQ_ERR_UNSUPPORTED, "attention: %lld row tiles in one call", (long long)grid);
-    static const cudaError_t attr = cudaFuncSetAttribute(attn_tile_kernel<T, D, SRC>,
-                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, P::kAlloc);
-    if (attr != cudaSuccess) return check_cuda(attr, "attn_tile_kernel shared memory");
-    attn_tile_kernel<T, D, SRC><<<(unsigned)grid, P::kThreads, P::kAlloc, stream>>>(tp);
+    auto kernel = attn_tile_kernel<T, D, SRC>;
+    static OncePerDevice limit;
+    if ((rc = allow_shared_memory(limit, kernel, P::kAlloc, "attn_tile_kernel shared memory"))) return rc;
+    kernel<<<(unsigned)grid, P::kThreads, P::kAlloc, stream>>>(tp);
     if ((rc = check_cuda(cudaGetLastError(), "attn_tile_kernel"))) return rc;
     if (shares) {
         attn_tile_join_kernel<T, D><<<4 * tp.sms, 32 * kJoinWarps, 0, stream>>>(tp);

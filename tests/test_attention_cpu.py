@@ -108,6 +108,40 @@ def test_cache_tensors():
         PagedKVCache(5, 2, 64, 32, 4)
 
 
+ONCE = r"""
+#include "wlq_once.h"
+#include <cstdio>
+int main() {
+    wlq::OncePerDevice once;
+    int calls[66] = {};
+    auto at = [&](int device, cudaError_t e) { return once.run(device, [&] { ++calls[device]; return e; }); };
+    bool ok = at(0, cudaErrorUnknown) == cudaErrorUnknown;       // a failure is not kept ...
+    ok = ok && at(0, cudaSuccess) == cudaSuccess && calls[0] == 2;  // ... and tried again
+    ok = ok && at(0, cudaErrorUnknown) == cudaSuccess && calls[0] == 2;
+    ok = ok && at(1, cudaSuccess) == cudaSuccess && calls[1] == 1;  // another device has a setting of its own
+    ok = ok && at(63, cudaSuccess) == cudaSuccess && at(63, cudaSuccess) == cudaSuccess && calls[63] == 1;
+    ok = ok && at(64, cudaSuccess) == cudaSuccess && at(64, cudaSuccess) == cudaSuccess && calls[64] == 2;  // not remembered
+    puts(ok ? "ok" : "wrong");
+}
+"""
+
+
+def test_settings_are_made_on_every_device(tmp_path):
+    import glob
+    import os
+    import re
+    import subprocess
+    from qwen_wlqfastshot_helen_beta_b200.build import CSRC, CUDA_HOME
+    (tmp_path / "once.cpp").write_text(ONCE)
+    exe = str(tmp_path / "once")
+    subprocess.run(["g++", "-std=c++17", "-I", CSRC, "-I", os.path.join(CUDA_HOME, "include"), str(tmp_path / "once.cpp"),
+                    "-o", exe], check=True)
+    assert subprocess.run([exe], capture_output=True, text=True, check=True).stdout == "ok\n"
+    # no kernel's attribute is kept for the whole process
+    for path in glob.glob(os.path.join(CSRC, "*.cu*")):
+        assert not re.search(r"static\s+(const\s+)?cudaError_t", open(path).read()), path
+
+
 def test_header_constants():
     import os
     import re
