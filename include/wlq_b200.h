@@ -336,7 +336,7 @@ WLQ_API int wlq_prompt_attention(const void* q, const void* k, const void* v, co
  * bound of n.  `workspace` (device memory of
  * wlq_paged_attention_workspace_bytes on the current device, 16-byte aligned,
  * its first WLQ_ATTENTION_ZERO_BYTES zero before the first use and left zero
- * by every call) joins the parts of sequences that several CTAs share; calls
+ * by every call, one that gave up a wait included) joins the parts of sequences that several CTAs share; calls
  * that share one must not overlap.  B * Hkv is at most
  * WLQ_ATTENTION_ZERO_BYTES / 4.  Results do not depend on timing. */
 #define WLQ_ATTENTION_ZERO_BYTES (256u * 1024u)

@@ -421,10 +421,14 @@ def init_workspaces(max_N, max_K, device):
 def device_error(device=None, clear: bool = True) -> int:
     """Device error word (bit 0: a bounded pipeline wait in a GEMM or
     attention kernel gave up, so that call's output is undefined; bit 1:
-    rope_kv_write met a position outside its table).  Synchronous."""
+    rope_kv_write met a position outside its table).  Synchronous.  Clearing
+    it also drops the workspaces that paged_attention keeps, so that nothing
+    of a call that gave up is left in them."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     flags = ctypes.c_uint(0)
     check(lib.wlq_device_error(dev.index or 0, ctypes.byref(flags), 1 if clear else 0), "wlq_device_error")
+    if clear:
+        _calls.drop_workspaces()
     return int(flags.value)
 
 

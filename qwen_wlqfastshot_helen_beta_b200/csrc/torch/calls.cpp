@@ -252,9 +252,10 @@ PyObject* prompt_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
 // process.  While a CUDA graph is captured the graph gets one of its own, from
 // its memory pool: a replay may overlap later calls on the stream that
 // captured it.
+auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>;  // never destroyed: CUDA may be gone by then
+std::mutex lock;
+
 at::Tensor workspace(at::Device dev, c10::cuda::CUDAStream stream, size_t bytes) {
-    static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>;  // never destroyed: CUDA may be gone by then
-    static std::mutex lock;
     auto make = [&] {
         at::Tensor t = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
         t.narrow(0, 0, WLQ_ATTENTION_ZERO_BYTES).zero_();
@@ -294,6 +295,27 @@ PyObject* paged_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     });
 }
 
+// The kept workspaces, and their end: the next calls begin with fresh ones.
+// (Memory goes back to its stream's pool, behind the calls that still use it.)
+PyObject* kept_workspaces(PyObject*, PyObject*) {
+    const std::lock_guard<std::mutex> hold(lock);
+    PyObject* list = PyList_New(0);
+    for (const auto& entry : *kept) {
+        PyObject* t = list ? THPVariable_Wrap(entry.second) : nullptr;
+        if (!t || PyList_Append(list, t) < 0) Py_CLEAR(list);
+        Py_XDECREF(t);
+    }
+    return list;
+}
+PyObject* drop_workspaces(PyObject*, PyObject*) {
+    std::map<std::pair<int, cudaStream_t>, at::Tensor> gone;
+    {
+        const std::lock_guard<std::mutex> hold(lock);
+        gone.swap(*kept);
+    }
+    Py_RETURN_NONE;
+}
+
 // setup((addresses in the order of Entries), WLQError)
 PyObject* setup(PyObject*, PyObject* args) {
     PyObject* addresses;
@@ -325,6 +347,8 @@ PyMethodDef methods[] = {{"rope_kv_write", fast(rope_kv_write), METH_FASTCALL, n
                          {"kv_read", fast(kv_read), METH_FASTCALL, nullptr},
                          {"prompt_attention", fast(prompt_attention), METH_FASTCALL, nullptr},
                          {"paged_attention", fast(paged_attention), METH_FASTCALL, nullptr},
+                         {"kept_workspaces", kept_workspaces, METH_NOARGS, nullptr},
+                         {"drop_workspaces", drop_workspaces, METH_NOARGS, nullptr},
                          {"setup", setup, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Attention operator calls over the C ABI", -1, methods,

@@ -495,6 +495,22 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
     const int gq = lane >> 2, tq = lane & 3;
     int g = 0;
     bool ok = true;
+    // the parts of the segment's (sequence, kv head), the first of them CTA c0's
+    auto parts_around = [&](int& c0) {
+        c0 = (int)blockIdx.x - w.part;
+        if (w.parts) return w.parts;
+        int hi;
+        cuts.inside(w.base, w.s.tiles, c0, hi);
+        --c0;
+        return hi - c0 + 1;
+    };
+    // counts this CTA's part as delivered (one thread); whether it is the last
+    auto deliver = [&](int parts) {
+        uint32_t* n = sp.arrived + w.b * p.Hkv + w.hk;
+        const bool last = add_acq_rel(n, 1u) == (uint32_t)(parts - 1);
+        if (last) *n = 0u;  // every part is here: nobody else looks at it in this call
+        return last;
+    };
     while (ok && w.next(p, RM)) {
         const StepSeq s = w.s;
         const int past = s.len - s.n;
@@ -866,23 +882,21 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
         }
         // its parts: the one a CTA ends its share with (slot 1), then those that begin with a cut (slot 0)
         if (!whole) {
-            int c0 = (int)blockIdx.x - w.part, parts = w.parts;
-            if (!parts) {
-                int hi;
-                cuts.inside(w.base, s.tiles, c0, hi);
-                --c0;
-                parts = hi - c0 + 1;
-            }
+            int c0;
+            const int parts = parts_around(c0);
             bar_sync_step();
-            if (threadIdx.x == 0) {
-                uint32_t* n = sp.arrived + w.b * p.Hkv + w.hk;
-                const bool last = add_acq_rel(n, 1u) == (uint32_t)(parts - 1);
-                if (last) *n = 0u;  // every part is here: nobody else looks at it in this call
-                last_part = last;
-            }
+            if (threadIdx.x == 0) last_part = deliver(parts);
             bar_sync_step();
             if (last_part) join_parts<T, D, NT>(sp, s.rows, w.hk, s.first, c0, parts, warp, lane);
         }
+    }
+    // A CTA that gave up still counts its parts: the counters are zero again after the call, whose output is undefined
+    // (the device error word says so), and the next call finds them as it must.
+    if (!ok && threadIdx.x == 0) {
+        do {
+            int c0;
+            if (w.t0 != 0 || w.t1 != w.s.tiles) deliver(parts_around(c0));
+        } while (w.next(p, RM));
     }
 }
 

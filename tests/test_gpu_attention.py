@@ -543,6 +543,30 @@ def test_paged_attention_streams_and_graph():
         R.check(out[i:i + 1], *R.attention(q[i:i + 1].double(), k, v, n, R.scale_of(D)))
 
 
+def test_paged_attention_recovers_from_a_workspace_left_dirty():
+    """A call that gave up may leave the kept workspace's counters as they should not be: reading and clearing the
+    device error word ends that."""
+    from qwen_wlqfastshot_helen_beta_b200 import _calls
+    g = gen_of("dirty")
+    Hq, Hkv, D, page, lens = 28, 4, 128, 16, [3000, 800, 2]
+    table, pages = R.pages_of(lens, page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, torch.bfloat16, 8)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = randn(g, 3, Hq, D).bfloat16()
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    C().paged_attention(q, kc, vc, table, kv_lens, want, None, 1, ke, ve)
+    kept = _calls.kept_workspaces()
+    assert kept and all(w.is_cuda and not w[:256 * 1024].any() for w in kept)  # calls leave the counters zero
+    for w in kept:
+        w[:256 * 1024].view(torch.int32).fill_(1)
+    assert C().device_error() == 0 and not _calls.kept_workspaces()
+    for _ in range(2):
+        out.fill_(float("nan"))
+        C().paged_attention(q, kc, vc, table, kv_lens, out, None, 1, ke, ve)
+        assert torch.equal(out, want)
+    assert not any(w[:256 * 1024].any() for w in _calls.kept_workspaces())
+
+
 # ------------------------------------------------------- refusals, the block ---
 
 def test_refusals_on_the_gpu():
