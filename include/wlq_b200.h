@@ -299,7 +299,8 @@ WLQ_API int wlq_gemv_get_overlap(void);
  * of 16, D <= 256.  slots[t] = page * page_size + offset; a slot outside the
  * pool (negative: a padding token) is not written.  8-bit rows are quantised
  * from the fp32 rotated values with e the smallest integer for which
- * max|x| <= 448 * 2^e (in fp16 values beyond +-61440 are stored as that).
+ * max|x| <= 448 * 2^e (in fp16 values beyond +-61440 are stored as that); a
+ * NaN is stored as the NaN code and has no say in its row's scale.
  * q_out may be q; k_out (the rotated k, for wlq_prompt_attention) may be
  * NULL.  A position outside the table sets WLQ_DEVERR_POSITION and leaves
  * the token's outputs and slot as they were. */

@@ -190,10 +190,12 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas) rope_kv_write_kernel(
                 if constexpr (QUANT) {
                     if (ActTraits<T>::kIsF16) {
                         // the largest e4m3 grid value below 65504, so that what is read back stays finite in fp16
+                        // (a NaN passes, and becomes the NaN code)
+                        auto within = [](float x) { return fabsf(x) > 61440.f ? copysignf(61440.f, x) : x; };
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            a[i] = fminf(fmaxf(a[i], -61440.f), 61440.f);
-                            b[i] = fminf(fmaxf(b[i], -61440.f), 61440.f);
+                            a[i] = within(a[i]);
+                            b[i] = within(b[i]);
                         }
                     }
                     float top = 0.f;

@@ -146,6 +146,44 @@ def test_rope_fp16_largest_values_stay_finite():
     assert (ko == 61440).all() and (vo == -61440).all()
 
 
+@pytest.mark.parametrize("dtype", BOTH, ids=str)
+@pytest.mark.parametrize("bits", [16, 8])
+def test_rope_nan_and_infinity_stay_what_they_are(dtype, bits):
+    """A NaN in k or v comes back as NaN and changes nothing else of its row; an infinity stays one (an 8-bit cache of
+    fp16 values holds up to 61440)."""
+    g = gen_of("nan", bits)
+    T, Hkv, D, page = 6, 2, 64, 16
+    q, k, v = (randn(g, T, Hkv, D).to(dtype) for _ in range(3))
+    k[1, 0, 5] = k[1, 0, 37] = v[2, 1, 9] = 0  # (5, 37) turn together
+    pos = torch.arange(T, device="cuda")
+    cs, cu = table_of(T, D), torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    tab = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+
+    def through():
+        kc, vc = (torch.zeros(1, Hkv, page, D, device="cuda").to(dtype if bits == 16 else torch.float8_e4m3fn)
+                  for _ in range(2))
+        ke, ve = ((torch.zeros(1, Hkv, page, dtype=torch.uint8, device="cuda") for _ in range(2)) if bits == 8
+                  else (None, None))
+        C().rope_kv_write(q, k, v, pos, cs, pos, kc, vc, torch.empty_like(q), None, ke, ve)
+        ko, vo = torch.empty_like(k), torch.empty_like(v)
+        C().kv_read(kc, vc, tab, cu, ko, vo, ke, ve)
+        return ko, vo
+
+    clean = through()
+    k[1, 0, 5] = v[2, 1, 9] = float("nan")
+    v[3, 0] = float("nan")
+    got = through()
+    where = [torch.zeros(T, Hkv, D, dtype=torch.bool, device="cuda") for _ in range(2)]
+    where[0][1, 0, [5, 37]] = True
+    where[1][2, 1, 9], where[1][3, 0] = True, True
+    for x, c, w in zip(got, clean, where):
+        assert torch.equal(torch.isnan(x.float()), w) and torch.equal(x[~w], c[~w])
+    v[4, 0, 3], v[4, 1, 3] = float("inf"), float("-inf")
+    most = 61440.0 if bits == 8 and dtype == torch.float16 else float("inf")
+    _, vo = through()
+    assert vo[4, 0, 3] == most and vo[4, 1, 3] == -most
+
+
 # -------------------------------------------------------------------- read ---
 
 def make_cache(g, pages, Hkv, page, D, dtype, bits, spread=True):
