@@ -97,10 +97,64 @@ __device__ __forceinline__ void load_row(const AttnParams& p, const RowOf& u, in
     }
 }
 
+// The last of the keys [j0, j1) whose v, as the 16-bit values the tensor cores
+// take, is not finite throughout; -1 if there is none.  By one warp, a key a lane.
+template <typename T, int D, int SRC>
+__device__ __noinline__ int last_not_finite(const AttnParams& p, const RowOf& u, int j0, int j1, int lane) {
+    for (int hi = j1; hi > j0; hi -= 32) {
+        const int j = hi - 1 - lane;
+        bool bad = false;
+        if (j >= j0) {
+            int64_t row = 0;
+            bool there = true;
+            if constexpr (SRC != kPacked) {
+                const int page = p.table[(int64_t)u.b * p.table_cols + (j >> p.log2_page)];
+                there = page >= 0 && page < p.num_pages;  // a page outside the pool reads as zeros
+                if (there) row = ((int64_t)page * p.Hkv + u.hk) * p.page_size + (j & (p.page_size - 1));
+            }
+            if constexpr (SRC == kPaged8) {
+                const uint8_t* s = static_cast<const uint8_t*>(p.v_cache) + row * D;
+                uint32_t top = 0;  // the largest code without its sign, a byte each
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint4 w = ldg16(s + 16 * i);
+                    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) top = __vmaxu4(top, x[y] & 0x7f7f7f7fu);
+                }
+                top = max(max(top & 0xff, (top >> 8) & 0xff), max((top >> 16) & 0xff, top >> 24));
+                const uint32_t e = p.v_exp[row];
+                float f[4];
+                e4m3x4_to_f32(top, f);
+                const uint32_t v = pack2<T>(f[0] * exp2_biased(e), 0.f);
+                bad = e == 255 || !isfinite(ActTraits<T>::bits_to_f32((uint16_t)v));
+            } else {
+                const uint16_t* s = SRC == kPacked ? p.v + (int64_t)(u.first + j) * p.v_tok + u.hk * p.v_head
+                                                   : static_cast<const uint16_t*>(p.v_cache) + row * D;
+                uint32_t top = 0;  // the largest value without its sign, two bytes each
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint4 w = ldg16(s + 8 * i);
+                    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) top = __vmaxu2(top, x[y] & 0x7fff7fffu);
+                }
+                bad = max(top & 0xffffu, top >> 16) >= (ActTraits<T>::kIsF16 ? 0x7c00u : 0x7f80u);
+            }
+            bad = bad && there;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, bad);
+        if (hit) return hi - __ffs(hit);
+    }
+    return -1;
+}
+
 // One row over its keys [j0, j1) without the tensor cores, by one warp.  A
 // tensor-core product multiplies the values of keys a row does not see by
 // zero; where those are infinite or NaN the product is NaN, and the row is
-// computed here instead.  m is in powers of two.
+// computed here instead.  m is in powers of two.  It takes about 0.5 us a key,
+// so the callers look for such a value first: a NaN that the rows do see is
+// no reason (a prompt of 4096 tokens with one took 58 ms, 0.12 without).
 template <typename T, int D, int SRC>
 __device__ __noinline__ void row_alone(const AttnParams& p, const RowOf& u, int row, int j0, int j1, int lane,
                                        float (&o)[D / 32], float& m, float& l) {
@@ -132,6 +186,11 @@ __device__ __noinline__ void row_alone(const AttnParams& p, const RowOf& u, int 
 #pragma unroll
         for (int i = 0; i < E; ++i) o[i] = o[i] * c + e * v[i];
         m = mn;
+        // NaN everywhere: whatever follows, the row stays so
+        bool nan = true;
+#pragma unroll
+        for (int i = 0; i < E; ++i) nan = nan && o[i] != o[i];
+        if (__all_sync(0xffffffffu, nan)) return;
     }
 }
 

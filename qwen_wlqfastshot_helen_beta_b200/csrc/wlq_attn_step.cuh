@@ -861,12 +861,13 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
             for (int y = 0; y < 2; ++y) {
                 const int r = rb + 4 * y;
                 if (r >= s.rows) break;
-                // with several new tokens, keys a row does not see may have spoilt it
-                if (s.n > 1 && ((__float_as_uint(x[y].w) >> r) & 1)) {
-                    const int seen = min(s.len, past + r / p.G + 1);
-                    if (seen < w.t1 * kStepKeys) {
-                        row_alone<T, D, Q8 ? kPaged8 : kPaged>(p, RowOf{w.b, w.hk, s.first}, r, w.t0 * kStepKeys, seen, lane,
-                                                               a[y], x[y].x, x[y].z);
+                // with several new tokens, keys a row does not see may have spoilt it (a sum that is NaN is so by what it sees)
+                if (s.n > 1 && ((__float_as_uint(x[y].w) >> r) & 1) && x[y].z == x[y].z) {
+                    constexpr int kSource = Q8 ? kPaged8 : kPaged;
+                    const int seen = max(0, min(s.len, past + r / p.G + 1)), j0 = w.t0 * kStepKeys;
+                    const RowOf u{w.b, w.hk, s.first};
+                    if (last_not_finite<T, D, kSource>(p, u, max(seen, j0), min(s.len, w.t1 * kStepKeys), lane) >= 0) {
+                        row_alone<T, D, kSource>(p, u, r, j0, seen, lane, a[y], x[y].x, x[y].z);
                         x[y].y = x[y].x;
                     }
                 }

@@ -647,9 +647,14 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
             }
             if (pdst)
                 *reinterpret_cast<float2*>(tp.stat + ((int64_t)u.slot * kRows + t * kRowsT + r) * 2) = make_float2(m * c, l);
-            // rows that values behind the mask may have spoilt
-            const bool masked = key0 + n * kKeys - 1 > lim;
-            unsigned again = __ballot_sync(0xffffffffu, ok && mine && masked && bad != bad);
+            // rows that values behind the mask have spoilt (a sum that is NaN is so by what the row sees)
+            const int end = key0 + n * kKeys;
+            unsigned again = __ballot_sync(0xffffffffu, ok && mine && end - 1 > lim && bad != bad && l == l);
+            if (again) {
+                const int j0 = __reduce_min_sync(0xffffffffu, (again >> lane) & 1 ? lim + 1 : end);
+                const int last = last_not_finite<T, D, SRC>(p, RowOf{u.b, u.hk, u.first}, max(j0, key0), min(u.len, end), lane);
+                again &= __ballot_sync(0xffffffffu, lim < last);
+            }
             if (!pdst) {
                 fence_proxy_async_smem();
                 const bool plain = bar_or_half(t, again != 0 || !ok) || u.tok0 + (t + 1) * tp.nt > u.n;
@@ -688,7 +693,7 @@ __global__ void __launch_bounds__(TilePlan<D, SRC>::kThreads, 1) attn_tile_kerne
                 const int rx = (r & ~31) + x, tx = __shfl_sync(0xffffffffu, tok, x), hx = rx % p.G;
                 const int j1 = __shfl_sync(0xffffffffu, lim, x) + 1;
                 float o[D / 32], mx, lx;
-                row_alone<T, D, SRC>(p, RowOf{u.b, u.hk, u.first}, tx * p.G + hx, key0, min(j1, key0 + n * kKeys), lane, o, mx, lx);
+                row_alone<T, D, SRC>(p, RowOf{u.b, u.hk, u.first}, tx * p.G + hx, key0, min(j1, end), lane, o, mx, lx);
                 if (u.slot < 0) {
                     const float ix = lx > 0.f ? 1.f / lx : (lx == lx ? 0.f : lx);
                     uint16_t* d = p.out + (int64_t)(u.first + tx) * p.o_tok + (u.hk * p.G + hx) * p.o_head + lane * (D / 32);

@@ -523,6 +523,85 @@ def test_paged_attention_later_tokens_do_not_leak(new, bits):
     assert torch.isnan(out[-1].float()).all()
 
 
+@pytest.mark.parametrize("new", [2, 50])
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("D", [64, 128])
+def test_paged_attention_later_tokens_do_not_leak_over_parts(new, bits, D):
+    """As above where several CTAs share the keys: the spoilt rows are parts."""
+    g = gen_of("pparts", new, bits, D)
+    Hq, Hkv, page, n = 6, 2, 16, 6000
+    table, pages = R.pages_of([n], page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, torch.bfloat16, bits)
+    q = randn(g, new, Hq, D).bfloat16()
+    cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    late = table[0, (n - 1) // page].long()
+    for c in (kc, vc):  # the last token
+        row = c[late, :, (n - 1) % page]
+        row.view(torch.uint8).fill_(0x7f) if bits == 8 else row.fill_(float("nan"))
+    out = torch.empty_like(q)
+    C().paged_attention(q, kc, vc, table, lens, out, cu, new, ke, ve)
+    R.check(out[:-1], *R.attention(q[:-1].double(), R.gather(kc, ke, table, 0, n - 1),
+                                   R.gather(vc, ve, table, 0, n - 1), n - new + 1, R.scale_of(D)))
+    assert torch.isnan(out[-1].float()).all()
+    # only v is spoilt, in one value: the last row has it in one column, the others not at all
+    kc[late, :, (n - 1) % page] = kc[late, :, (n - 2) % page]
+    vc[late, :, (n - 1) % page] = vc[late, :, (n - 2) % page]
+    row = vc[late, :, (n - 1) % page]
+    (row.view(torch.uint8)[:, 7] if bits == 8 else row[:, 7]).fill_(0x7f if bits == 8 else float("nan"))
+    C().paged_attention(q, kc, vc, table, lens, out, cu, new, ke, ve)
+    R.check(out[:-1], *R.attention(q[:-1].double(), R.gather(kc, ke, table, 0, n - 1),
+                                   R.gather(vc, ve, table, 0, n - 1), n - new + 1, R.scale_of(D)))
+    assert torch.isnan(out[-1, :, 7].float()).all() and torch.isfinite(out[-1, :, :7]).all()
+
+
+def seconds(call):
+    call()
+    times = []
+    for _ in range(3):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        call()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e-3)
+    return min(times)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")], ids=str)
+def test_a_value_that_rows_see_costs_them_nothing(bad):
+    """A NaN or infinity in an early token's v reaches the rows that see it, and no row is computed anew for it (a row
+    alone takes half a microsecond a key: 100 ms for this prompt, where 2 are asked for)."""
+    g = gen_of("early", bad)
+    n, Hq, Hkv, D = 4096, 28, 4, 128
+    q, k, v = (randn(g, n, h, D).bfloat16() for h in (Hq, Hkv, Hkv))
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    C().prompt_attention(q, k, v, cu, clean)
+    v[5, :, 3] = bad
+    assert seconds(lambda: C().prompt_attention(q, k, v, cu, out)) < 2e-3
+    first = R.attention(q[:5].double(), k[:5].double(), v[:5].double(), 1, R.scale_of(D))
+    R.check(out[:5], *first)  # (the rows before it share a tile with it: they are the ones computed anew)
+    assert not torch.isfinite(out[5:, :, 3]).any()
+    assert torch.equal(out[5:, :, :3], clean[5:, :, :3]) and torch.equal(out[5:, :, 4:], clean[5:, :, 4:])
+    v[5:] = float("nan")
+    assert seconds(lambda: C().prompt_attention(q, k, v, cu, out)) < 2e-3
+    assert torch.isnan(out[5:].float()).all()
+    R.check(out[:5], *first)
+    # three new tokens over a cache with such a value: the same in the kernel of few rows, and in that of many
+    page, m, Hq, Hkv = 16, 60000, 4, 1
+    table, pages = R.pages_of([m], page, g)
+    kc, vc, _, _ = make_cache(g, pages, Hkv, page, D, torch.bfloat16, 16)
+    vc[table[0, 0].long(), :, 1, 9] = bad
+    lens = torch.tensor([m], dtype=torch.int32, device="cuda")
+    for new in (3, 40):
+        q = randn(g, new, Hq, D).bfloat16()
+        out, cu = torch.empty_like(q), torch.tensor([0, new], dtype=torch.int32, device="cuda")
+        assert seconds(lambda: C().paged_attention(q, kc, vc, table, lens, out, cu, new)) < 2e-3
+        assert not torch.isfinite(out[..., 9]).any() and torch.isfinite(out[..., :9]).all()
+    assert C().device_error() == 0
+
+
 def test_paged_attention_past_32_bits():
     """A pool whose values pass 2^32: the last pages are read where they are."""
     g = gen_of("wide")
