@@ -96,6 +96,48 @@ def test_rope_table():
         rope_frequencies(64, 1e4, {"type": "other", "factor": 2.0})
 
 
+def test_rope_dynamic_scaling_goes_by_the_length():
+    """Dynamic NTK: base (f L / n - (f - 1)) ** (d / (d - 2)) beyond the n trained positions, the base as it is up to there."""
+    from qwen_wlqfastshot_helen_beta_b200.attention import rope_frequencies, rope_table
+    s = {"type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 4096}
+    plain = rope_frequencies(64, 1e4)[0]
+    for length in (None, 1, 4095, 4096):
+        assert torch.equal(rope_frequencies(64, 1e4, s, length)[0], plain)
+    for length, stretch in ((6144, 2.0), (8192, 3.0), (32768, 15.0)):
+        got = rope_frequencies(64, 1e4, s, length)[0]
+        assert got[0] == 1.0
+        for i in (1, 7, 31):
+            want = (1e4 * stretch ** (64 / 62)) ** (-2 * i / 64)
+            assert abs(got[i].item() / want - 1) < 1e-12
+    assert torch.equal(rope_table(4096, 64, 1e4, s, "cpu"), rope_table(4096, 64, 1e4, device="cpu"))
+    long = rope_table(8192, 64, 1e4, s, "cpu")
+    a = 8191 * (1e4 * 3.0 ** (64 / 62)) ** (-62 / 64)
+    assert abs(long[8191, 31].item() - math.cos(a)) < 1e-7 and abs(long[8191, 63].item() - math.sin(a)) < 1e-7
+    assert torch.equal(rope_table(4096, 64, 1e4, s, "cpu", length=8192), long[:4096])
+    assert torch.equal(rope_table(8192, 64, 1e4, s, "cpu", length=4096), rope_table(8192, 64, 1e4, device="cpu"))
+    bare = {"type": "dynamic", "factor": 2.0}
+    with pytest.raises(ValueError, match="original_max_position_embeddings"):
+        rope_table(8192, 64, 1e4, bare, "cpu")
+    with pytest.warns(UserWarning, match="ntk"):
+        fixed = rope_frequencies(64, 1e4, bare)[0]
+    assert torch.equal(fixed, rope_frequencies(64, 1e4, {"type": "ntk", "factor": 2.0}, 100)[0])
+
+
+def test_rope_scaling_as_config_files_write_it():
+    """Keys with null count as absent, keys that would change the angles and are not known are refused."""
+    from qwen_wlqfastshot_helen_beta_b200.attention import rope_frequencies
+    s = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
+    f, a = rope_frequencies(128, 1e6, s)
+    g, b = rope_frequencies(128, 1e6, dict(s, attention_factor=None, beta_fast=None, beta_slow=None, mscale=None))
+    assert torch.equal(f, g) and a == b
+    assert rope_frequencies(128, 1e6, dict(s, attention_factor=1.5, mscale=1.0))[1] == 1.5
+    for bad, word in ((dict(s, mscale=1.0, mscale_all_dim=1.0), "mscale"), (dict(s, truncate=False), "truncate"),
+                      ({"type": "yarn", "factor": 4.0}, "original_max"), ({"type": "linear"}, "factor"),
+                      ({"type": "linear", "factor": None}, "factor")):
+        with pytest.raises(ValueError, match=word):
+            rope_frequencies(128, 1e6, bad)
+
+
 def test_cache_tensors():
     from qwen_wlqfastshot_helen_beta_b200.attention import PagedKVCache
     c = PagedKVCache(5, 2, 64, 32, 8, torch.float16, "cpu")
