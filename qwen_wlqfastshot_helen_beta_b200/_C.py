@@ -19,14 +19,34 @@ from typing import Optional, Tuple
 import numpy as np
 import torch
 
-from . import _calls
 from ._lib import (WLQ_DTYPE_BF16, WLQ_DTYPE_F16, WLQ_LUT_F16, WLQ_LUT_PREPACKED, WLQError, check, lib)
 
 _NONE = None
 
-_calls.setup(tuple(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-    "wlq_rope_kv_write", "wlq_kv_read", "wlq_prompt_attention", "wlq_paged_attention_workspace_bytes",
-    "wlq_paged_attention", "wlq_last_error")), WLQError)
+
+class _NoCalls:
+    """Stands for the extension module where it is missing or was built for
+    another torch or Python: the linears do without it, attention says why."""
+
+    def __init__(self, why):
+        self._why = why
+
+    def drop_workspaces(self):
+        pass
+
+    def __getattr__(self, name):
+        raise RuntimeError(f"wlq: {name}: the extension module _calls did not load ({self._why}); "
+                           "run qwen_wlqfastshot_helen_beta_b200/build.py with this torch and Python")
+
+
+try:
+    from . import _calls
+except ImportError as _e:
+    _calls = _NoCalls(_e)
+else:
+    _calls.setup(tuple(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+        "wlq_rope_kv_write", "wlq_kv_read", "wlq_prompt_attention", "wlq_paged_attention_workspace_bytes",
+        "wlq_paged_attention", "wlq_last_error")), WLQError)
 
 
 def _ptr(t: Optional[torch.Tensor]):

@@ -96,7 +96,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         calls = ex.submit(_build_calls)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
-        calls.result()
     if force or _stale(LIB, objs):
         # export the C ABI only (sources are compiled with hidden visibility;
         # the extern "C" entry points are marked visible in wlq_b200.h's users
@@ -109,6 +108,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    calls.result()  # raises what went wrong with _calls; the library, which the linears need alone, is there
     return LIB
 
 

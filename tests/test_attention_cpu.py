@@ -75,6 +75,49 @@ def test_python_refuses_cpu_tensors_and_wrong_arguments():
         _calls.setup((1, 2), RuntimeError)
 
 
+def test_linears_do_without_the_extension_module():
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.modules["qwen_wlqfastshot_helen_beta_b200._calls"] = None  # as if it were not there
+import numpy as np, torch
+import qwen_wlqfastshot_helen_beta_b200 as pkg
+from qwen_wlqfastshot_helen_beta_b200 import _C
+assert hasattr(torch.ops.wlq_fastShot, "gemv") and _C.lib.wlq_abi_version() == 1
+x = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+try:
+    _C.prompt_attention(x, x, x, x, x)
+except RuntimeError as e:
+    assert "wlq: prompt_attention" in str(e) and "_calls" in str(e) and "build.py" in str(e), e
+    print("ok")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stderr
+
+
+def test_the_library_is_linked_where_the_extension_module_does_not_compile(tmp_path, monkeypatch):
+    import os
+    import subprocess
+    from qwen_wlqfastshot_helen_beta_b200 import build
+    (tmp_path / "a.c").write_text("int wlq_a(void) { return 1; }")
+    subprocess.run(["gcc", "-fPIC", "-c", str(tmp_path / "a.c"), "-o", str(tmp_path / "a.o")], check=True)
+
+    def no_calls():
+        raise RuntimeError("compile failed: no torch headers")
+
+    monkeypatch.setattr(build, "_build_calls", no_calls)
+    monkeypatch.setattr(build, "_compile", lambda src, verbose: str(tmp_path / "a.o"))
+    monkeypatch.setattr(build.glob, "glob", lambda pattern: [str(tmp_path / "a.c")] if pattern.endswith(".cpp") else [])
+    monkeypatch.setattr(build, "OBJ", str(tmp_path))
+    monkeypatch.setattr(build, "LIB", str(tmp_path / "lib.so"))
+    with pytest.raises(RuntimeError, match="no torch headers"):
+        build.build()
+    assert os.path.exists(build.LIB)
+
+
 def test_rope_table():
     from qwen_wlqfastshot_helen_beta_b200.attention import rope_frequencies, rope_table
     t = rope_table(1000, 64, 1e4, device="cpu")
