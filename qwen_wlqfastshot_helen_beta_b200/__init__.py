@@ -175,16 +175,17 @@ def _register_attention_ops():
         op.register_fake(_fake)
 
 
-def _ops_registered() -> bool:
+def _registered(name: str) -> bool:
     try:
-        return torch._C._dispatch_has_kernel_for_dispatch_key("wlq_fastShot::gemv", "CompositeExplicitAutograd") or \
-            hasattr(torch.ops.wlq_fastShot, "gemv")
+        return torch._C._dispatch_has_kernel_for_dispatch_key(f"wlq_fastShot::{name}", "CompositeExplicitAutograd") or \
+            hasattr(torch.ops.wlq_fastShot, name)
     except (AttributeError, RuntimeError):
         return False
 
 
-if not _ops_registered():
+if not _registered("gemv"):
     _register_ops()
+if not _registered("rope_kv_write"):
     _register_attention_ops()
 
 

@@ -98,6 +98,27 @@ except RuntimeError as e:
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stderr
 
 
+def test_attention_ops_beside_somebody_elses_linears():
+    """Another plugin's wlq_fastShot::gemv leaves the attention ops where they are; a second import changes nothing."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+lib = torch.library.Library("wlq_fastShot", "FRAGMENT")
+lib.define("gemv(Tensor x) -> Tensor")
+import qwen_wlqfastshot_helen_beta_b200 as pkg
+for name in ("rope_kv_write", "kv_read", "prompt_attention", "paged_attention"):
+    assert hasattr(torch.ops.wlq_fastShot, name), name
+import importlib
+importlib.reload(pkg)
+print("ok")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stderr
+
+
 def test_the_library_is_linked_where_the_extension_module_does_not_compile(tmp_path, monkeypatch):
     import os
     import subprocess
