@@ -181,6 +181,7 @@ int wlq_paged_attention(const void* q, const void* k_cache, const void* v_cache,
     if ((rc = bad_cache(fn, k_cache, v_cache, k_exp, v_exp, num_pages, page_size))) return rc;
     if (T == 0) return WLQ_OK;
     if (!block_table || !kv_lens) return fail(WLQ_ERR_INVALID_ARG, "%s: block_table and kv_lens are required", fn);
+    if (B < 1) return fail(WLQ_ERR_INVALID_ARG, "%s: %lld tokens of 0 sequences", fn, (long long)T);
     if (!cu_q && (T != B || max_q != 1))
         return fail(WLQ_ERR_INVALID_ARG, "%s: without cu_q every sequence has one new token (T=%lld, B=%d, max_q=%d)", fn,
                     (long long)T, B, max_q);

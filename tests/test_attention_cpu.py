@@ -53,6 +53,12 @@ def test_refusals(call, code, word):
     assert call() == code and word in lib().wlq_last_error()
 
 
+def test_paged_refuses_tokens_of_no_sequence():
+    """As the prompt form does: the launch would have no CTA."""
+    for max_q in (1, 60):
+        assert paged(T=2, B=0, cu=P, max_q=max_q) == 1 and b"sequences" in lib().wlq_last_error()
+
+
 def test_nothing_to_do_is_no_error():
     assert rope(T=0) == 0 and prompt(T=0, B=0) == 0 and paged(T=0, B=0) == 0 and read(T=0, B=0) == 0
 
