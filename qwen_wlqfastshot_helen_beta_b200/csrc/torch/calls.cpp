@@ -146,6 +146,11 @@ struct Args {
     }
 };
 
+// Strides of a [tokens, heads, head size] tensor.  Those of a single token or
+// head are never used, and torch may have anything there.
+int64_t token_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+int64_t head_stride(const at::Tensor& t) { return t.size(1) > 1 ? t.stride(1) : t.size(2); }
+
 template <typename T>
 T* ptr(const at::Tensor& t) {
     return static_cast<T*>(t.data_ptr());
@@ -196,9 +201,9 @@ PyObject* rope_kv_write(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
         status("wlq_rope_kv_write",
                lib.rope_kv_write(q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr<int64_t>(pos), ptr<float>(cs),
                                  ptr<int64_t>(slots), c.k->data_ptr(), c.v->data_ptr(), c.ke, c.ve, qo.data_ptr(),
-                                 ko ? ko->data_ptr() : nullptr, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                                 v.stride(0), v.stride(1), qo.stride(0), qo.stride(1), ko ? ko->stride(0) : 0,
-                                 ko ? ko->stride(1) : 0, T, cs.size(0), c.pages, (int)Hq, (int)c.Hkv, (int)c.D,
+                                 ko ? ko->data_ptr() : nullptr, token_stride(q), head_stride(q), token_stride(k), head_stride(k),
+                                 token_stride(v), head_stride(v), token_stride(qo), head_stride(qo), ko ? token_stride(*ko) : 0,
+                                 ko ? head_stride(*ko) : 0, T, cs.size(0), c.pages, (int)Hq, (int)c.Hkv, (int)c.D,
                                  (int)cs.size(1), (int)c.ps, x.truth(12), x.dtype(),
                                  c10::cuda::getCurrentCUDAStream(x.dev.index()).stream()));
     });
@@ -240,8 +245,8 @@ PyObject* prompt_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
         const c10::cuda::CUDAGuard guard(x.dev);
         status("wlq_prompt_attention",
                lib.prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr<int32_t>(cu), o.data_ptr(),
-                                    q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                                    o.stride(0), o.stride(1), T, (int)(cu.numel() - 1), (int)Hq, (int)k.size(1), (int)D,
+                                    token_stride(q), head_stride(q), token_stride(k), head_stride(k), token_stride(v), head_stride(v),
+                                    token_stride(o), head_stride(o), T, (int)(cu.numel() - 1), (int)Hq, (int)k.size(1), (int)D,
                                     x.scale(5, D), x.truth(6), x.dtype(),
                                     c10::cuda::getCurrentCUDAStream(x.dev.index()).stream()));
     });
@@ -288,8 +293,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
         const at::Tensor ws = workspace(x.dev, stream, lib.workspace_bytes((int)Hq, (int)c.Hkv, (int)c.D, (int)max_q));
         status("wlq_paged_attention",
                lib.paged_attention(q.data_ptr(), c.k->data_ptr(), c.v->data_ptr(), c.ke, c.ve, ptr<int32_t>(table),
-                                   ptr<int32_t>(lens), cu, o.data_ptr(), q.stride(0), q.stride(1), o.stride(0),
-                                   o.stride(1), T, (int)B, (int)Hq, (int)c.Hkv, (int)c.D, (int)c.ps, c.pages,
+                                   ptr<int32_t>(lens), cu, o.data_ptr(), token_stride(q), head_stride(q), token_stride(o),
+                                   head_stride(o), T, (int)B, (int)Hq, (int)c.Hkv, (int)c.D, (int)c.ps, c.pages,
                                    table.size(1), (int)max_q, x.scale(10, c.D), x.dtype(), ws.data_ptr(),
                                    (size_t)ws.numel(), stream.stream()));
     });

@@ -348,6 +348,26 @@ def test_prompt_attention_strides_and_streams():
         R.check(buf[a:b, :, :D], *R.attention(q[a:b].double(), k[a:b].double(), v[a:b].double(), 1, 0.3))
 
 
+def test_the_stride_of_a_single_token_or_head_does_not_matter():
+    g = gen_of("single")
+    D, page = 64, 16
+    cs, zero, cu = table_of(4, D), torch.zeros(1, dtype=torch.int64, device="cuda"), torch.tensor([0, 1], dtype=torch.int32,
+                                                                                                  device="cuda")
+    base = randn(g, 1, 1, D).bfloat16()
+    odd = [base.as_strided((1, 1, D), s) for s in ((D + 1, D, 1), (D, D + 3, 1), (7, 5, 1))]
+    kc, vc = (torch.zeros(1, 1, page, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    for x in odd:
+        out = torch.full((1, 1, D), float("nan"), device="cuda", dtype=torch.bfloat16)
+        C().prompt_attention(x, x, x, cu, out.as_strided((1, 1, D), x.stride()))
+        assert torch.equal(out, base)
+        C().rope_kv_write(x, x, x, zero, cs, zero, kc, vc, out.as_strided((1, 1, D), x.stride()))
+        assert torch.equal(out, base) and torch.equal(kc[0, 0, 0], base[0, 0])  # position 0 turns by no angle
+        out.fill_(float("nan"))
+        C().paged_attention(x, kc, vc, table, lens, out.as_strided((1, 1, D), x.stride()))
+        assert torch.equal(out, base)
+
+
 # ------------------------------------------------------------------- paged ---
 
 PAGED = [  # kv_lens, new tokens, Hq, Hkv, D, page
