@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import argparse
 import json
-from typing import Optional
+from typing import Callable, Optional, Union
 
 import torch
 
@@ -23,8 +23,13 @@ from .attention import PagedKVCache, rope_table
 from .synthetic import SyntheticLayer, ceil_div, make_layer
 
 
-def _linear(layer: SyntheticLayer, x: torch.Tensor) -> torch.Tensor:
-    """One WLQ linear through the batched torch op (h = A x inside or beside it)."""
+Linear = Union[SyntheticLayer, Callable[[torch.Tensor], torch.Tensor]]
+
+
+def _linear(layer: Linear, x: torch.Tensor) -> torch.Tensor:
+    """One WLQ linear through the batched torch op (h = A x inside or beside it), or the caller's own."""
+    if callable(layer):
+        return layer(x)
     out = torch.empty((x.shape[0], layer.N), dtype=x.dtype, device=x.device)
     lut, cols, vals, fmt = layer.operands_for(x.dtype)
     torch.ops.wlq_fastShot.gemm(x, layer.q_packed, lut, out, layer.N, layer.K, 4, layer.words_per_row,
@@ -35,15 +40,20 @@ def _linear(layer: SyntheticLayer, x: torch.Tensor) -> torch.Tensor:
 
 class AttentionBlock:
     """qkv: a WLQ layer with (heads + 2 kv_heads) * head_size rows, o: one
-    with hidden_size rows; both prepacked for the activation type of `cache`."""
+    with hidden_size rows; both prepacked for the activation type of `cache`,
+    or functions of the rows, for layers loaded elsewhere (``lambda x:
+    method.apply(layer, x)``).  qkv_bias is added to the qkv rows."""
 
-    def __init__(self, qkv: SyntheticLayer, o: SyntheticLayer, heads: int, kv_heads: int, head_size: int,
-                 cache: PagedKVCache, cos_sin: torch.Tensor, interleaved: bool = False):
+    def __init__(self, qkv: Linear, o: Linear, heads: int, kv_heads: int, head_size: int, cache: PagedKVCache,
+                 cos_sin: torch.Tensor, interleaved: bool = False, qkv_bias: Optional[torch.Tensor] = None):
         self.qkv, self.o, self.cache, self.cos_sin, self.interleaved = qkv, o, cache, cos_sin, interleaved
+        self.qkv_bias = qkv_bias
         self.heads, self.kv_heads, self.head_size = heads, kv_heads, head_size
 
     def _project(self, x, positions, slots, want_k):
         qkv = _linear(self.qkv, x)
+        if self.qkv_bias is not None:
+            qkv = qkv + self.qkv_bias
         h, kv, d = self.heads, self.kv_heads, self.head_size
         q, k, v = (t.view(x.shape[0], -1, d) for t in qkv.split([h * d, kv * d, kv * d], dim=1))
         k_c, v_c, k_exp, v_exp = self.cache.tensors

@@ -813,3 +813,35 @@ def test_attention_block(bits, tol):
     for s in range(2):
         y, w = torch.cat(got[s]).float(), want[s].float()
         assert ((y - w).norm() / w.norm()).item() <= tol
+
+
+def test_attention_block_with_a_bias_and_loaded_layers():
+    """Layers given as functions, and the bias that a model's qkv projection has."""
+    from qwen_wlqfastshot_helen_beta_b200 import attention_block as B
+    hidden, heads, kv_heads, d, n = 256, 4, 2, 64, 50
+    block = B.synthetic_block(hidden, heads, kv_heads, d, pages=8, bits=16, max_position=64, seed=5)
+    g = gen_of("bias")
+    bias = randn(g, (heads + 2 * kv_heads) * d).bfloat16()
+    x = randn(g, n, hidden).bfloat16()
+    pos, cu = torch.arange(n, device="cuda"), torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    plain = block.prompt(x, pos, pos, cu)
+
+    qkv = B._linear(block.qkv, x) + bias
+    q, k, v = (t.reshape(n, -1, d).contiguous() for t in qkv.split([heads * d, kv_heads * d, kv_heads * d], 1))
+    C().rope_kv_write(q, k, v, pos, block.cos_sin, pos, block.cache.k.clone(), block.cache.v.clone(), q, k)
+    out = torch.empty_like(q)
+    C().prompt_attention(q, k, v, cu, out)
+    want = B._linear(block.o, out.view(n, -1))
+
+    biased = B.AttentionBlock(block.qkv, block.o, heads, kv_heads, d, block.cache, block.cos_sin, qkv_bias=bias)
+    assert torch.equal(biased.prompt(x, pos, pos, cu), want) and not torch.equal(want, plain)
+    calls = []
+
+    def layer(which):
+        def run(rows):
+            calls.append(rows.shape[0])
+            return B._linear(which, rows)
+        return run
+
+    own = B.AttentionBlock(layer(block.qkv), layer(block.o), heads, kv_heads, d, block.cache, block.cos_sin)
+    assert torch.equal(own.prompt(x, pos, pos, cu), plain) and calls == [n, n]
