@@ -103,29 +103,25 @@ def _register_ops():
         return None
 
 
+if "_library" not in globals():  # its ops live as long as it does: one for all reloads
+    _library = torch.library.Library("wlq_fastShot", "FRAGMENT")
+
+
 def _register_attention_ops():
     """The attention operators as torch ops (the same arguments as the _C
     functions, outputs and caches mutated in place), for graphs and
     torch.compile; eager callers that count microseconds call _C."""
 
-    @torch.library.custom_op("wlq_fastShot::rope_kv_write",
-                             mutates_args={"k_cache", "v_cache", "q_out", "k_out", "k_exp", "v_exp"})
-    def _rope(
-        q: torch.Tensor,
-        k: torch.Tensor,
-        v: torch.Tensor,
-        positions: torch.Tensor,
-        cos_sin: torch.Tensor,
-        slots: torch.Tensor,
-        k_cache: torch.Tensor,
-        v_cache: torch.Tensor,
-        q_out: torch.Tensor,
-        k_out: Optional[torch.Tensor] = None,
-        k_exp: Optional[torch.Tensor] = None,
-        v_exp: Optional[torch.Tensor] = None,
-        interleaved: bool = False,
-    ) -> None:
+    # by its schema: with optional arguments that are mutated, custom_op fails where a call leaves them out
+    _library.define("rope_kv_write(Tensor q, Tensor k, Tensor v, Tensor positions, Tensor cos_sin, Tensor slots, "
+                    "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) q_out, Tensor(d!)? k_out=None, "
+                    "Tensor(e!)? k_exp=None, Tensor(f!)? v_exp=None, bool interleaved=False) -> ()")
+
+    def _rope(q, k, v, positions, cos_sin, slots, k_cache, v_cache, q_out, k_out=None, k_exp=None, v_exp=None,
+              interleaved=False):
         _C.rope_kv_write(q, k, v, positions, cos_sin, slots, k_cache, v_cache, q_out, k_out, k_exp, v_exp, interleaved)
+
+    _library.impl("rope_kv_write", _rope, "CompositeExplicitAutograd")
 
     @torch.library.custom_op("wlq_fastShot::kv_read", mutates_args={"k_out", "v_out"})
     def _read(
@@ -171,7 +167,8 @@ def _register_attention_ops():
     def _fake(*args, **kwargs):
         return None
 
-    for op in (_rope, _read, _prompt, _paged):
+    torch.library.register_fake("wlq_fastShot::rope_kv_write", _fake, lib=_library)
+    for op in (_read, _prompt, _paged):
         op.register_fake(_fake)
 
 

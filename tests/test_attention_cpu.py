@@ -116,9 +116,15 @@ lib.define("gemv(Tensor x) -> Tensor")
 import qwen_wlqfastshot_helen_beta_b200 as pkg
 for name in ("rope_kv_write", "kv_read", "prompt_attention", "paged_attention"):
     assert hasattr(torch.ops.wlq_fastShot, name), name
-import importlib
+import gc, importlib
 importlib.reload(pkg)
-print("ok")
+gc.collect()
+x = torch.zeros(2, 4, 64)
+try:
+    torch.ops.wlq_fastShot.rope_kv_write(x, x, x, x, x, x, x, x, x)
+except RuntimeError as e:
+    assert "wlq: rope_kv_write: q must be a CUDA tensor" in str(e), e
+    print("ok")
 """
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root)

@@ -772,6 +772,51 @@ def test_torch_ops_agree_with_the_calls():
         assert torch.equal(x, y)
 
 
+def test_rope_torch_op_without_its_optional_arguments():
+    import qwen_wlqfastshot_helen_beta_b200  # noqa: F401  (registers the ops)
+    g = gen_of("bare")
+    T, Hkv, D = 5, 2, 64
+    q, k, v = (randn(g, T, Hkv, D).bfloat16() for _ in range(3))
+    cs, pos = table_of(8, D), torch.arange(T, device="cuda")
+
+    def run(fn, *more, **kw):
+        kc, vc = (torch.zeros(1, Hkv, 16, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        out = torch.empty_like(q)
+        fn(q, k, v, pos, cs, pos, kc, vc, out, *more, **kw)
+        return torch.stack((kc, vc)), out
+
+    op, want = torch.ops.wlq_fastShot.rope_kv_write, run(C().rope_kv_write)
+    for got in (run(op), run(op, None, None, None, False), run(op, k_out=None)):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    want, got = run(C().rope_kv_write, interleaved=True), run(op, interleaved=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_opcheck_of_the_torch_ops():
+    import qwen_wlqfastshot_helen_beta_b200  # noqa: F401  (registers the ops)
+    g = gen_of("opcheck")
+    T, Hq, Hkv, D, page = 20, 4, 2, 64, 16
+    q, k, v = (randn(g, T, h, D).bfloat16() for h in (Hq, Hkv, Hkv))
+    cs, pos = table_of(64, D), torch.arange(T, device="cuda")
+    table, pages = R.pages_of([T], page, g)
+    slots = table[0, pos // page].long() * page + pos % page
+    lens, cu = torch.tensor([T], dtype=torch.int32, device="cuda"), torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    ops = torch.ops.wlq_fastShot
+    for bits in (8, 16):
+        kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, torch.bfloat16, bits)
+        q2, k2, v2 = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        for op, args in ((ops.rope_kv_write, (q, k, v, pos, cs, slots, kc, vc, q2, k2, ke, ve, True)),
+                         (ops.rope_kv_write, (q, k, v, pos, cs, slots, kc, vc, q2, None, ke, ve)),
+                         (ops.rope_kv_write, (q, k, v, pos, cs, slots, kc, vc, q2) + ((None, ke, ve) if bits == 8 else ())),
+                         (ops.kv_read, (kc, vc, table, cu, k2, v2, ke, ve)),
+                         (ops.prompt_attention, (q, k, v, cu, q2, 0.2, False)),
+                         (ops.paged_attention, (q, kc, vc, table, lens, q2, cu, T, ke, ve)),
+                         (ops.paged_attention, (q[:1], kc, vc, table, lens, q2[:1], None, 1, ke, ve, 0.2))):
+            # (the schema test compares arguments with products, which torch lacks for e4m3)
+            tests = ("test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
+            torch.library.opcheck(op.default, args, test_utils=tests if bits == 8 else ("test_schema",) + tests)
+
+
 @pytest.mark.parametrize("bits,tol", [(16, 2e-2), (8, 8e-2)])
 def test_attention_block(bits, tol):
     """A prompt, a chunk and a single token through the block agree with the same tokens as one prompt: what the
