@@ -417,6 +417,30 @@ def test_paged_attention(lens, new, Hq, Hkv, D, page, dtype, bits):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,D,page", [
+    ([30000] * 4, 28, 4, 128, 16),                                    # an even cut: several segments a CTA
+    ([20000, 1, 33001, 700, 0, 64, 41003], 8, 4, 64, 64),             # the same, of very different lengths
+    ([300 + 90 * i for i in range(40)], 14, 2, 64, 32),               # more sequences than a warp's lanes, equal parts
+    ([1 + 37 * i % 500 for i in range(96)], 28, 4, 128, 16),
+    ([64 * (i % 9) for i in range(130)], 32, 8, 128, 128),            # more (sequence, kv head) pairs than CTAs
+    ([70000, 30] * 17, 16, 1, 128, 128),                              # 16 rows of one kv head, an even cut
+], ids=["long", "uneven", "40", "96", "pairs", "rows"])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_paged_attention_single_tokens_of_many_sequences(lens, Hq, Hkv, D, page, bits):
+    g = gen_of("steps", D, bits, len(lens))
+    table, pages = R.pages_of(lens, page, g)
+    kc, vc, ke, ve = make_cache(g, pages, Hkv, page, D, torch.bfloat16, bits)
+    q = randn(g, len(lens), Hq, D).bfloat16()
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, again = (torch.full_like(q, float("nan")) for _ in range(2))
+    for o in (out, again):
+        C().paged_attention(q, kc, vc, table, kv_lens, o, None, 1, ke, ve)
+    assert C().device_error() == 0 and torch.equal(out, again)
+    for i, n in enumerate(lens):
+        k, v = R.gather(kc, ke, table, i, n), R.gather(vc, ve, table, i, n)
+        R.check(out[i:i + 1], *R.attention(q[i:i + 1].double(), k, v, n, R.scale_of(D)))
+
+
 @pytest.mark.parametrize("lens,new,Hq,Hkv,D", [
     ([700] * 4, [700] * 4, 14, 2, 64),                                # row tiles of several waves, few key tiles
     ([2100, 900, 1300, 33], [250, 900, 17, 20], 28, 4, 128),          # shared and whole rows together
