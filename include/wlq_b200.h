@@ -349,7 +349,7 @@ WLQ_API int wlq_paged_attention(const void* q, const void* k_cache, const void* 
              void* workspace, size_t workspace_bytes, wlq_stream_t stream);
 
 /* Device error word of `device`: bit 0 (WLQ_DEVERR_WAIT_TIMEOUT) is set when
- * a pipeline wait inside a tensor-core GEMM kernel gave up (the kernel then
+ * a pipeline wait inside a GEMM or attention kernel gave up (the kernel then
  * abandons its tile and its output is undefined), bit 1 (WLQ_DEVERR_POSITION)
  * when wlq_rope_kv_write met a position outside its table.  Synchronous; clears the
  * word when `clear` is non-zero.  No reference counterpart: the reference

@@ -6,7 +6,12 @@ namespace wlq {
 
 namespace {
 // A sequence's new rows of one kv head fill one or two MMA column blocks of
-// the step kernel, or take the tensor-core tiles.
+// the step kernel, or take the tensor-core tiles.  With 7, 8, 14 and 16 rows the
+// step kernel is ahead by a tenth to a half (us, tiles' in brackets; 28 heads
+// over 4, D 128; 7 rows: 32 sequences of 1280 in 8 bits 25 (42), in 16 bits 34
+// (40), of 8192 73 (157) and 118 (132), one of 1500 16 (28); 14 rows: 32 (44), 37
+// (40), 92 (159), 117 (132), 24 (29)) but for 14 rows over a single long sequence
+// (16384 tokens in 16 bits: 38 (32), in 8 bits 37 (36)).
 constexpr int kFewRows = 16;
 bool few_rows(int64_t max_q, int G) { return max_q * G <= kFewRows; }
 }  // namespace

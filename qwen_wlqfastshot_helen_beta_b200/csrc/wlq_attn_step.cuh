@@ -25,11 +25,11 @@
 // the p relative to the largest score (m0), so neither the scales' spread
 // nor rows of zeros cost any precision.
 // What bounds it: long caches the memory (32 sequences of 16384 tokens, 28
-// heads over 4, D 128: 16-bit 174 us, 6.2 TB/s, 94 % of the measured copy rate;
+// heads over 4, D 128: 16-bit 180 us, 6.0 TB/s, 91 % of the measured copy rate;
 // 8-bit 104 us, 5.2 TB/s: a page of one head is then 2 KB at a random place).
 // Short ones a chain of round trips: finding the share 1.6 us, first tile 1.5,
 // a tile 0.4 to 0.75, the warps' merge and the output 1.2, joining parts 2 to 3
-// (one sequence of 64 tokens 6 us, of 1501 11 us).  Scores transposed, one
+// (one sequence of 64 tokens 8 us, of 1501 12 us).  Scores transposed, one
 // 16-key MMA per warp and tile: with two groups of 16 keys per warp the time
 // per key stayed the same.
 #pragma once
@@ -330,20 +330,20 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
         total = __reduce_add_sync(0xffffffffu, total) * p.Hkv;
         units = __reduce_add_sync(0xffffffffu, units) * p.Hkv;
         // n tiles of a (sequence, kv head) in P parts take n / P * 0.75 us and, for P > 1, 3 us + P * 0.05 us to be
-        // joined: least at P = sqrt(15 n), and worth it from 6 tiles on.  Where such parts, T tiles each, are no more
+        // joined: least at P = sqrt(15 n), and worth it from 6 tiles on.  Where such parts, `size` tiles each, are no more
         // than the CTAs, every CTA has one: a sequence's parts are alike, whatever the other sequences' lengths are.
         const int grid = (int)gridDim.x;
-        int T = 0, parts = 0, part = 0, hk = 0;
+        int size = 0, parts = 0, part = 0, hk = 0;
         if (total / grid < 16 && units <= grid) {
             const float n = (float)total / (float)max(units, 1);
-            T = n < 6.f ? 6 : max(1, (int)(n / fminf(n, sqrtf(15.f * n)) + 0.5f));
+            size = n < 6.f ? 6 : max(1, (int)(n / fminf(n, sqrtf(15.f * n)) + 0.5f));
             for (int tries = 0; tries < 6; ++tries) {
-                int sum = parts_of(tiles0, T);
+                int sum = parts_of(tiles0, size);
                 for (int b0 = 32; b0 < p.B; b0 += 32)
-                    sum += b0 + lane < p.B ? parts_of(step_seq(p, b0 + lane, RM).tiles, T) : 0;
+                    sum += b0 + lane < p.B ? parts_of(step_seq(p, b0 + lane, RM).tiles, size) : 0;
                 sum = __reduce_add_sync(0xffffffffu, sum) * p.Hkv;
                 if (sum <= grid) break;
-                T = tries == 5 ? 0 : mul_div(T, sum, grid, false) + 1;  // 0: shared out evenly after all
+                size = tries == 5 ? 0 : mul_div(size, sum, grid, false) + 1;  // 0: shared out evenly after all
             }
         }
         // Otherwise the list of tiles is cut evenly; a part is worth 4 tiles or more.
@@ -353,12 +353,12 @@ __global__ void __launch_bounds__(kStepThreads, StepPlan<D, Q8, NT>::kCtas) attn
         cuts.slack = min(max(total / cuts.G / 2, 4), 8);
         // this CTA's first tile and the next one's, each with the sequence it lies in
         int first = 0, cum0 = 0, at = total, end = total;
-        if (T) {
+        if (size) {
             at = end = 0;
             int before = 0;
             for (int b0 = 0; b0 < p.B; b0 += 32) {
                 const int tiles = b0 == 0 ? tiles0 : b0 + lane < p.B ? step_seq(p, b0 + lane, RM).tiles : 0;
-                const int ps = parts_of(tiles, T), cum = before + warp_scan(ps * p.Hkv, lane);
+                const int ps = parts_of(tiles, size), cum = before + warp_scan(ps * p.Hkv, lane);
                 const unsigned hit = __ballot_sync(0xffffffffu, (int)blockIdx.x < cum);
                 if (hit) {
                     const int l = __ffs(hit) - 1;

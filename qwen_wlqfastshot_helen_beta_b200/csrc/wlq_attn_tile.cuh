@@ -34,12 +34,15 @@
 //
 // What bounds it: the chain of one half, softmax (2000 cycles: scores read 200,
 // maximum 450, 128 exponentials a thread 1350) then P V and the next S (1024),
-// against 2048 cycles of MMAs for a pair of tiles; a pair takes 3300.  One
-// prompt of 8192 tokens, 28 heads over 4, D 128, bf16: 400 us, 1.2 PFLOP/s of
-// the causal products, 73 % of the measured cuBLAS burst rate (61 % of the
-// tensor pipe's cycles).  4 x 512 new tokens over 16384 cached ones: 342 us
-// from 16-bit pages; from 8-bit ones 424 us, where writing and reading the
-// 16-bit tiles beside the MMAs' operands takes the shared memory's rate.
+// against 2048 cycles of MMAs for a pair of tiles; a pair takes 3300 (61 % of
+// the tensor pipe's cycles).  One prompt of 8192 tokens, 28 heads over 4, D 128,
+// bf16, values spread as activations are, call after call under the power cap:
+// 454 us, 1.06 PFLOP/s of the causal products, 64 % of the measured cuBLAS
+// burst rate; normal values, a call at a time: 382 us, 1.26 PFLOP/s.  The latter
+// way 4 x 512 new tokens over 16384 cached ones take 458 us from 16-bit pages of 16
+// tokens, 441 from pages of 64, and 580 us from 8-bit ones, where writing and
+// reading the 16-bit tiles beside the MMAs' operands takes the shared memory's
+// rate (and 96 registers a thread spill 64 to 76 bytes in the softmax groups).
 // Tried: a polynomial for a part of the exponentials (1.5 % faster for
 // prompts, 4 to 15 % slower over pages); exponentials before the maximum (10 %
 // slower); references that rise by 2^8 (4 % slower than by 2^14); prompts' row
@@ -1025,7 +1028,7 @@ int launch_tile(const AttnParams& a, cudaStream_t stream) {
     tp.part = reinterpret_cast<float*>(tp.joins) + kJoinListBytes / 4;
     tp.stat = tp.part + (size_t)kPartsPerSm * tp.sms * kRows * D;
     // the most CTAs there can be work for: those beyond what there is start, search and end, 1.7 us per 148 of them
-    // (3 x 196 tokens over 3071: 12 us, 17.4 with 3 x 148 CTAs more than row tiles)
+    // (3 x 196 tokens over 3071, 10 heads over 5, D 64: 23.3 us, 28.8 with 3 x 148 CTAs more than row tiles)
     int64_t grid = (a.T / (2 * tp.nt) + a.B) * a.Hkv;
     const int64_t tiles = SRC == kPacked ? 0 : ((a.table_cols << a.log2_page) + kKeys - 1) / kKeys;
     const bool shares = tiles > kFewTiles;

@@ -13,8 +13,8 @@ namespace wlq {
 
 // Device-side failure word: set when a bounded wait gives up; read with
 // wlq_device_error().  A kernel that gives up abandons its work and returns
-// after releasing what it holds.  One word per translation unit: only the
-// GEMM's kernels (wlq_gemm.cu) wait on mbarriers.
+// after releasing what it holds.  One word per translation unit: the GEMM's
+// and the attention kernels', which all wait on mbarriers.
 static __device__ unsigned int g_wlq_device_error = 0;
 constexpr unsigned int kErrWaitTimeout = 1u;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s

@@ -1,4 +1,4 @@
-// Tensor-map (TMA descriptor) encoding for the kernels' 2-D tile copies,
+// Tensor-map (TMA descriptor) encoding for the kernels' 2-D and 3-D tile copies,
 // through the driver's cuTensorMapEncodeTiled taken from the runtime (no
 // link-time dependency on libcuda).
 #include <cuda.h>
