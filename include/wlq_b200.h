@@ -339,7 +339,7 @@ WLQ_API int wlq_prompt_attention(const void* q, const void* k, const void* v, co
  * its first WLQ_ATTENTION_ZERO_BYTES zero before the first use and left zero
  * by every call, one that gave up a wait included) joins the parts of sequences that several CTAs share; calls
  * that share one must not overlap.  B * Hkv is at most
- * WLQ_ATTENTION_ZERO_BYTES / 4.  Results do not depend on timing. */
+ * WLQ_ATTENTION_ZERO_BYTES / 4, and B * Hkv * table_cols * page_size / 64 below 2^31.  Results do not depend on timing. */
 #define WLQ_ATTENTION_ZERO_BYTES (256u * 1024u)
 WLQ_API size_t wlq_paged_attention_workspace_bytes(int Hq, int Hkv, int D, int max_q);
 WLQ_API int wlq_paged_attention(const void* q, const void* k_cache, const void* v_cache, const uint8_t* k_exp,

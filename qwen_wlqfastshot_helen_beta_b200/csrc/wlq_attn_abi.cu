@@ -191,6 +191,10 @@ int wlq_paged_attention(const void* q, const void* k_cache, const void* v_cache,
     if ((int64_t)B * Hkv > (int64_t)WLQ_ATTENTION_ZERO_BYTES / 4)
         return fail(WLQ_ERR_UNSUPPORTED, "%s: %d sequences of %d kv heads (at most %u pairs)", fn, B, Hkv,
                     WLQ_ATTENTION_ZERO_BYTES / 4);
+    // the few-row kernel counts the key tiles of all sequences and kv heads in 31 bits
+    if ((int64_t)B * Hkv * ((table_cols * page_size + 63) / 64) > 0x7fffffff)
+        return fail(WLQ_ERR_UNSUPPORTED, "%s: too many tokens for one call (%d sequences of up to %lld, %d kv heads)", fn, B,
+                    (long long)(table_cols * page_size), Hkv);
     if (k_exp && (!aligned16(k_exp) || !aligned16(v_exp)))
         return fail(WLQ_ERR_ALIGNMENT, "%s: k_exp and v_exp must be 16-byte aligned", fn);
     if ((rc = require_sm100())) return rc;

@@ -59,6 +59,14 @@ def test_paged_refuses_tokens_of_no_sequence():
         assert paged(T=2, B=0, cu=P, max_q=max_q) == 1 and b"sequences" in lib().wlq_last_error()
 
 
+def test_paged_refuses_more_key_tiles_than_it_can_count():
+    """The few-row kernel's list of tiles (64 keys of a kv head) is counted in 31 bits."""
+    assert paged(T=32768, B=32768, page=128, cols=1 << 17) == 2 and b"too many" in lib().wlq_last_error()  # 2^34 tiles
+    assert paged(T=32768, B=32768, page=128, cols=1 << 14) == 2 and b"too many" in lib().wlq_last_error()  # 2^31
+    paged(T=32768, B=32768, page=128, cols=(1 << 14) - 1)
+    assert b"too many" not in lib().wlq_last_error()
+
+
 def test_nothing_to_do_is_no_error():
     assert rope(T=0) == 0 and prompt(T=0, B=0) == 0 and paged(T=0, B=0) == 0 and read(T=0, B=0) == 0
 
