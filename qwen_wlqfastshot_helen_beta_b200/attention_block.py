@@ -103,7 +103,7 @@ def main(argv=None):
     a = ap.parse_args(argv)
     dev, page = torch.device("cuda"), 16
     per = ceil_div(a.prompt + a.gen + 1, page)
-    block = synthetic_block(pages=a.batch * per, page_size=page, bits=a.bits)
+    block = synthetic_block(pages=a.batch * per, page_size=page, bits=a.bits, max_position=max(32768, per * page))
     table = torch.arange(a.batch * per, dtype=torch.int32, device=dev).view(a.batch, per)
     seq = torch.arange(a.batch, device=dev)
 

@@ -914,3 +914,12 @@ def test_attention_block_with_a_bias_and_loaded_layers():
 
     own = B.AttentionBlock(layer(block.qkv), layer(block.o), heads, kv_heads, d, block.cache, block.cos_sin)
     assert torch.equal(own.prompt(x, pos, pos, cu), plain) and calls == [n, n]
+
+
+def test_attention_block_command_with_a_long_prompt(capsys):
+    """More positions than the block's default table holds."""
+    import json
+    from qwen_wlqfastshot_helen_beta_b200 import attention_block as B
+    B.main(["--batch", "1", "--prompt", "33000", "--gen", "2"])
+    line = json.loads(capsys.readouterr().out)
+    assert C().device_error() == 0 and line["finite"] and line["prompt_ms"] > 0 and line["step_us"] > 0
