@@ -303,9 +303,13 @@ PyObject* paged_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
 // The kept workspaces, and their end: the next calls begin with fresh ones.
 // (Memory goes back to its stream's pool, behind the calls that still use it.)
 PyObject* kept_workspaces(PyObject*, PyObject*) {
-    const std::lock_guard<std::mutex> hold(lock);
+    std::map<std::pair<int, cudaStream_t>, at::Tensor> all;
+    {
+        const std::lock_guard<std::mutex> hold(lock);  // (not while Python runs)
+        all = *kept;
+    }
     PyObject* list = PyList_New(0);
-    for (const auto& entry : *kept) {
+    for (const auto& entry : all) {
         PyObject* t = list ? THPVariable_Wrap(entry.second) : nullptr;
         if (!t || PyList_Append(list, t) < 0) Py_CLEAR(list);
         Py_XDECREF(t);
