@@ -14,7 +14,7 @@
 // Both kernels are HBM-bound: every value is read once and written once.
 // Measured, 28 heads over 4, D 128, 8-bit cache: the write of 32 prompts of 1024
 // tokens (571 MB) 106 us, 5.4 TB/s, 82 % of the measured copy rate, one step of
-// 32 tokens 3.0 us in a graph; the read-back of 180554 tokens (556 MB) 93 us, 6.0 TB/s, 91 %.
+// 32 tokens 3.0 us in a graph; the read-back of 180554 tokens (556 MB) 90 us, 6.2 TB/s, 94 %.
 #include <cuda_fp8.h>
 
 #include "wlq_attn.cuh"
@@ -349,8 +349,10 @@ int launch_rope_kv_write(RopeParams& p, bool f16, bool quant, cudaStream_t strea
 }
 
 int launch_kv_read(KvReadParams& p, bool f16, bool quant, cudaStream_t stream) {
-    // a few tokens per CTA until every SM has some
-    p.tokens = p.T >= (int64_t)device_sm_count() * 2 * kReadTokens ? kReadTokens : 8;
+    // A CTA takes the tokens of one round of its threads (four items each); few rows, 8 tokens, which start more CTAs.  4
+    // heads of 128, 8 bits, in a graph: 500 rows 2.7 us with 8 tokens and 2.8 with 32, 1500 rows 3.7 and 3.1, 16000 17.4 and
+    // 7.8, 100000 104 and 50 (51 with 64); 8 heads 115 with 8, 96 with 16, 100 with 64; 2 heads of 64 41 with 8, 15 with 64.
+    p.tokens = p.T < 1000 ? 8 : std::clamp(4 * kReadThreads / (p.Hkv * (p.D >> 4)), 8, kReadTokens);
     p.per_magic = magic_u32((uint32_t)(p.Hkv * (p.D >> 4)));
     p.chunk_magic = magic_u32((uint32_t)(p.D >> 4));
     const dim3 grid((unsigned)((p.T + p.tokens - 1) / p.tokens), 2);
