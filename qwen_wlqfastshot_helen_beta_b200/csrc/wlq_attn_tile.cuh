@@ -153,7 +153,12 @@ constexpr int kLanesSeqs = 32;  // sequences whose split is searched for
 // tiles is shared by several CTAs.  Up to 32 sequences: of 16 sizes the one
 // with the least waves of CTAs times a part's duration (its tiles, about 3
 // more for starting and ending, and once 6 for joining the parts).  More
-// sequences: an even share of all tiles.
+// sequences: an even share of all tiles.  The search's time, the even share's in
+// brackets (us, 28 heads over 4, D 128, 16-bit): 8 x 40 tokens over 16384 124 (143),
+// 1 x 512 over 16384 133 (146), 4 x 64 over 8192 57 (60), 4 x 128 over 4096 51 (52); but
+// where one wave of CTAs does all, 1 x 64 over 16384 36 (28), 1 x 64 over 65536 87 (65), 3
+// x 196 over 3071 43 (36): the host launches up to four CTAs an SM for the search, and
+// those without work wait for an SM until the others end.
 __device__ __forceinline__ int tiles_per_part(const AttnParams& p, int nt, int sms, int lane) {
     if (p.B > kLanesSeqs) {
         int64_t w = 0;
@@ -237,7 +242,11 @@ __device__ __forceinline__ bool find_unit(const AttnParams& p, int nt, int sms, 
 }
 
 // The lists of joins, written by one warp of CTA 0: those of up to
-// kJoinWarps parts from the front, the others from the back.
+// kJoinWarps parts, which take a warp a piece, from the front, the others, which
+// take a block a piece, from the back.  Chunk and join (us, all joins by blocks
+// in brackets): 4 x 128 over 4096 51 (64), 3 x 196 over 3071 43 (58), 8 x 40 over 16384 125
+// (134), 1 x 64 over 4096, 8 parts, 23.5 (21.8); with all by warps 1 x 64 over 16384 41
+// instead of 36, over 65536 96 instead of 87.
 constexpr int kJoinWarps = 8;
 constexpr int kMaxJoins = (kJoinListBytes - 8) / (int)sizeof(Join);
 

@@ -329,7 +329,8 @@ int launch_rope_kv_write(RopeParams& p, bool f16, bool quant, cudaStream_t strea
     p.lanes_per_row = 1;
     while (p.lanes_per_row * 16 < p.D) p.lanes_per_row <<= 1;
     const int steps = (p.Hq + 2 * p.Hkv + 32 / p.lanes_per_row - 1) / (32 / p.lanes_per_row);
-    // enough warps for 16 per SM before a warp walks several steps
+    // enough warps for 16 per SM before a warp walks several steps (28 heads over 4, D 128, 8-bit, in a graph: 1 to 32
+    // tokens 2.7 us, 5.2 with a warp a token; 300 tokens 4.5 and 5.5; 4000 the same)
     const int64_t want = (int64_t)device_sm_count() * 16;
     const int64_t resident = (int64_t)device_sm_count() * kRopeCtas;
     p.parts = (int)std::min(std::min<int64_t>(steps, resident), std::max<int64_t>(1, (want + p.T - 1) / p.T));
